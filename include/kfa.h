@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-enum kfa_dtype { KFA_F16 = 0, KFA_BF16 = 1, KFA_F32 = 2, KFA_BOOL = 3, KFA_I32 = 4 };
+enum kfa_dtype { KFA_F16 = 0, KFA_BF16 = 1, KFA_F32 = 2, KFA_BOOL = 3, KFA_I32 = 4, KFA_U8 = 5 };
 
 /* Non-owning tensor description; strides are in elements.  The reference passes
  * the same information as non-owning DLTensor views (native.cpp:205-210). */
@@ -228,6 +228,28 @@ KFA_API int kfa_backward_partial(const kfa_tensor* q, const kfa_tensor* k, const
  */
 KFA_API int kfa_merge_splits(kfa_tensor* out, kfa_tensor* maximum, kfa_tensor* logsum, const kfa_tensor* part_out,
                      const kfa_tensor* part_maximum, const kfa_tensor* part_logsum, float scale, void* stream);
+
+/*
+ * Causal attention with a sliding window and sinks (no counterpart in the reference).  Query row r of batch b stands
+ * at key position pos = start_b + r and sees key c iff c <= pos and (c > pos - window or c < sinks).  start_b is
+ * `start` for every batch when `starts` is NULL, else starts[b] (int32 [B] in device memory, read by the kernels: the
+ * call can be captured in a graph and replayed with new positions).  Any position is allowed: a row that sees no key
+ * yields out = 0, maximum = -inf, logsum = 0.  window >= 1, sinks >= 0, any other operand as for kfa_forward; the
+ * statistics may both be NULL.
+ *
+ * kfa_window_backward takes the forward's out/maximum/logsum and one `start` >= 0 for all batches; `workspace` holds
+ * kfa_window_backward_workspace_bytes() bytes, 256-byte aligned.  Every gradient has one owner and a fixed order of
+ * additions.
+ */
+KFA_API int kfa_window_forward(const kfa_tensor* q, const kfa_tensor* k, const kfa_tensor* v, const kfa_tensor* starts,
+                       kfa_tensor* out, kfa_tensor* maximum, kfa_tensor* logsum, int64_t start, int64_t window,
+                       int64_t sinks, float scale, void* stream);
+KFA_API size_t kfa_window_backward_workspace_bytes(const kfa_tensor* q, const kfa_tensor* k, int64_t start,
+                       int64_t window, int64_t sinks);
+KFA_API int kfa_window_backward(const kfa_tensor* q, const kfa_tensor* k, const kfa_tensor* v, const kfa_tensor* out,
+                       const kfa_tensor* maximum, const kfa_tensor* logsum, const kfa_tensor* dout, kfa_tensor* dq,
+                       kfa_tensor* dk, kfa_tensor* dv, void* workspace, size_t workspace_bytes, int64_t start,
+                       int64_t window, int64_t sinks, float scale, void* stream);
 
 /* Number of kernel variants configured so far / forget them.  Replace `cache_size`
  * and `clear_cache` (native.cpp:1055-1065). */

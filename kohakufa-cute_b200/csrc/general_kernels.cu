@@ -19,6 +19,7 @@
 #include "kfa_common.cuh"
 #include "row_access.cuh"
 #include "launchers.h"
+#include "window.cuh"
 
 namespace kfa {
 
@@ -66,8 +67,13 @@ __global__ void __launch_bounds__(kWarps * 32) general_forward(AttnParams p) {
         for (int i = 0; i < DI2; ++i) acc[r][i][0] = acc[r][i][1] = 0.f;
     }
     const int last_row = min(row0 + R, p.Sq) - 1;
-    const int kend = p.causal ? min(p.Sk, last_row + 1) : p.Sk;
+    const bool windowed = p.window > 0;
+    const int64_t start = windowed ? window_start(p, b) : 0;
+    const int first_lo = windowed ? window_span(start, row0, p.window, p.Sk).lo : 0;
+    const int kend = windowed ? window_span(start, last_row, p.window, p.Sk).hi
+                              : (p.causal ? min(p.Sk, last_row + 1) : p.Sk);
     for (int k0 = 0; k0 < kend; k0 += 32) {
+        if (windowed && k0 >= p.sinks && k0 + 32 <= first_lo) continue;  // between the sinks and the window
         if (p.has_mask && (k0 & 63) == 0) {
             // skip a 64-key block that the tile table marks hidden for every row of this warp
             int tq0 = row0 >> 6, tq1 = last_row >> 6;
@@ -99,6 +105,7 @@ __global__ void __launch_bounds__(kWarps * 32) general_forward(AttnParams p) {
         for (int r = 0; r < R; ++r) {
             const int row = row0 + r;
             bool vis = in_range && row < p.Sq && (!p.causal || c <= row);
+            if (windowed) vis = vis && window_sees(window_span(start, row, p.window, p.Sk), p.sinks, c);
             if (vis && p.has_mask) vis = mask_bit(p, b, h, row, c);
             const float sp = vis ? s[r] * sign : -INFINITY;
             const float m_new = fmaxf(m[r], warp_max(sp));
@@ -218,8 +225,13 @@ __global__ void __launch_bounds__(kWarps * 32) general_backward_q(AttnParams p) 
         for (int i = 0; i < DI2; ++i) acc[r][i][0] = acc[r][i][1] = 0.f;
     }
     const int last_row = min(row0 + R, p.Sq) - 1;
-    const int kend = p.causal ? min(p.Sk, last_row + 1) : p.Sk;
+    const bool windowed = p.window > 0;
+    const int64_t start = windowed ? window_start(p, b) : 0;
+    const int first_lo = windowed ? window_span(start, row0, p.window, p.Sk).lo : 0;
+    const int kend = windowed ? window_span(start, last_row, p.window, p.Sk).hi
+                              : (p.causal ? min(p.Sk, last_row + 1) : p.Sk);
     for (int k0 = 0; k0 < kend; k0 += 32) {
+        if (windowed && k0 >= p.sinks && k0 + 32 <= first_lo) continue;  // between the sinks and the window
         if (p.has_mask && (k0 & 63) == 0) {
             int tq0 = row0 >> 6, tq1 = last_row >> 6;
             bool any = tile_state(p, b, h, tq0, k0 >> 6) != 0 || tile_state(p, b, h, tq1, k0 >> 6) != 0;
@@ -253,6 +265,7 @@ __global__ void __launch_bounds__(kWarps * 32) general_backward_q(AttnParams p) 
         for (int r = 0; r < R; ++r) {
             const int row = row0 + r;
             bool vis = in_range && row < p.Sq && (!p.causal || c <= row);
+            if (windowed) vis = vis && window_sees(window_span(start, row, p.window, p.Sk), p.sinks, c);
             if (vis && p.has_mask) vis = mask_bit(p, b, h, row, c);
             const float pr = vis ? fast_ex2((s[r] * sign - mx[r]) * c2 - ls[r]) : 0.f;
             ds[r] = round_low<T>(round_low<T>(pr) * (dp[r] - dl[r]));
@@ -324,13 +337,21 @@ __global__ void __launch_bounds__(kWarps * 32) general_backward_kv(AttnParams p)
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int i = 0; i < DI2; ++i) ak[r][i][0] = ak[r][i][1] = av[r][i][0] = av[r][i][1] = 0.f;
-    const int q_begin = p.causal ? (key0 & ~31) : 0;  // causal: only queries r >= key see the key
+    int q_begin = p.causal ? (key0 & ~31) : 0;  // causal: only queries r >= key see the key
+    int q_end = p.Sq;
+    const bool windowed = p.window > 0;
+    const int64_t start = windowed ? window_start(p, b) : 0;
+    if (windowed) {  // rows at positions key .. key + window - 1, or any later row where the key is a sink
+        const int64_t first = key0 - start, last = min(key0 + R, p.Sk) - 1 + p.window - start;
+        q_begin = (int)(first < 0 ? 0 : (first > p.Sq ? p.Sq : first)) & ~31;
+        if (key0 >= p.sinks) q_end = (int)(last < 0 ? 0 : (last > p.Sq ? p.Sq : last));
+    }
     for (int g = 0; g < p.group; ++g) {
         const int h = kvh * p.group + g;
         const T* qb = reinterpret_cast<const T*>(p.q) + (int64_t)b * p.qs[0] + (int64_t)h * p.qs[1];
         const T* gb = reinterpret_cast<const T*>(p.dout) + (int64_t)b * p.gs[0] + (int64_t)h * p.gs[1];
         const int64_t sbase = ((int64_t)b * p.Hq + h) * p.Sq;
-        for (int q0 = q_begin; q0 < p.Sq; q0 += 32) {
+        for (int q0 = q_begin; q0 < q_end; q0 += 32) {
             if (p.has_mask && (q0 & 63) == 0) {
                 int tk0 = key0 >> 6, tk1 = (min(key0 + R, p.Sk) - 1) >> 6;
                 bool any = tile_state(p, b, h, q0 >> 6, tk0) != 0 || tile_state(p, b, h, q0 >> 6, tk1) != 0;
@@ -338,6 +359,7 @@ __global__ void __launch_bounds__(kWarps * 32) general_backward_kv(AttnParams p)
             }
             const int row = q0 + lane;
             const bool in_range = row < p.Sq;
+            const WindowSpan span = windowed ? window_span(start, row, p.window, p.Sk) : WindowSpan{0, 0};
             float s[R], dp[R];
 #pragma unroll
             for (int r = 0; r < R; ++r) s[r] = dp[r] = 0.f;
@@ -368,6 +390,7 @@ __global__ void __launch_bounds__(kWarps * 32) general_backward_kv(AttnParams p)
             for (int r = 0; r < R; ++r) {
                 const int c = key0 + r;
                 bool vis = in_range && c < p.Sk && (!p.causal || c <= row);
+                if (windowed) vis = vis && window_sees(span, p.sinks, c);
                 if (vis && p.has_mask) vis = mask_bit(p, b, h, row, c);
                 const float pr = vis ? fast_ex2((s[r] * sign - mx) * c2 - ls) : 0.f;
                 pl[r] = round_low<T>(pr);

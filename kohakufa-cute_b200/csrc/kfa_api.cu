@@ -1056,6 +1056,105 @@ int kfa_neighborhood_backward(const kfa_tensor* q, const kfa_tensor* k, const kf
     return 0;
 }
 
+}  // extern "C"
+
+namespace {
+
+// The window arguments of a call: positions per batch (device) or one position for all.
+int fill_window(kfa::AttnParams& p, const kfa_tensor* starts, int64_t start, int64_t window, int64_t sinks) {
+    if (window < 1 || sinks < 0)
+        return fail(KFA_INVALID_ARGUMENT, "window attention requires window >= 1 and sinks >= 0");
+    if (starts && (!starts->data || starts->dtype != KFA_I32 || starts->ndim != 1 || starts->sizes[0] != p.B ||
+                   (p.B > 1 && starts->strides[0] != 1)))
+        return fail(KFA_INVALID_ARGUMENT, "window attention requires contiguous int32 [batch] query positions");
+    if (!starts && (start > INT32_MAX || start < INT32_MIN))
+        return fail(KFA_INVALID_ARGUMENT, "window attention: the query position exceeds 32 bits");
+    // positions stay below 2^32 + 2^31: a longer window is the same as none
+    p.window = std::min<int64_t>(window, int64_t(1) << 40);
+    p.sinks = (int)std::min<int64_t>(sinks, p.Sk);
+    p.start = start;
+    p.starts = starts ? static_cast<const int32_t*>(starts->data) : nullptr;
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int kfa_window_forward(const kfa_tensor* q, const kfa_tensor* k, const kfa_tensor* v, const kfa_tensor* starts,
+                       kfa_tensor* out, kfa_tensor* maximum, kfa_tensor* logsum, int64_t start, int64_t window,
+                       int64_t sinks, float scale, void* stream) {
+    if (int e = check_device_ok()) return e;
+    if (int e = check_qkv(q, k, v)) return e;
+    kfa::AttnParams p;
+    if (int e = fill_common(p, q, k, v, nullptr, scale, 0, static_cast<cudaStream_t>(stream))) return e;
+    if (int e = fill_window(p, starts, start, window, sinks)) return e;
+    if (int e = check_like(out, q, "out")) return e;
+    const bool keep_statistics = maximum != nullptr || logsum != nullptr;
+    if (keep_statistics && (!contiguous3(maximum, p.B, p.Hq, p.Sq) || !contiguous3(logsum, p.B, p.Hq, p.Sq)))
+        return fail(KFA_INVALID_ARGUMENT, "maximum/logsum must be contiguous float32 [B,Hq,Sq] (or both NULL)");
+    p.out = out->data;
+    copy4(p.os, out->strides);
+    p.maximum = keep_statistics ? static_cast<float*>(maximum->data) : nullptr;
+    p.logsum = keep_statistics ? static_cast<float*>(logsum->data) : nullptr;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool bf16 = q->dtype == KFA_BF16;
+    cudaError_t ce = timed("general_forward", st, [&] { return kfa::launch_general_forward(p, bf16, st); });
+    if (ce != cudaSuccess) return cuda_fail(ce, "window forward launch");
+    return 0;
+}
+
+size_t kfa_window_backward_workspace_bytes(const kfa_tensor* q, const kfa_tensor* k, int64_t start, int64_t window,
+                                           int64_t sinks) {
+    (void)k, (void)start, (void)window, (void)sinks;
+    if (!q || q->ndim != 4) return 0;
+    return delta_bytes(q);
+}
+
+int kfa_window_backward(const kfa_tensor* q, const kfa_tensor* k, const kfa_tensor* v, const kfa_tensor* out,
+                        const kfa_tensor* maximum, const kfa_tensor* logsum, const kfa_tensor* dout, kfa_tensor* dq,
+                        kfa_tensor* dk, kfa_tensor* dv, void* workspace, size_t workspace_bytes, int64_t start,
+                        int64_t window, int64_t sinks, float scale, void* stream) {
+    if (int e = check_device_ok()) return e;
+    if (int e = check_qkv(q, k, v)) return e;
+    kfa::AttnParams p;
+    if (int e = fill_common(p, q, k, v, nullptr, scale, 0, static_cast<cudaStream_t>(stream))) return e;
+    if (start < 0) return fail(KFA_INVALID_ARGUMENT, "window backward requires a query position >= 0");
+    if (int e = fill_window(p, nullptr, start, window, sinks)) return e;
+    if (int e = check_like(out, q, "out")) return e;
+    if (int e = check_like(dout, q, "dout")) return e;
+    if (int e = check_like(dq, q, "dq")) return e;
+    if (int e = check_like(dk, k, "dk")) return e;
+    if (int e = check_like(dv, v, "dv")) return e;
+    if (!contiguous3(maximum, p.B, p.Hq, p.Sq) || !contiguous3(logsum, p.B, p.Hq, p.Sq))
+        return fail(KFA_INVALID_ARGUMENT, "maximum/logsum must be contiguous float32 [B,Hq,Sq]");
+    if (!workspace || workspace_bytes < kfa_window_backward_workspace_bytes(q, k, start, window, sinks) ||
+        reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
+        return fail(KFA_INVALID_ARGUMENT, "window backward workspace too small or not 256-byte aligned");
+    p.out = const_cast<void*>(out->data);
+    copy4(p.os, out->strides);
+    p.maximum = static_cast<float*>(maximum->data);
+    p.logsum = static_cast<float*>(logsum->data);
+    p.dout = dout->data;
+    copy4(p.gs, dout->strides);
+    p.delta = static_cast<float*>(workspace);
+    p.dq = dq->data;
+    copy4(p.dqs, dq->strides);
+    p.dk = dk->data;
+    copy4(p.dks, dk->strides);
+    p.dv = dv->data;
+    copy4(p.dvs, dv->strides);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool bf16 = q->dtype == KFA_BF16;
+    cudaError_t ce = timed("output_delta", st, [&] { return kfa::launch_output_delta(p, bf16, st); });
+    if (ce != cudaSuccess) return cuda_fail(ce, "output_delta launch");
+    ce = timed("general_backward_q", st, [&] { return kfa::launch_general_backward(p, bf16, 0, st); });
+    if (ce != cudaSuccess) return cuda_fail(ce, "window backward (dQ) launch");
+    ce = timed("general_backward_kv", st, [&] { return kfa::launch_general_backward(p, bf16, 1, st); });
+    if (ce != cudaSuccess) return cuda_fail(ce, "window backward (dK/dV) launch");
+    return 0;
+}
+
 int kfa_merge_splits(kfa_tensor* out, kfa_tensor* maximum, kfa_tensor* logsum, const kfa_tensor* part_out,
                      const kfa_tensor* part_maximum, const kfa_tensor* part_logsum, float scale, void* stream) {
     if (!out || !out->data || out->ndim != 4 || !is_half_type(out))

@@ -62,6 +62,12 @@ struct AttnParams {
     float* dq_acc;
     int running;
     int grad_f32;
+    // Sliding window with sinks (window > 0; see window.cuh): row r of batch b stands at key position
+    // start_b + r, start_b = starts[b] where `starts` is given (device memory), `start` otherwise.
+    int64_t window;
+    int sinks;
+    int64_t start;
+    const int32_t* starts;
     int* status;      // device-visible status word (mapped host memory)
     int* abort_flag;  // device memory: set by the first CTA whose bounded wait gives up; later CTAs skip their work
 };

@@ -11,6 +11,7 @@ from .api import (
     neighborhood_attention,
     neighborhood_attention_3d,
     scaled_dot_product_attention,
+    sliding_window_attention,
 )
 
 __version__ = "0.1.0"
@@ -20,4 +21,5 @@ __all__ = [
     "automatic_scaled_dot_product_attention",
     "neighborhood_attention",
     "neighborhood_attention_3d",
+    "sliding_window_attention",
 ]

@@ -126,6 +126,46 @@ def automatic_scaled_dot_product_attention(
     return _native_sdpa(query, key, value, attn_mask, dropout_p, is_causal, scale=scale, enable_gqa=enable_gqa)
 
 
+def _window_arguments(name, batch, device, window, sinks, query_start):
+    """``(starts, start)`` of checked window arguments: a tensor of positions per sequence, or ``None`` and one int."""
+    if not isinstance(window, int) or isinstance(window, bool) or window < 1:
+        raise ValueError(f"{name}: window must be a positive integer.")
+    if not isinstance(sinks, int) or isinstance(sinks, bool) or sinks < 0:
+        raise ValueError(f"{name}: sinks must be a nonnegative integer.")
+    if isinstance(query_start, torch.Tensor):
+        if query_start.dtype != torch.int32 or query_start.shape != (batch,) or query_start.device != device:
+            raise ValueError(f"{name}: a query_start tensor must be int32 [batch] on the Q device.")
+        return query_start.contiguous(), 0
+    if not isinstance(query_start, int) or isinstance(query_start, bool) or not 0 <= query_start < 2**31:
+        raise ValueError(f"{name}: query_start must be a nonnegative 32-bit integer or an int32 [batch] tensor.")
+    return None, query_start
+
+
+def _resolved_scale(name, scale, head_dim):
+    scale = head_dim**-0.5 if scale is None else float(scale)
+    if not isfinite(scale) or abs(scale) > torch.finfo(torch.float32).max:
+        raise ValueError(f"{name}: scale must be a finite FP32 number.")
+    return scale
+
+
+def sliding_window_attention(q, k, v, *, window, sinks=0, query_start=0, scale=None):
+    """Causal attention with a sliding window and a few first tokens (sinks) that stay visible.
+
+    Q is ``[B, Hq, Sq, D]``, K/V are ``[B, Hkv, Sk, D]`` with ``Hq % Hkv == 0``.  Query row ``r`` stands at position
+    ``p = query_start + r`` of its key sequence and sees key ``c`` iff ``c <= p`` and (``c > p - window`` or
+    ``c < sinks``); a row that sees no key is zero.  ``query_start`` is an int (0: queries and keys start together, as
+    in training), or an int32 ``[B]`` CUDA tensor with one position per sequence, read by the kernels (a captured
+    graph can be replayed with new positions; any value is allowed, keys behind a sequence's last position may hold
+    anything).  Differentiable with respect to Q, K and V when ``query_start`` is an int.
+    """
+    _check_arguments(q, k, v, None, 0.0, False, True)
+    starts, start = _window_arguments("sliding_window_attention", q.shape[0], q.device, window, sinks, query_start)
+    scale = _resolved_scale("sliding_window_attention", scale, q.shape[-1])
+    from . import window_ops
+
+    return window_ops.attention(q, k, v, starts, start, window, sinks, scale)
+
+
 def neighborhood_attention(q, k, v, *, spatial_shape, window_size, scale=None):
     """Non-causal 2-D/3-D neighbourhood attention, stride and dilation one, head dim 64.
 

@@ -18,13 +18,14 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIBRARY_PATH = os.path.join(_HERE, "libkfa.so")
 
-KFA_F16, KFA_BF16, KFA_F32, KFA_BOOL, KFA_I32 = range(5)
+KFA_F16, KFA_BF16, KFA_F32, KFA_BOOL, KFA_I32, KFA_U8 = range(6)
 _DTYPES = {
     torch.float16: KFA_F16,
     torch.bfloat16: KFA_BF16,
     torch.float32: KFA_F32,
     torch.bool: KFA_BOOL,
     torch.int32: KFA_I32,
+    torch.uint8: KFA_U8,
 }
 
 
@@ -69,6 +70,10 @@ SIGNATURES = {
                                                               _I64P, ctypes.c_float, ctypes.c_void_p]),
     "kfa_merge_partial": (ctypes.c_int, [_TP] * 6 + [ctypes.c_float, ctypes.c_void_p]),
     "kfa_merge_splits": (ctypes.c_int, [_TP] * 6 + [ctypes.c_float, ctypes.c_void_p]),
+    "kfa_window_forward": (ctypes.c_int, [_TP] * 7 + [ctypes.c_int64] * 3 + [ctypes.c_float, ctypes.c_void_p]),
+    "kfa_window_backward_workspace_bytes": (ctypes.c_size_t, [_TP, _TP] + [ctypes.c_int64] * 3),
+    "kfa_window_backward": (ctypes.c_int, [_TP] * 10 + [ctypes.c_void_p, ctypes.c_size_t] + [ctypes.c_int64] * 3 +
+                            [ctypes.c_float, ctypes.c_void_p]),
     "kfa_cache_size": (ctypes.c_int, []),
     "kfa_clear_cache": (None, []),
     "kfa_launch_count": (ctypes.c_uint64, []),
@@ -423,6 +428,47 @@ def neighborhood_backward(q, k, v, out, maximum, logsum, dout, spatial, window, 
         _check(lib.kfa_neighborhood_backward(*[_ref(r) for r in records], ctypes.c_void_p(workspace.data_ptr()), need,
                                              _int64_array(spatial), len(spatial), _int64_array(window), float(scale),
                                              _stream(q.device)))
+    return dq, dk, dv
+
+
+def window_forward(q, k, v, starts, start, window, sinks, scale, statistics=True):
+    """(out, maximum, logsum) of causal attention with a sliding window and sinks (``kfa_window_forward``);
+    ``starts`` is an int32 ``[B]`` tensor of query positions or ``None`` (then ``start`` holds for every batch).
+    With ``statistics=False`` the two row statistics come back as ``None``."""
+    lib = library()
+    q, k, v = _plain(q), _plain(k), _plain(v)
+    originals = (q, k, v)
+    (q, k, v), _ = _for_tensor_cores([q, k, v])
+    if any(a is not b for a, b in zip((q, k, v), originals)):
+        out, maximum, logsum = window_forward(q, k, v, starts, start, window, sinks, scale, statistics)
+        return _like(originals[0], out), maximum, logsum
+    with torch.cuda.device(q.device):
+        out = torch.empty_like(q)
+        maximum = torch.empty(q.shape[:-1], device=q.device, dtype=torch.float32) if statistics else None
+        logsum = torch.empty_like(maximum) if statistics else None
+        records = [describe(t) for t in (q, k, v, starts, out, maximum, logsum)]
+        _check(lib.kfa_window_forward(*[_ref(r) for r in records], start, window, sinks, float(scale),
+                                      _stream(q.device)))
+    return out, maximum, logsum
+
+
+def window_backward(q, k, v, out, maximum, logsum, dout, start, window, sinks, scale):
+    """(dq, dk, dv) of ``window_forward`` (``kfa_window_backward``)."""
+    lib = library()
+    q, k, v, out, dout = (_plain(t) for t in (q, k, v, out, dout))
+    originals = (q, k, v)
+    (q, k, v, dout, out), _ = _for_tensor_cores([q, k, v, dout, out])
+    if any(a is not b for a, b in zip((q, k, v), originals)):
+        grads = window_backward(q, k, v, out, maximum, logsum, dout, start, window, sinks, scale)
+        return tuple(_like(o, g) for o, g in zip(originals, grads))
+    with torch.cuda.device(q.device):
+        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        rq, rk = describe(q), describe(k)
+        need = lib.kfa_window_backward_workspace_bytes(_ref(rq), _ref(rk), start, window, sinks)
+        workspace = torch.empty(need, device=q.device, dtype=torch.uint8)
+        records = [rq, rk] + [describe(t) for t in (v, out, maximum, logsum, dout, dq, dk, dv)]
+        _check(lib.kfa_window_backward(*[_ref(r) for r in records], ctypes.c_void_p(workspace.data_ptr()), need, start,
+                                       window, sinks, float(scale), _stream(q.device)))
     return dq, dk, dv
 
 

@@ -1,0 +1,264 @@
+"""Causal attention with a sliding window and sinks against the FP64 oracle: gradients, positions, positions per
+sequence, hidden rows, layouts, graphs, streams, the compiled route and the refusals."""
+
+import pytest
+import torch
+
+from oracle import attention_oracle as ao
+from tests.helpers import TOL, check_against_oracle, make_inputs, run_attention, strided_like_projection
+
+pytestmark = pytest.mark.gpu
+
+
+def api():
+    import kohakufa_cute
+
+    return kohakufa_cute
+
+
+def native():
+    from kohakufa_cute import native as module
+
+    return module
+
+
+def window_mask(starts, Sq, Sk, window, sinks):
+    """[B, 1, Sq, Sk] visibility from the definition."""
+    pos = torch.as_tensor(starts, dtype=torch.int64)[:, None, None] + torch.arange(Sq)[None, :, None]
+    key = torch.arange(Sk)[None, None, :]
+    return ((key <= pos) & ((key > pos - window) | (key < sinks)))[:, None]
+
+
+SHAPES = (
+    # B, Hq, Hkv, Sq, Sk, D, window, sinks, start
+    (1, 4, 2, 300, 300, 128, 64, 4, 0),
+    (2, 2, 2, 129, 257, 64, 1, 0, 128),        # every row sees itself only
+    (1, 4, 1, 513, 700, 96, 130, 130, 187),    # the sinks reach into the second key tile
+    (2, 4, 2, 1025, 1025, 128, 300, 5, 0),     # tiles between the sinks and the window
+    (1, 2, 2, 1, 1, 64, 5, 0, 0),              # one token
+    (1, 4, 4, 1, 600, 128, 100, 2, 599),       # one row at the end of its keys
+    (1, 2, 1, 70, 65, 17, 9, 2, 0),            # more rows than keys, an odd head
+    (1, 2, 2, 200, 200, 256, 33, 3, 0),        # a head beyond the pipeline kernels
+    (1, 2, 2, 260, 260, 64, 100000, 0, 0),     # a window longer than the sequence: plain causal
+    (1, 2, 2, 200, 300, 128, 50, 2, 500),      # behind the keys: the sinks only
+    (1, 2, 1, 300, 300, 64, 20, 0, 150),       # the last rows see nothing
+    (1, 2, 2, 400, 1000, 64, 128, 1000, 300),  # every key a sink
+    (1, 8, 1, 640, 640, 80, 256, 1, 0),
+)
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("shape", SHAPES)
+def test_forward_and_gradients_match_the_oracle(shape, dtype):
+    B, Hq, Hkv, Sq, Sk, D, window, sinks, start = shape
+    q, k, v, dout = make_inputs(B, Hq, Hkv, Sq, Sk, D, dtype, seed=Sq + Sk + window)
+    mask = window_mask([start] * B, Sq, Sk, window, sinks)
+    for scale in (None, -0.11):
+        actual = run_attention(api().sliding_window_attention, q, k, v, dout, window=window, sinks=sinks,
+                               query_start=start, scale=scale)
+        if window == 1 and sinks == 0:
+            # As with a single key: P = 1 and dS = 0 exactly, so O = V, dQ = dK = 0 and dV = dO summed over the group
+            # (the rounding contract's two independent FP32 reductions of dP and delta would invent a few-ulp gradient).
+            exact = ao.math_reference([t.cpu() for t in (q, k, v)], dout.cpu(), mask, False, scale)
+            assert torch.equal(actual[0].cpu().double(), exact[0]) and torch.equal(actual[3].cpu(), exact[3].to(dtype))
+            assert float(actual[1].abs().max()) == 0 and float(actual[2].abs().max()) == 0
+        else:
+            check_against_oracle(actual, q, k, v, dout, mask, False, scale)
+        blind = ~mask.expand(B, Hq, Sq, Sk).any(-1)
+        assert float(actual[0].cpu()[blind].abs().sum()) == 0 and float(actual[1].cpu()[blind].abs().sum()) == 0
+        unseen = ~mask.any(2)[:, 0]
+        assert all(float(g.cpu().transpose(1, 2)[unseen].abs().sum()) == 0 for g in actual[2:])
+    with torch.no_grad():
+        inference = api().sliding_window_attention(q, k, v, window=window, sinks=sinks, query_start=start, scale=-0.11)
+    if float(actual[0].abs().max()) > 0:
+        assert ao.per_head_relative_error(inference.cpu(), actual[0].cpu().double()) < TOL[dtype]["norm"]
+    else:
+        assert float(inference.abs().max()) == 0
+    assert native().device_status(reset=True) == 0
+
+
+def test_a_zero_scale_averages_the_visible_values():
+    q, k, v, dout = make_inputs(1, 2, 1, 150, 150, 64, torch.bfloat16, seed=1)
+    actual = run_attention(api().sliding_window_attention, q, k, v, dout, window=40, sinks=2, scale=0.0)
+    mask = window_mask([0], 150, 150, 40, 2)
+    want = ao.math_reference([t.cpu() for t in (q, k, v)], dout.cpu(), mask, False, 0.0)
+    # the output is one rounding (2^-9 of the value) of an average of at most 42 values below about 5
+    torch.testing.assert_close(actual[0].cpu().double(), want[0], atol=5 * 2**-9, rtol=2**-7)
+    assert float(actual[1].abs().max()) == 0 and float(actual[2].abs().max()) == 0
+
+
+def test_the_gradient_matches_differences():
+    """d(sum(out * dout)) along random directions against central differences of the FP64 definition, at the gradients'
+    own 1 % gate (the kernels' gradients are rounded to 16 bits, the differences are formed in 64 bits)."""
+    B, Hq, Hkv, S, D, window, sinks = 1, 4, 2, 200, 64, 48, 3
+    q, k, v, dout = make_inputs(B, Hq, Hkv, S, S, D, torch.float16, seed=9)
+    grads = run_attention(api().sliding_window_attention, q, k, v, dout, window=window, sinks=sinks)[1:]
+    mask = window_mask([0], S, S, window, sinks)
+    base = [t.cpu().double() for t in (q, k, v)]
+
+    def value(tensors):
+        qq, kk, vv = tensors
+        kk, vv = (t.repeat_interleave(Hq // Hkv, dim=1) for t in (kk, vv))
+        s = (qq @ kk.transpose(-1, -2) * D**-0.5).masked_fill(~mask, float("-inf"))
+        return float((torch.softmax(s, -1) @ vv * dout.cpu().double()).sum())
+
+    gen = torch.Generator().manual_seed(4)
+    for which, grad in enumerate(grads):
+        direction = grad.cpu().double() / grad.cpu().double().norm()
+        direction = direction + 0.1 * torch.randn(direction.shape, generator=gen).double() / direction.numel() ** 0.5
+        h = 1e-4
+        ends = []
+        for sign in (1, -1):
+            moved = list(base)
+            moved[which] = base[which] + sign * h * direction
+            ends.append(value(moved))
+        want = (ends[0] - ends[1]) / (2 * h)
+        got = float((grad.cpu().double() * direction).sum())
+        assert abs(got - want) < 0.01 * abs(want)
+
+
+@pytest.mark.parametrize("case", (
+    # Hq, Hkv, Sq, Sk, D, window, sinks, starts
+    (4, 2, 300, 900, 128, 128, 4, (600, 100, 0, -40)),
+    (8, 2, 1, 700, 128, 256, 4, (699, 5, 0, -1)),
+    (8, 8, 4, 515, 64, 100, 0, (511, 1, 700, -3)),
+    (8, 1, 3, 1000, 128, 64, 130, (2**31 - 1, 996, 129, -(2**31))),
+    (6, 2, 257, 400, 80, 90, 1, (143, 20, 390, 600)),
+    (4, 2, 40, 200, 256, 30, 2, (100, 160, 0, 7)),
+))
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+def test_positions_per_sequence(case, dtype):
+    """Ragged positions from a device tensor; whatever lies behind a sequence's last position is never looked at."""
+    Hq, Hkv, Sq, Sk, D, window, sinks, starts = case
+    B = len(starts)
+    q, k, v, dout = make_inputs(B, Hq, Hkv, Sq, Sk, D, dtype, seed=Sk + Sq)
+    mask = window_mask(starts, Sq, Sk, window, sinks)
+    want = ao.math_reference([t.cpu() for t in (q, k, v)], dout.cpu(), mask, False, None)[0]
+    garbage = [t.clone() for t in (k, v)]
+    for b, start in enumerate(starts):
+        end = max(0, min(Sk, start + Sq))
+        garbage[0][b, :, end:], garbage[1][b, :, end:] = float("nan"), float("inf")
+    at = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        got = api().sliding_window_attention(q, *garbage, window=window, sinks=sinks, query_start=at)
+        again = api().sliding_window_attention(q, *garbage, window=window, sinks=sinks, query_start=at)
+    assert torch.equal(got, again) and bool(torch.isfinite(got).all())
+    for b in range(B):
+        seen = mask[b].any()
+        if not seen:
+            assert float(got[b].abs().max()) == 0
+            continue
+        assert ao.per_head_relative_error(got[b:b + 1].cpu(), want[b:b + 1]) < TOL[dtype]["norm"]
+    blind = ~mask.any(-1).expand(B, Hq, Sq)
+    assert float(got.cpu()[blind].abs().sum()) == 0
+    if starts[0] >= 0 and starts[0] < 2**31 - 1:  # the int form is the same call
+        one = api().sliding_window_attention(q[:1], k[:1], v[:1], window=window, sinks=sinks, query_start=starts[0])
+        torch.testing.assert_close(one, got[:1], atol=TOL[dtype]["elem"], rtol=TOL[dtype]["elem"])
+    assert native().device_status(reset=True) == 0
+
+
+def test_layouts_give_the_same_result():
+    B, Hq, Hkv, S, D, window, sinks = 2, 4, 2, 333, 64, 77, 4
+    q, k, v, dout = make_inputs(B, Hq, Hkv, S, S, D, torch.bfloat16, seed=2)
+    call = dict(window=window, sinks=sinks)
+    want = run_attention(api().sliding_window_attention, q, k, v, dout, **call)
+    strided = run_attention(api().sliding_window_attention, *(strided_like_projection(t) for t in (q, k, v)),
+                            strided_like_projection(dout), **call)
+    wide = torch.zeros(B, Hq, S, 2 * D, device="cuda", dtype=torch.bfloat16)
+    wide[..., ::2] = q
+    channels = run_attention(api().sliding_window_attention, wide[..., ::2], k, v, dout, **call)
+    for a, b, c in zip(want, strided, channels):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@pytest.mark.parametrize("Sq", (1, 300))
+def test_captured_calls_follow_new_positions(Sq):
+    B, Hq, Hkv, Sk, D, window, sinks = 3, 8, 2, 800, 128, 200, 4
+    q, k, v, _ = make_inputs(B, Hq, Hkv, Sq, Sk, D, torch.bfloat16, seed=7)
+    at = torch.tensor([400, 20, 0], dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        api().sliding_window_attention(q, k, v, window=window, sinks=sinks, query_start=at)
+        graphs, outs = [], []
+        for _ in range(2):  # two graphs alive at once, replayed in turn
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                outs.append(api().sliding_window_attention(q, k, v, window=window, sinks=sinks, query_start=at))
+            graphs.append(graph)
+        for positions in ([400, 20, 0], [499, 300, 77], [-5, 700, 250]):
+            at.copy_(torch.tensor(positions, dtype=torch.int32))
+            want = api().sliding_window_attention(q, k, v, window=window, sinks=sinks, query_start=at)
+            for graph, out in zip(graphs, outs):
+                graph.replay()
+                torch.cuda.synchronize()
+                assert torch.equal(out, want)
+
+
+def test_training_step_in_a_graph_and_on_another_stream():
+    q, k, v, dout = make_inputs(1, 4, 2, 500, 500, 128, torch.bfloat16, seed=3)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+
+    def step():
+        out = api().sliding_window_attention(*leaves, window=150, sinks=4)
+        return (out, *torch.autograd.grad(out, leaves, dout))
+
+    want = [t.detach().clone() for t in step()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = [t.detach().clone() for t in step()]
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want, other))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = [t.detach() for t in step()]
+    graph.replay()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, held))
+
+
+@pytest.mark.parametrize("D", (64, 128))
+def test_repeated_calls_are_bit_identical(D):
+    q, k, v, dout = make_inputs(1, 4, 2, 1536, 1536, D, torch.bfloat16, seed=6)
+    first = None
+    for _ in range(25):
+        got = run_attention(api().sliding_window_attention, q, k, v, dout, window=300, sinks=5)
+        assert all(bool(torch.isfinite(t).all()) for t in got)
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
+    assert native().device_status(reset=True) == 0
+
+
+def test_compiled_route():
+    q, k, v, dout = make_inputs(1, 4, 2, 200, 200, 64, torch.bfloat16, seed=5)
+    want = run_attention(api().sliding_window_attention, q, k, v, dout, window=50, sinks=2)
+
+    def f(q, k, v):
+        return api().sliding_window_attention(q, k, v, window=50, sinks=2)
+
+    got = run_attention(torch.compile(f, fullgraph=True, backend="aot_eager"), q, k, v, dout)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_refusals():
+    q, k, v, _ = make_inputs(2, 4, 2, 8, 8, 64, torch.bfloat16, seed=5)
+    f = api().sliding_window_attention
+    at = torch.zeros(2, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="gradients need one query_start"):
+        f(q.clone().requires_grad_(True), k, v, window=4, query_start=at)
+    with pytest.raises(ValueError, match="int32"):
+        f(q, k, v, window=4, query_start=at.cpu())
+    with pytest.raises(ValueError, match="FP16/BF16"):
+        f(q.float(), k.float(), v.float(), window=4)
+    with pytest.raises(ValueError, match="divisible"):
+        f(q[:, :3], k, v, window=4)
+    with pytest.raises(ValueError, match="window >= 1"):
+        native().window_forward(q, k, v, None, 0, 0, 0, 0.1)
+    with pytest.raises(ValueError, match="position >= 0"):
+        out, m, l = native().window_forward(q, k, v, None, 0, 4, 0, 0.1)
+        native().window_backward(q, k, v, out, m, l, out, -1, 4, 0, 0.1)
+    with pytest.raises(ValueError, match="int32"):
+        native().window_forward(q, k, v, at[:1], 0, 4, 0, 0.1)
+    assert native().device_status(reset=True) == 0
