@@ -719,6 +719,32 @@ int check_f32_like(const kfa_tensor* t, const kfa_tensor* like, const char* name
     return 0;
 }
 
+// The two gradient kernels of the pipeline family, behind delta on `st`.
+int pipeline_gradients(const kfa::AttnParams& p, bool bf16, cudaStream_t st, const char* kv_name, const char* q_name) {
+    // The two gradient owners depend on delta only, not on each other: the key owners go to a side
+    // stream so that the query owners' CTAs fill the SMs the first grid frees while it drains.
+    // (Not while per-kernel timing is on: an event pair must bracket one kernel alone.)
+    Side* side = g_profile_on.load(std::memory_order_relaxed) ? nullptr : side_stream_for(st);
+    cudaStream_t kv_stream = st;
+    if (side && cudaEventRecord(side->fork, st) == cudaSuccess &&
+        cudaStreamWaitEvent(side->stream, side->fork, 0) == cudaSuccess)
+        kv_stream = side->stream;
+    cudaError_t ce = timed(kv_name, kv_stream, [&] { return kfa::launch_pipeline_backward(p, bf16, 1, kv_stream); });
+    if (ce == cudaSuccess && p.sink_tiles > 0)
+        ce = timed("combine_sink_gradients", kv_stream,
+                   [&] { return kfa::launch_combine_sink_gradients(p, bf16, kv_stream); });
+    cudaError_t cq = timed(q_name, st, [&] { return kfa::launch_pipeline_backward(p, bf16, 0, st); });
+    if (kv_stream != st) {
+        // always join, also after a failed launch: the caller's stream must not lose the side stream
+        cudaError_t cj = cudaEventRecord(side->join, kv_stream);
+        if (cj == cudaSuccess) cj = cudaStreamWaitEvent(st, side->join, 0);
+        if (ce == cudaSuccess) ce = cj;
+    }
+    if (ce != cudaSuccess) return cuda_fail(ce, "pipeline backward (dK/dV) launch");
+    if (cq != cudaSuccess) return cuda_fail(cq, "pipeline backward (dQ) launch");
+    return 0;
+}
+
 // grad_f32 = 0: the operator's backward.  Otherwise the block-wise form: FP32 gradients (bit 0), added to dq
 // (bit 1) and to dk, dv (bit 2) instead of overwriting them.
 int backward_impl(const kfa_tensor* q, const kfa_tensor* k, const kfa_tensor* v, const kfa_tensor* mask,
@@ -791,25 +817,7 @@ int backward_impl(const kfa_tensor* q, const kfa_tensor* k, const kfa_tensor* v,
         return cuda_fail(ce, "output_delta launch");
     }
     if (pipeline) {
-        // The two gradient owners depend on delta only, not on each other: the key owners go to a side
-        // stream so that the query owners' CTAs fill the SMs the first grid frees while it drains.
-        // (Not while per-kernel timing is on: an event pair must bracket one kernel alone.)
-        Side* side = g_profile_on.load(std::memory_order_relaxed) ? nullptr : side_stream_for(st);
-        cudaStream_t kv_stream = st;
-        if (side && cudaEventRecord(side->fork, st) == cudaSuccess &&
-            cudaStreamWaitEvent(side->stream, side->fork, 0) == cudaSuccess)
-            kv_stream = side->stream;
-        ce = timed("pipeline_backward_kv", kv_stream,
-                   [&] { return kfa::launch_pipeline_backward(p, bf16, 1, kv_stream); });
-        cudaError_t cq = timed("pipeline_backward_q", st, [&] { return kfa::launch_pipeline_backward(p, bf16, 0, st); });
-        if (kv_stream != st) {
-            // always join, also after a failed launch: the caller's stream must not lose the side stream
-            cudaError_t cj = cudaEventRecord(side->join, kv_stream);
-            if (cj == cudaSuccess) cj = cudaStreamWaitEvent(st, side->join, 0);
-            if (ce == cudaSuccess) ce = cj;
-        }
-        if (ce != cudaSuccess) return cuda_fail(ce, "pipeline backward (dK/dV) launch");
-        if (cq != cudaSuccess) return cuda_fail(cq, "pipeline backward (dQ) launch");
+        if (int e = pipeline_gradients(p, bf16, st, "pipeline_backward_kv", "pipeline_backward_q")) return e;
     } else if (wide) {
         void* stored = static_cast<char*>(workspace) + delta_bytes(q);
         static const char* const names[3] = {"wide_scores_p", "wide_scores_ds", "wide_grad"};
@@ -1077,6 +1085,32 @@ int fill_window(kfa::AttnParams& p, const kfa_tensor* starts, int64_t start, int
     return 0;
 }
 
+// A row that sees one key has P = 1 and exactly zero dS: like a single key, a window of one token without sinks goes
+// to the general kernels, which keep it exactly zero.
+bool window_on_pipeline(const kfa::AttnParams& p) { return p.window > 1 || p.sinks > 0; }
+
+// How the key tiles that hold sinks are split over CTAs in the backward (AttnParams::sink_tiles).  An ordinary key
+// tile streams the query tiles of one window length, a sink tile all of them; it is cut into pieces of about one
+// window length when it is more than twice as long, as far as that still adds CTAs to a grid with few of them (four
+// per SM: beyond that the long CTAs start first and the others fill in behind them).
+struct SinkPlan {
+    int tiles = 0, chunks = 0;
+    size_t bytes = 0;
+};
+SinkPlan sink_plan(const kfa_tensor* q, const kfa_tensor* k, int64_t window, int64_t sinks) {
+    SinkPlan plan;
+    const int64_t B = q->sizes[0], Sq = q->sizes[2], D = q->sizes[3], Hkv = k->sizes[1], Sk = k->sizes[2];
+    const int64_t tiles = (std::min(sinks, Sk) + 127) / 128, nq = (Sq + 127) / 128;
+    const int64_t reach = std::min<int64_t>(window, Sq) / 128 + 2;
+    if (tiles == 0 || nq <= 2 * reach || D > 128) return plan;
+    const int64_t chunks = std::min((nq + reach - 1) / reach, 4 * 148 / (tiles * B * Hkv));
+    if (chunks < 2) return plan;
+    plan.tiles = (int)tiles;
+    plan.chunks = (int)chunks;
+    plan.bytes = (size_t)(chunks * B * Hkv * tiles * 128 * 2 * D) * sizeof(float);
+    return plan;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1099,16 +1133,18 @@ int kfa_window_forward(const kfa_tensor* q, const kfa_tensor* k, const kfa_tenso
     p.logsum = keep_statistics ? static_cast<float*>(logsum->data) : nullptr;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool bf16 = q->dtype == KFA_BF16;
-    cudaError_t ce = timed("general_forward", st, [&] { return kfa::launch_general_forward(p, bf16, st); });
+    cudaError_t ce = window_on_pipeline(p) && kfa::pipeline_forward_supported(p, bf16)
+                         ? timed("pipeline_forward_window", st, [&] { return kfa::launch_pipeline_forward(p, bf16, st); })
+                         : timed("general_forward", st, [&] { return kfa::launch_general_forward(p, bf16, st); });
     if (ce != cudaSuccess) return cuda_fail(ce, "window forward launch");
     return 0;
 }
 
 size_t kfa_window_backward_workspace_bytes(const kfa_tensor* q, const kfa_tensor* k, int64_t start, int64_t window,
                                            int64_t sinks) {
-    (void)k, (void)start, (void)window, (void)sinks;
-    if (!q || q->ndim != 4) return 0;
-    return delta_bytes(q);
+    (void)start;
+    if (!q || !k || q->ndim != 4 || k->ndim != 4 || window < 1 || sinks < 0) return 0;
+    return delta_bytes(q) + sink_plan(q, k, window, sinks).bytes;
 }
 
 int kfa_window_backward(const kfa_tensor* q, const kfa_tensor* k, const kfa_tensor* v, const kfa_tensor* out,
@@ -1146,8 +1182,18 @@ int kfa_window_backward(const kfa_tensor* q, const kfa_tensor* k, const kfa_tens
     copy4(p.dvs, dv->strides);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool bf16 = q->dtype == KFA_BF16;
-    cudaError_t ce = timed("output_delta", st, [&] { return kfa::launch_output_delta(p, bf16, st); });
+    const bool pipeline = window_on_pipeline(p) && kfa::pipeline_backward_supported(p, bf16);
+    cudaError_t ce = timed("output_delta", st, [&] {
+        return pipeline ? kfa::launch_pipeline_delta(p, bf16, st) : kfa::launch_output_delta(p, bf16, st);
+    });
     if (ce != cudaSuccess) return cuda_fail(ce, "output_delta launch");
+    if (pipeline) {
+        const SinkPlan plan = sink_plan(q, k, window, sinks);
+        p.sink_tiles = plan.tiles;
+        p.sink_chunks = plan.chunks;
+        p.sink_partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(q));
+        return pipeline_gradients(p, bf16, st, "pipeline_backward_kv_window", "pipeline_backward_q_window");
+    }
     ce = timed("general_backward_q", st, [&] { return kfa::launch_general_backward(p, bf16, 0, st); });
     if (ce != cudaSuccess) return cuda_fail(ce, "window backward (dQ) launch");
     ce = timed("general_backward_kv", st, [&] { return kfa::launch_general_backward(p, bf16, 1, st); });

@@ -68,6 +68,12 @@ struct AttnParams {
     int sinks;
     int64_t start;
     const int32_t* starts;
+    // Windowed backward: the key tiles that hold sinks are seen by every later query, not only by a window's length
+    // of them, so each of the first `sink_tiles` tiles is split over `sink_chunks` CTAs by ranges of queries; they
+    // write FP32 partial gradients [chunk][batch, K/V head][sink_tiles * 128 rows][dK, dV][D], added up in order
+    // afterwards.  0 = not split.
+    int sink_tiles, sink_chunks;
+    float* sink_partial;
     int* status;      // device-visible status word (mapped host memory)
     int* abort_flag;  // device memory: set by the first CTA whose bounded wait gives up; later CTAs skip their work
 };

@@ -46,6 +46,8 @@ bool pipeline_forward_supported(const AttnParams& p, bool bf16);
 cudaError_t launch_pipeline_forward(const AttnParams& p, bool bf16, cudaStream_t st);
 bool pipeline_backward_supported(const AttnParams& p, bool bf16);
 cudaError_t launch_pipeline_backward(const AttnParams& p, bool bf16, int which, cudaStream_t st);
+// Windowed backward with split sink tiles (AttnParams::sink_tiles): adds the partial dK, dV up.
+cudaError_t launch_combine_sink_gradients(const AttnParams& p, bool bf16, cudaStream_t st);
 cudaError_t launch_pipeline_delta(const AttnParams& p, bool bf16, cudaStream_t st);
 
 // Wide heads (256/384/512 channels) on the tensor-memory pipeline.  The backward needs two 16-bit

@@ -21,8 +21,9 @@ namespace {
 using namespace bwd;
 
 // Key/value-gradient kernel.  MASKED = false is the instantiation for calls without a mask: the flag is
-// cleared at compile time, so none of the mask-table or mask-element code survives in it.
-template <int D, bool BF16, bool MASKED>
+// cleared at compile time, so none of the mask-table or mask-element code survives in it.  WINDOW is the
+// instantiation for sliding-window calls (window.cuh; neither a mask nor `causal` then).
+template <int D, bool BF16, bool MASKED, bool WINDOW>
 __global__ void __launch_bounds__(kThreads, 1) pipeline_backward_kv(const __grid_constant__ Maps maps, AttnParams p) {
     if (!MASKED) p.has_mask = 0;
     using C = kv::Cfg<D>;
@@ -34,7 +35,7 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_backward_kv(const __grid
     kv::Shared& sh = *reinterpret_cast<kv::Shared*>(s_stat + C::kStatsBytes);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    Work<true> w;
+    Work<true, WINDOW> w;
     w.init(p);
 
     if (threadIdx.x == 0) {
@@ -92,7 +93,7 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_backward_kv(const __grid
 }
 
 // Query-gradient kernel.
-template <int D, bool BF16, bool MASKED>
+template <int D, bool BF16, bool MASKED, bool WINDOW>
 __global__ void __launch_bounds__(kThreads, 1) pipeline_backward_q(const __grid_constant__ Maps maps, AttnParams p) {
     if (!MASKED) p.has_mask = 0;
     using C = q::Cfg<D>;
@@ -104,7 +105,7 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_backward_q(const __grid_
     q::Shared& sh = *reinterpret_cast<q::Shared*>(s_values + C::kValueSlots * C::kTileBytes);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    Work<false> w;
+    Work<false, WINDOW> w;
     w.init(p);
 
     if (threadIdx.x == 0) {
@@ -200,6 +201,37 @@ __global__ void __launch_bounds__(256) output_delta_rows(AttnParams p) {
     }
 }
 
+// dK, dV of the split sink tiles: the chunks' FP32 sums added in order, dK scaled, each rounded once.  A thread owns
+// eight channels of one row of dK or dV; the loads of the chunks are independent.  A few MB at most: latency-bound.
+template <typename T>
+__global__ void __launch_bounds__(128) combine_sink_gradients(AttnParams p) {
+    const int per_row = p.D / 8;
+    const int64_t rows = (int64_t)p.sink_tiles * kTile, units = (int64_t)p.B * p.Hkv;
+    const int64_t id = (int64_t)blockIdx.x * 128 + threadIdx.x;
+    if (id >= units * rows * 2 * per_row) return;
+    const int d = (int)(id % per_row) * 8;
+    const int which = (int)(id / per_row % 2);
+    const int64_t row = id / (2 * per_row) % rows, unit = id / (2 * per_row * rows);
+    if (row >= p.Sk) return;
+    const float* src = p.sink_partial + ((unit * rows + row) * 2 + which) * p.D + d;
+    const int64_t step = units * rows * 2 * p.D;
+    float sum[8] = {};
+#pragma unroll 4
+    for (int c = 0; c < p.sink_chunks; ++c) {
+        const float4 a = *reinterpret_cast<const float4*>(src + c * step);
+        const float4 e = *reinterpret_cast<const float4*>(src + c * step + 4);
+        sum[0] += a.x, sum[1] += a.y, sum[2] += a.z, sum[3] += a.w;
+        sum[4] += e.x, sum[5] += e.y, sum[6] += e.z, sum[7] += e.w;
+    }
+    const int64_t* st = which == 0 ? p.dks : p.dvs;
+    T* dst = reinterpret_cast<T*>(which == 0 ? p.dk : p.dv) + unit / p.Hkv * st[0] + unit % p.Hkv * st[1] + row * st[2] + d;
+    const float mul = which == 0 ? p.scale : 1.f;
+    T out[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) out[e] = from_float<T>(sum[e] * mul);
+    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(out);
+}
+
 std::atomic<int> g_configured{0};
 
 template <int D, bool BF16, bool KV>
@@ -207,8 +239,14 @@ cudaError_t launch_t(const AttnParams& p, cudaStream_t st) {
     constexpr int kSmem = KV ? kv::Cfg<D>::kSmemBytes : q::Cfg<D>::kSmemBytes;
     using Kernel = void (*)(const Maps, AttnParams);
     Kernel kernel;
-    if (KV) kernel = p.has_mask ? pipeline_backward_kv<D, BF16, true> : pipeline_backward_kv<D, BF16, false>;
-    else kernel = p.has_mask ? pipeline_backward_q<D, BF16, true> : pipeline_backward_q<D, BF16, false>;
+    if (KV)
+        kernel = p.window > 0 ? pipeline_backward_kv<D, BF16, false, true>
+                 : p.has_mask ? pipeline_backward_kv<D, BF16, true, false>
+                              : pipeline_backward_kv<D, BF16, false, false>;
+    else
+        kernel = p.window > 0 ? pipeline_backward_q<D, BF16, false, true>
+                 : p.has_mask ? pipeline_backward_q<D, BF16, true, false>
+                              : pipeline_backward_q<D, BF16, false, false>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
     constexpr int variant = (D == 128 ? 0 : 4) + (BF16 ? 0 : 2) + (KV ? 1 : 0);
@@ -229,7 +267,8 @@ cudaError_t launch_t(const AttnParams& p, cudaStream_t st) {
         if (!encode_bhsd_map(&maps.dq, p.dq, dt, p.D, p.Sq, p.Hq, p.B, p.dqs, 64, kTile)) return cudaErrorInvalidValue;
         maps.dk = maps.dv = maps.dq;
     }
-    const int64_t tiles = KV ? (p.Sk + kTile - 1) / kTile : (p.Sq + kTile - 1) / kTile;
+    int64_t tiles = KV ? (p.Sk + kTile - 1) / kTile : (p.Sq + kTile - 1) / kTile;
+    if (KV && p.sink_tiles > 0) tiles += (int64_t)p.sink_tiles * (p.sink_chunks - 1);
     const int64_t grid = tiles * p.B * (KV ? p.Hkv : p.Hq);
     kernel<<<(unsigned)grid, kThreads, kSmem, st>>>(maps, p);
     return cudaGetLastError();
@@ -265,6 +304,14 @@ cudaError_t launch_pipeline_backward(const AttnParams& p, bool bf16, int which, 
     }
     if (which == 0) return bf16 ? launch_t<64, true, false>(p, st) : launch_t<64, false, false>(p, st);
     return bf16 ? launch_t<64, true, true>(p, st) : launch_t<64, false, true>(p, st);
+}
+
+cudaError_t launch_combine_sink_gradients(const AttnParams& p, bool bf16, cudaStream_t st) {
+    const int64_t threads = (int64_t)p.B * p.Hkv * p.sink_tiles * kTile * 2 * (p.D / 8);
+    const unsigned grid = (unsigned)((threads + 127) / 128);
+    if (bf16) combine_sink_gradients<__nv_bfloat16><<<grid, 128, 0, st>>>(p);
+    else combine_sink_gradients<__half><<<grid, 128, 0, st>>>(p);
+    return cudaGetLastError();
 }
 
 // delta for the pipeline family (rows are 16-byte aligned and channel-contiguous there)

@@ -2,6 +2,7 @@
 #pragma once
 #include "kfa_common.cuh"
 #include "sm100_ptx.cuh"
+#include "window.cuh"
 
 namespace kfa {
 namespace bwd {
@@ -33,18 +34,49 @@ __device__ __forceinline__ int tile_state(const AttnParams& p, int b, int h, int
     return (s00 & s01 & s10 & s11) == 2 ? 2 : 1;
 }
 
-// The CTA's place in the problem and its stream of work units.
-template <bool KV>
+// The CTA's place in the problem and its stream of work units.  WINDOW: a sliding-window call (window.cuh).
+template <bool KV, bool WINDOW>
 struct Work {
+    static constexpr bool kWindow = WINDOW;
     int b, head, owner0;  // batch, owner head (query head or K/V head), first owner row
     int first, end;       // streamed tile range [first, end)
     int groups;           // query heads per owner (KV) or 1
+    int64_t start;        // windowed calls: key position of query row 0
+    WindowTiles keys;     // windowed query owners: the key tiles to walk
+    float* partial;       // windowed key owners: this CTA's FP32 partial gradients, or null (it owns its rows alone)
     int fixed;            // state shared by every unit of this CTA (2 without a mask), or -1: look each unit up
 
     __device__ __forceinline__ void init(const AttnParams& p) {
         const int owner_len = KV ? p.Sk : p.Sq;
         const int heads = KV ? p.Hkv : p.Hq;
-        const int nblk = (owner_len + kTile - 1) / kTile;
+        int nblk = (owner_len + kTile - 1) / kTile;
+        partial = nullptr;
+        start = WINDOW ? p.start : 0;
+        int64_t index = blockIdx.x;
+        if (WINDOW && KV && p.sink_tiles > 0) {
+            // the split sink tiles first; the others follow in the order below
+            const int64_t units = (int64_t)p.B * heads * p.sink_tiles;
+            if (index < units * p.sink_chunks) {
+                const int chunk = (int)(index / units), tile = (int)(index % units) % p.sink_tiles;
+                const int bh = (int)(index % units) / p.sink_tiles;
+                head = bh % heads;
+                b = bh / heads;
+                owner0 = tile * kTile;
+                fixed = 2;
+                groups = p.group;
+                const WindowRange r =
+                    window_query_tiles(start, owner0, min(owner0 + kTile, p.Sk), p.window, p.sinks, p.Sq);
+                const int each = (r.end - r.first + p.sink_chunks - 1) / p.sink_chunks;
+                first = r.first + chunk * each;
+                end = min(r.end, first + each);
+                if (first > end) first = end;
+                partial = p.sink_partial +
+                          (((int64_t)chunk * p.B * heads + bh) * p.sink_tiles + tile) * kTile * 2 * p.D;
+                return;
+            }
+            index -= units * p.sink_chunks;
+            nblk -= p.sink_tiles;
+        }
         // Heavy tiles first (late query tiles, early key tiles under a causal mask), tile row by tile row over a
         // chunk of heads: the grid then ends with the light tiles of its last chunk, whereas a head-by-head order
         // starts heavy tiles of the last heads in the final wave.  A chunk holds as many heads as keep the streamed
@@ -55,23 +87,34 @@ struct Work {
         chunk = chunk < 1 ? 1 : (chunk > nbh ? nbh : chunk);
         if ((int64_t)gridDim.x < KFA_ROW_MAJOR_LIMIT) chunk = nbh;
         const int64_t per_chunk = chunk * nblk, full = nbh / chunk;
-        int64_t c = blockIdx.x / per_chunk, within, size;
+        int64_t c = index / per_chunk, within, size;
         if (c < full) {
-            within = blockIdx.x - c * per_chunk;
+            within = index - c * per_chunk;
             size = chunk;
         } else {
             c = full;
-            within = blockIdx.x - full * per_chunk;
+            within = index - full * per_chunk;
             size = nbh - full * chunk;
         }
         int blk = (int)(within / size);
         if (!KV) blk = nblk - 1 - blk;
+        else if (WINDOW) blk += p.sink_tiles;
         const int64_t bh = c * chunk + within % size;
         head = (int)(bh % heads);
         b = (int)(bh / heads);
         owner0 = blk * kTile;
         fixed = p.has_mask ? -1 : 2;
-        if (KV) {
+        if (WINDOW && KV) {
+            groups = p.group;
+            const WindowRange r = window_query_tiles(start, owner0, min(owner0 + kTile, p.Sk), p.window, p.sinks, p.Sq);
+            first = r.first;
+            end = r.end;
+        } else if (WINDOW) {
+            groups = 1;
+            keys = window_key_tiles(start, owner0, min(p.Sq, owner0 + kTile), p.window, p.sinks, p.Sk);
+            first = keys.begin();
+            end = keys.end;
+        } else if (KV) {
             groups = p.group;
             first = p.causal ? owner0 / kTile : 0;  // only queries r >= key see the key
             end = (p.Sq + kTile - 1) / kTile;
@@ -109,7 +152,8 @@ struct Work {
         settle(p, g, i);
     }
     __device__ __forceinline__ void next(const AttnParams& p, int& g, int& i) const {
-        ++i;
+        if (WINDOW && !KV) i = keys.next(i);
+        else ++i;
         settle(p, g, i);
     }
     __device__ __forceinline__ bool valid(int g) const { return g < groups; }

@@ -18,8 +18,8 @@ namespace kfa {
 namespace bwd {
 namespace kv {
 
-template <int D, bool BF16>
-__device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams& p, const Work<true>& w, Shared& sh,
+template <int D, bool BF16, class W>
+__device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams& p, const W& w, Shared& sh,
                                               uint32_t tmem, uint8_t* s_owner, int wg, int warp, int lane) {
     using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
     volatile int* abort_word = &sh.abort_word;
@@ -35,6 +35,13 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
     const bool key_padding = p.has_mask && p.ms[1] == 0 && p.ms[2] == 0;  // one line for all heads and queries
     if (row_ok && key_padding) row_ok = mask_b[(int64_t)owner_row * p.ms[3]] != 0;
 
+    // a windowed call: the queries [query_lo, query_hi) that see this thread's key
+    int query_lo = 0, query_hi = 0;
+    if (W::kWindow) {
+        const int64_t from = owner_row - w.start, to = owner_row < p.sinks ? p.Sq : from + p.window;
+        query_lo = (int)(from < 0 ? 0 : (from > p.Sq ? p.Sq : from));
+        query_hi = (int)(to < 0 ? 0 : (to > p.Sq ? p.Sq : to));
+    }
     const uint32_t s_addr = lane_base + kColS + wg * kCols, dp_addr = lane_base + kColDp + wg * kCols;
     int g, i;
     w.begin(p, g, i);
@@ -52,8 +59,13 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
         // columns [lo, 64) of this thread's 64 are visible: the query index must be >= the key index
         const int col0 = i * kTile + wg * kCols;  // first query of this thread's columns
         int lo = p.causal ? owner_row - col0 : 0;
+        int hi = kCols;
+        if (W::kWindow) {  // columns [lo, hi): queries from the key's own position on, and at most a window behind it
+            lo = query_lo - min(col0, query_lo);
+            hi = query_hi - min(col0, query_hi);
+        }
         if (!row_ok) lo = kCols;
-        const bool masked = __any_sync(0xffffffffu, lo > 0) || state == 1;
+        const bool masked = __any_sync(0xffffffffu, lo > 0 || (W::kWindow && hi < kCols)) || state == 1;
 
         // ------------------------------------------------------------ P_low
         PH(4);
@@ -75,6 +87,10 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
                 if (apply_mask) {
                     pa = c >= lo ? pa : 0.f;
                     pb = c + 1 >= lo ? pb : 0.f;
+                    if (W::kWindow) {
+                        pa = c < hi ? pa : 0.f;
+                        pb = c + 1 < hi ? pb : 0.f;
+                    }
                     if (state == 1) {
                         pa = mline[(int64_t)min(col0 + c, p.Sq - 1) * p.ms[2]] != 0 ? pa : 0.f;
                         pb = mline[(int64_t)min(col0 + c + 1, p.Sq - 1) * p.ms[2]] != 0 ? pb : 0.f;
@@ -155,6 +171,34 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
                (int64_t)owner_row * p.dks[2] + ch0;
         out2 = reinterpret_cast<T*>(p.dv) + (int64_t)w.b * p.dvs[0] + (int64_t)w.head * p.dvs[1] +
                (int64_t)owner_row * p.dvs[2] + ch0;
+    }
+    if (W::kWindow && w.partial) {
+        // one range of queries of a sink tile: unscaled FP32 sums, added up by combine_sink_gradients
+        if (!ok) return;
+        float* f1 = w.partial + (int64_t)r * 2 * p.D + ch0;
+        float* f2 = f1 + p.D;
+        const int valid = p.D - ch0;
+        if (unit == 0) {
+            for (int d = 0; d < kHalf && d < valid; d += 4) {
+                *reinterpret_cast<float4*>(f1 + d) = make_float4(0.f, 0.f, 0.f, 0.f);
+                *reinterpret_cast<float4*>(f2 + d) = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            return;
+        }
+        if (!mbar_wait(&sh.final_done, 0, abort_word, 150)) return;
+        tc_fence_after();
+        constexpr int kStepP = kHalf < 32 ? 16 : 32;
+#pragma unroll
+        for (int c = 0; c < kHalf; c += kStepP) {
+            uint32_t v[kStepP];
+            tmem_ld(lane_base + kColDk + ch0 + c, v);
+            tmem_wait_ld();
+            put_f32(f1 + c, v, valid - c, 1.f, false);
+            tmem_ld(lane_base + kColDv + ch0 + c, v);
+            tmem_wait_ld();
+            put_f32(f2 + c, v, valid - c, 1.f, false);
+        }
+        return;
     }
     if (p.grad_f32) {
         // FP32 partial gradients of a block-wise call: plain vector stores (or read-add-write) per row

@@ -77,8 +77,8 @@ __device__ __forceinline__ uint64_t umma_desc_plain(uint32_t saddr) {
     return d;
 }
 
-template <int D>
-__device__ __forceinline__ void loader_role(const Maps& maps, const AttnParams& p, const Work<true>& w, Shared& sh,
+template <int D, class W>
+__device__ __forceinline__ void loader_role(const Maps& maps, const AttnParams& p, const W& w, Shared& sh,
                                             uint8_t* s_owner, uint8_t* s_ring) {
     using C = Cfg<D>;
     volatile int* abort_word = &sh.abort_word;
@@ -118,8 +118,8 @@ __device__ __forceinline__ void loader_role(const Maps& maps, const AttnParams& 
 // S(u+1) into the score columns that product has just read; once dS_low(u) is back: dK += dS_low(u) x Q(u),
 // then dP(u+1) into the dP columns.  The consumers form dS_low(u) while dV(u) and S(u+1) run, and P_low(u+1)
 // while dK(u) and dP(u+1) run.
-template <int D, bool BF16>
-__device__ __forceinline__ void mma_role(const AttnParams& p, const Work<true>& w, Shared& sh, uint32_t tmem,
+template <int D, bool BF16, class W>
+__device__ __forceinline__ void mma_role(const AttnParams& p, const W& w, Shared& sh, uint32_t tmem,
                                          uint8_t* s_owner, uint8_t* s_ring, uint8_t* s_stat) {
     using C = Cfg<D>;
     volatile int* abort_word = &sh.abort_word;
@@ -240,7 +240,8 @@ __device__ __forceinline__ void split3(float x, uint32_t& h1, uint32_t& h2, uint
 // queries the row [m1 m2 m3 l1 l2 l3 0 0 | d1 d2 d3 0 0 0 0 0] of BF16 pieces.  A query beyond the
 // sequence end, or one that saw no key in the forward pass (maximum = -inf), gets a huge maximum so
 // that its probabilities evaluate to exactly zero.
-__device__ __forceinline__ void stats_role(const AttnParams& p, const Work<true>& w, Shared& sh, uint8_t* s_stat,
+template <class W>
+__device__ __forceinline__ void stats_role(const AttnParams& p, const W& w, Shared& sh, uint8_t* s_stat,
                                            int lane) {
     volatile int* abort_word = &sh.abort_word;
     int g, i;

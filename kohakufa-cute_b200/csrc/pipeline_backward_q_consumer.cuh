@@ -16,8 +16,8 @@ namespace kfa {
 namespace bwd {
 namespace q {
 
-template <int D, bool BF16>
-__device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams& p, const Work<false>& w, Shared& sh,
+template <int D, bool BF16, class W>
+__device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams& p, const W& w, Shared& sh,
                                               uint32_t tmem, uint8_t* s_owner, int wg, int warp, int lane) {
     using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
     volatile int* abort_word = &sh.abort_word;
@@ -43,6 +43,8 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
 
     // every row of this warp has visible keys (no mask, no row beyond the sequence end): statistics are finite
     const bool rows_real = !p.has_mask && __all_sync(0xffffffffu, owner_row < p.Sq && row_m != INFINITY);
+    const WindowSpan span =
+        W::kWindow ? window_span(w.start, min(owner_row, p.Sq - 1), p.window, p.Sk) : WindowSpan{0, 0};
     int g, i;
     w.begin(p, g, i);
     int unit = 0;
@@ -58,7 +60,15 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
         const int col0 = i * kTile + wg * kCols;
         int hi = p.Sk - col0;
         if (p.causal) hi = min(hi, owner_row - col0 + 1);
-        const bool masked = __any_sync(0xffffffffu, hi < kCols) || state == 1;
+        // a windowed call: the columns [0, hi) that lie at or behind `lo`, or below `sink`
+        int lo = 0, sink = 0;
+        if (W::kWindow) {
+            hi = span.hi - col0;
+            lo = span.lo - col0;
+            sink = p.sinks - col0;
+            if (lo <= sink) lo = 0;
+        }
+        const bool masked = __any_sync(0xffffffffu, hi < kCols || lo > 0) || state == 1;
 
         // ------------------------------------------------------------ P_low
         PH(4);
@@ -81,6 +91,10 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
                 if (apply_mask) {
                     pa = c < hi ? pa : 0.f;
                     pb = c + 1 < hi ? pb : 0.f;
+                    if (W::kWindow) {
+                        pa = c >= lo || c < sink ? pa : 0.f;
+                        pb = c + 1 >= lo || c + 1 < sink ? pb : 0.f;
+                    }
                     if (state == 1) {
                         pa = mline_head[(int64_t)min(col0 + c, p.Sk - 1) * p.ms[3]] != 0 ? pa : 0.f;
                         pb = mline_head[(int64_t)min(col0 + c + 1, p.Sk - 1) * p.ms[3]] != 0 ? pb : 0.f;

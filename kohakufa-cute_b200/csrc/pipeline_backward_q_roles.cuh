@@ -48,8 +48,8 @@ struct Shared {
 
 constexpr uint32_t kColS = 0, kColDp = 256, kColGrad = 384;
 
-template <int D>
-__device__ __forceinline__ void loader_role(const Maps& maps, const AttnParams& p, const Work<false>& w, Shared& sh,
+template <int D, class W>
+__device__ __forceinline__ void loader_role(const Maps& maps, const AttnParams& p, const W& w, Shared& sh,
                                             uint8_t* s_owner, uint8_t* s_keys, uint8_t* s_values) {
     using C = Cfg<D>;
     volatile int* abort_word = &sh.abort_word;
@@ -94,8 +94,8 @@ __device__ __forceinline__ void loader_role(const Maps& maps, const AttnParams& 
 //   chain 0:  S of every unit, into the two score buffers in turn
 //   chain 1:  dP of the coming unit as soon as the consumers hold the current one, then dQ += dS_low x K
 // s_free orders the two chains on a score buffer (chain 1 reads dS_low out of it, chain 0 refills it).
-template <int D, bool BF16>
-__device__ __forceinline__ void mma_role(const AttnParams& p, const Work<false>& w, Shared& sh, uint32_t tmem,
+template <int D, bool BF16, class W>
+__device__ __forceinline__ void mma_role(const AttnParams& p, const W& w, Shared& sh, uint32_t tmem,
                                          uint8_t* s_owner, uint8_t* s_keys, uint8_t* s_values, int chain) {
     using C = Cfg<D>;
     volatile int* abort_word = &sh.abort_word;

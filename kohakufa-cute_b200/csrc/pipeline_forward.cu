@@ -30,6 +30,7 @@
 #include "launchers.h"
 #include "sm100_ptx.cuh"
 #include "tensor_map.h"
+#include "window.cuh"
 
 #include <atomic>
 #include <type_traits>
@@ -97,7 +98,10 @@ __device__ __forceinline__ int key_tile_state(const AttnParams& p, int b, int h,
 }
 
 // MASKED = false is the instantiation for calls without a mask (the flag is cleared at compile time).
-template <int D, bool BF16, bool MASKED>
+// WINDOW is the instantiation for sliding-window calls (window.cuh; neither a mask nor `causal` then): a query tile
+// walks the key tiles of the sinks and of its window, two tiles of a CTA need not see the same ones, and positions
+// come from device memory where the call gives one per sequence.
+template <int D, bool BF16, bool MASKED, bool WINDOW>
 __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_constant__ FwdMaps maps, AttnParams p) {
     if (!MASKED) p.has_mask = 0;
     using Cfg = FwdCfg<D>;
@@ -122,13 +126,23 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
     const int kvh = h / p.group;
     const int q0 = qblk * 2 * kTileQ;
 
-    // key tiles each query tile may see
+    // key tiles each query tile may see: those below n_t[t]; in a windowed call the ones its `wt` names (n_t[t] is
+    // the end of them) and, for the CTA, their union `both`
     int n_t[2];
+    const int64_t start = WINDOW ? window_start(p, b) : 0;
+    WindowTiles wt[2] = {{0, 0, 0}, {0, 0, 0}}, both = {0, 0, 0};
+    int lo_t[2] = {0, 0}, hi_t[2] = {0, 0};  // keys some row of the tile sees, apart from sinks below lo_t
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         const int row_lo = q0 + t * kTileQ;
         if (row_lo >= p.Sq) {
             n_t[t] = 0;
+        } else if (WINDOW) {
+            const int row_hi = min(p.Sq, row_lo + kTileQ);
+            wt[t] = window_key_tiles(start, row_lo, row_hi, p.window, p.sinks, p.Sk);
+            lo_t[t] = window_span(start, row_lo, p.window, p.Sk).lo;
+            hi_t[t] = window_span(start, row_hi - 1, p.window, p.Sk).hi;
+            n_t[t] = wt[t].end;
         } else {
             const int row_hi = min(p.Sq, row_lo + kTileQ);
             const int k_hi = p.causal ? min(p.Sk, row_hi) : p.Sk;
@@ -136,6 +150,14 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
         }
     }
     const int n_max = max(n_t[0], n_t[1]);
+    if (WINDOW) {
+        const bool some0 = wt[0].first < wt[0].end, some1 = wt[1].first < wt[1].end;
+        both.sink_end = max(wt[0].sink_end, wt[1].sink_end);
+        both.end = n_max;
+        both.first = some0 ? (some1 ? min(wt[0].first, wt[1].first) : wt[0].first) : (some1 ? wt[1].first : n_max);
+        both.first = max(both.first, both.sink_end);
+    }
+    const int cta_hi = max(hi_t[0], hi_t[1]);
 
     if (threadIdx.x == 0) {
         sh.abort_word = *reinterpret_cast<volatile int*>(p.abort_flag) != 0 ? 90 : 0;  // 90: an earlier CTA gave up
@@ -165,6 +187,20 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
     const uint8_t* states = sh.tile_state;
     const bool masked_call = p.has_mask != 0;
     auto state_of = [&](int j) -> int { return masked_call ? states[j] : 2; };
+    // the CTA's walk over its key tiles, and which of them query tile t sees
+    auto first_tile = [&]() -> int {
+        if (WINDOW) return both.begin();
+        int j = 0;
+        while (j < n_max && state_of(j) == 0) ++j;
+        return j;
+    };
+    auto next_tile = [&](int j) -> int {
+        if (WINDOW) return both.next(j);
+        ++j;
+        while (j < n_max && state_of(j) == 0) ++j;
+        return j;
+    };
+    auto sees = [&](int t, int j) -> bool { return WINDOW ? wt[t].has(j) : j < n_t[t]; };
     volatile int* abort_word = &sh.abort_word;
 
     const bool dead = sh.abort_word != 0;  // set before the barrier above: skip straight to the tear-down
@@ -186,8 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
                                     q0 + t * kTileQ, h, b);
             int slot_use = 0;
             bool ok = true;
-            for (int j = 0; j < n_max && ok; ++j) {
-                if (state_of(j) == 0) continue;
+            for (int j = first_tile(); j < n_max && ok; j = next_tile(j)) {
                 for (int which = 0; which < 2 && ok; ++which) {  // K tile, then V tile
                     const int slot = slot_use % Cfg::kStages, round = slot_use / Cfg::kStages;
                     if (round > 0) ok = mbar_wait(&sh.kv_empty[slot], (round - 1) & 1, abort_word, 10);
@@ -230,19 +265,45 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
                     umma_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, umma_desc_advance(v_desc, b0 + kk * 2048),
                             idesc_o, accumulate || kk > 0);
             };
+            // The same in a windowed call: steps of 16 keys that no row of the tile sees are left out.
+            bool begun[2] = {false, false};  // the tile's accumulator holds something
+            auto issue_o_window = [&](int t, int slot, int half, int j) {
+                const uint32_t b0 = slot * Cfg::kTileBytes;
+#pragma unroll
+                for (int kk = half * (kTileK / 32); kk < (half + 1) * (kTileK / 32); ++kk) {
+                    const int key = j * kTileK + kk * 16;
+                    if (key >= hi_t[t] || (key + 16 <= lo_t[t] && key >= p.sinks)) continue;
+                    umma_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, umma_desc_advance(v_desc, b0 + kk * 2048),
+                            idesc_o, begun[t]);
+                    begun[t] = true;
+                }
+            };
+            // Values behind the last key that the CTA's rows see may never have been written (the free end of a
+            // cache): their probabilities are zero, but zero times a NaN is not.  The rest of the 16-key step the
+            // last key falls into is overwritten with zeros (at most 15 rows; rows beyond Sk arrive as zeros).
+            auto clear_unseen = [&](int slot, int j) {
+                const int r0 = cta_hi - j * kTileK;
+                if (r0 <= 0 || r0 >= kTileK || cta_hi >= p.Sk || r0 % 16 == 0) return;
+                uint8_t* tile = sKV + slot * Cfg::kTileBytes;
+                for (int r = r0; r % 16 != 0; ++r)
+                    for (int c = 0; c < Cfg::kChunks; ++c)
+#pragma unroll
+                        for (int x = 0; x < 8; ++x)
+                            *reinterpret_cast<uint4*>(tile + c * (kTileK * 128) + r * 128 + x * 16) = make_uint4(0, 0, 0, 0);
+                fence_async_smem();
+            };
             bool ok = mbar_wait(&sh.q_full, 0, abort_word, 20);
             int slot_use = 0, iter[2] = {0, 0};
             PH_DECL;
             // first visible key tile
-            int j = 0;
-            while (j < n_max && state_of(j) == 0) ++j;
+            int j = first_tile();
             if (ok && j < n_max) {
                 const int slot = slot_use % Cfg::kStages;
                 ok = mbar_wait(&sh.kv_full[slot], (slot_use / Cfg::kStages) & 1, abort_word, 21);
                 if (ok) {
                     tc_fence_after();
                     for (int t = 0; t < 2; ++t)
-                        if (j < n_t[t]) {
+                        if (sees(t, j)) {
                             issue_s(t, slot);
                             umma_commit(&sh.s_ready[t]);
                         }
@@ -251,8 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
                 }
             }
             while (ok && j < n_max) {
-                int jn = j + 1;
-                while (jn < n_max && state_of(jn) == 0) ++jn;
+                const int jn = next_tile(j);
                 const int v_slot = slot_use % Cfg::kStages, v_par = (slot_use / Cfg::kStages) & 1;
                 ++slot_use;
                 int k_slot = -1, k_par = 0;
@@ -265,21 +325,28 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
                 ok = mbar_wait(&sh.kv_full[v_slot], v_par, abort_word, 22);
                 PH(0);
                 bool k_waited = false;
+                if (WINDOW && ok) clear_unseen(v_slot, j);
                 for (int t = 0; t < 2 && ok; ++t) {
-                    if (j >= n_t[t]) continue;
-                    ok = mbar_wait(&sh.p_half[t][0], iter[t] & 1, abort_word, 23 + t);
-                    if (!ok) break;
-                    PH(1);
-                    tc_fence_after();
-                    issue_o(t, v_slot, 0, iter[t] > 0);
-                    PH(2);
-                    ok = mbar_wait(&sh.p_half[t][1], iter[t] & 1, abort_word, 26 + t);
-                    if (!ok) break;
-                    PH(1);
-                    tc_fence_after();
-                    issue_o(t, v_slot, 1, true);
-                    PH(2);
-                    if (jn < n_t[t]) {
+                    const bool now = sees(t, j), then = sees(t, jn);
+                    if (!now && !(WINDOW && then)) continue;
+                    if (now) {
+                        ok = mbar_wait(&sh.p_half[t][0], iter[t] & 1, abort_word, 23 + t);
+                        if (!ok) break;
+                        PH(1);
+                        tc_fence_after();
+                        if (WINDOW) issue_o_window(t, v_slot, 0, j);
+                        else issue_o(t, v_slot, 0, iter[t] > 0);
+                        PH(2);
+                        ok = mbar_wait(&sh.p_half[t][1], iter[t] & 1, abort_word, 26 + t);
+                        if (!ok) break;
+                        PH(1);
+                        tc_fence_after();
+                        if (WINDOW) issue_o_window(t, v_slot, 1, j);
+                        else issue_o(t, v_slot, 1, true);
+                        PH(2);
+                        ++iter[t];
+                    }
+                    if (then) {
                         if (!k_waited) {
                             ok = mbar_wait(&sh.kv_full[k_slot], k_par, abort_word, 25);
                             if (!ok) break;
@@ -289,10 +356,12 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
                         PH(3);
                         issue_s(t, k_slot);
                     }
-                    umma_commit(&sh.s_ready[t]);
+                    // one commit per score tile and one behind the last product; a tile that pauses between the
+                    // sinks and its window gets the next score tile's commit
+                    if (!WINDOW || then || jn >= n_t[t]) umma_commit(&sh.s_ready[t]);
                     PH(4);
-                    ++iter[t];
                 }
+                if (WINDOW && ok && k_slot >= 0 && !k_waited) ok = mbar_wait(&sh.kv_full[k_slot], k_par, abort_word, 25);
                 if (!ok) break;
                 umma_commit(&sh.kv_empty[v_slot]);
                 if (k_slot >= 0) umma_commit(&sh.kv_empty[k_slot]);
@@ -319,7 +388,11 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
         int iter = 0;
         bool ok = true;
         PH_DECL;
-        for (int j = 0; j < n_t[t] && ok; ++j) {
+        // a windowed call: this row's window, and the tile's own walk
+        const WindowSpan span = WINDOW ? window_span(start, min(row, p.Sq - 1), p.window, p.Sk) : WindowSpan{0, 0};
+        const WindowTiles mine = t == 0 ? wt[0] : wt[1];
+        const int n_mine = t == 0 ? n_t[0] : n_t[1];
+        for (int j = WINDOW ? mine.begin() : 0; j < n_mine && ok; j = WINDOW ? mine.next(j) : j + 1) {
             const int state = state_of(j);
             if (state == 0) continue;
             PH(5);
@@ -342,10 +415,18 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
             const int key0 = j * kTileK;
             // leading columns of this tile that pass the sequence-end and causal bounds for this row
             int lim = p.Sk - key0;
-            if (p.causal) lim = min(lim, row - key0 + 1);
+            if (WINDOW) lim = span.hi - key0;
+            else if (p.causal) lim = min(lim, row - key0 + 1);
             if (lim < kTileK) {
 #pragma unroll
                 for (int c = 0; c < kTileK; ++c) s[c] = c < lim ? s[c] : -INFINITY;
+            }
+            if (WINDOW) {  // columns before the window, apart from the sinks
+                const int lo = span.lo - key0, sink = p.sinks - key0;
+                if (lo > 0 && lo > sink) {
+#pragma unroll
+                    for (int c = 0; c < kTileK; ++c) s[c] = c < lo && c >= sink ? -INFINITY : s[c];
+                }
             }
             if (state == 1) {
 #pragma unroll
@@ -430,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
         }
         if ((threadIdx.x & 127) == 0) PH_FLUSH(t);
         // epilogue: wait for the last product, normalise, store
-        if (ok && iter == 0 && row < p.Sq && n_t[t] > 0 && !p.running) {
+        if (ok && iter == 0 && row < p.Sq && (WINDOW || n_t[t] > 0) && !p.running) {
             // every key tile of this row is hidden: zero output, empty statistics
             using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
             T* orow = reinterpret_cast<T*>(p.out) + (int64_t)b * p.os[0] + (int64_t)h * p.os[1] + (int64_t)row * p.os[2];
@@ -536,7 +617,9 @@ template <int D, bool BF16>
 cudaError_t launch_t(const AttnParams& p, cudaStream_t st) {
     using Cfg = FwdCfg<D>;
     // The shared-memory opt-in is per device; it is cheap, so it is simply repeated per call.
-    auto kernel = p.has_mask ? pipeline_forward<D, BF16, true> : pipeline_forward<D, BF16, false>;
+    auto kernel = p.window > 0 ? pipeline_forward<D, BF16, false, true>
+                  : p.has_mask ? pipeline_forward<D, BF16, true, false>
+                               : pipeline_forward<D, BF16, false, false>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
     if (e != cudaSuccess) return e;
     constexpr int variant = (D == 128 ? 0 : 2) + (BF16 ? 0 : 1);  // D = channels the kernel runs with (p.D rounded up)
