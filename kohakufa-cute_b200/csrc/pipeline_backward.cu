@@ -126,6 +126,8 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_backward_q(const __grid_
         mbar_init(&sh.ds_done, kConsumers);
         mbar_init(&sh.final_done, 2);
         mbar_init(&sh.out_staged, kConsumers);
+        mbar_init(&sh.mean_ready, 1);
+        mbar_init(&sh.sums_staged, kConsumers);
         mbar_fence_init();
     }
     if (warp == kRoleWarp) {
@@ -145,6 +147,8 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_backward_q(const __grid_
             if (elect_one()) q::mma_role<D, BF16>(p, w, sh, tmem, s_owner, s_keys, s_values, warp - kRoleWarp);
         } else if (warp == kRoleWarp + 2) {
             if (elect_one()) q::loader_role<D>(maps, p, w, sh, s_owner, s_keys, s_values);
+        } else if (WINDOW) {
+            q::mean_role<D, typename std::conditional<BF16, __nv_bfloat16, __half>::type>(p, w, sh, lane);
         }
     } else {
         reg_alloc<200>();

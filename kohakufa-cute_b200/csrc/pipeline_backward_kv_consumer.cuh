@@ -8,7 +8,7 @@
 //   P      = ex2(s~ * c)          c = |scale| * log2(e)
 //   P_low  = round(P)             one rounding to the input type
 //   dS_low = round(P_low * dP~)
-// Hidden entries get P = 0.  The work of a unit runs in two phases so that the tensor core never waits
+// (windowed calls form dS_low from the unrounded P, one rounding less).  Hidden entries get P = 0.  The work of a unit runs in two phases so that the tensor core never waits
 // for all of it: P_low needs only the score tile and goes back at once (dV and the next score tile run
 // under the second phase), dS_low needs the dP tile and the P_low values kept in registers.
 #pragma once
@@ -74,8 +74,15 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
         PH(0);
         tc_fence_after();
         uint32_t pw[kCols / 2];
+        uint32_t s[kCols];  // a windowed call keeps the unrounded probabilities in place of the scores for dS
+        auto keep = [&](int c, float pa, float pb) {
+            if (W::kWindow) {
+                s[c] = __float_as_uint(pa);
+                s[c + 1] = __float_as_uint(pb);
+            }
+            pw[c / 2] = pack2<BF16>(pa, pb);
+        };
         {
-            uint32_t s[kCols];
             tmem_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
             tmem_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
             tmem_wait_ld();
@@ -96,7 +103,7 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
                         pb = mline[(int64_t)min(col0 + c + 1, p.Sq - 1) * p.ms[2]] != 0 ? pb : 0.f;
                     }
                 }
-                pw[c / 2] = pack2<BF16>(pa, pb);
+                keep(c, pa, pb);
             };
             // Both consumer warpgroups form probabilities at the same time, and together they ask the
             // special-function unit for one result per score: where no score is hidden (no mask, every streamed
@@ -104,7 +111,7 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
             auto prob_poly = [&](int c) {
                 float pa, pb;
                 ex2_poly_pair(f2_mul(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), c2_pair), pa, pb);
-                pw[c / 2] = pack2<BF16>(pa, pb);
+                keep(c, pa, pb);
             };
             if (masked) {
 #pragma unroll
@@ -141,7 +148,8 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
             PH(1);
 #pragma unroll
             for (int c = 0; c < kCols; c += 2) {
-                const float2 pl = unpack2<BF16>(pw[c / 2]);
+                const float2 pl = W::kWindow ? make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1]))
+                                             : unpack2<BF16>(pw[c / 2]);
                 float da, db;
                 f2_unpack(f2_mul(f2_pack(pl.x, pl.y), f2_pack(__uint_as_float(dp[c]), __uint_as_float(dp[c + 1]))),
                           da, db);

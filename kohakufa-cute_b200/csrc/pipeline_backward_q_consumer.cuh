@@ -9,6 +9,8 @@
 // P_low of a unit is formed as soon as its score tile is there (the tensor core is still busy with
 // the previous unit's dQ and this unit's dP); the dP values are then pulled into registers, the dP
 // buffer is handed back, and dS_low is packed over the thread's own (dead) score columns.
+// Windowed calls have no reference to round like: they form dS_low = round(P * (dP - delta)) from the unrounded P (one
+// rounding less) and take the row sum of dS_low times a mean key off dQ (see mean_role).
 #pragma once
 #include "pipeline_backward_q_roles.cuh"
 
@@ -49,6 +51,7 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
     w.begin(p, g, i);
     int unit = 0;
     bool ok = true;
+    uint64_t row_sum = f2_pack(0.f, 0.f);  // windowed calls: sum of this thread's dS_low (see mean_role)
     PH_DECL;
     while (w.valid(g) && ok) {
         PH(5);
@@ -76,9 +79,18 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
         if (!ok) break;
         PH(0);
         tc_fence_after();
+        // P_low packed in pairs; a windowed call keeps the unrounded probabilities (in place of the scores)
         uint32_t pw[kCols / 2];
+        uint32_t s[kCols];
+        auto keep = [&](int c, float pa, float pb) {
+            if (W::kWindow) {
+                s[c] = __float_as_uint(pa);
+                s[c + 1] = __float_as_uint(pb);
+            } else {
+                pw[c / 2] = pack2<BF16>(pa, pb);
+            }
+        };
         {
-            uint32_t s[kCols];
             tmem_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
             tmem_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
             tmem_wait_ld();
@@ -100,7 +112,7 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
                         pb = mline_head[(int64_t)min(col0 + c + 1, p.Sk - 1) * p.ms[3]] != 0 ? pb : 0.f;
                     }
                 }
-                pw[c / 2] = pack2<BF16>(pa, pb);
+                keep(c, pa, pb);
             };
             // Both consumer warpgroups form probabilities at the same time, and together they ask the
             // special-function unit for one result per score: where no score is hidden, every fourth pair is
@@ -109,7 +121,7 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
                 float pa, pb;
                 ex2_poly_pair(f2_sub(f2_mul(f2_sub(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), m_pair),
                                             c2_pair), ls_pair), pa, pb);
-                pw[c / 2] = pack2<BF16>(pa, pb);
+                keep(c, pa, pb);
             };
             if (masked) {
 #pragma unroll
@@ -144,12 +156,17 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
             PH(1);
 #pragma unroll
             for (int c = 0; c < kCols; c += 2) {
-                const float2 pl = unpack2<BF16>(pw[c / 2]);
+                const float2 pl = W::kWindow ? make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1]))
+                                             : unpack2<BF16>(pw[c / 2]);
                 float da, db;
                 f2_unpack(f2_mul(f2_pack(pl.x, pl.y),
                                  f2_sub(f2_pack(__uint_as_float(dp[c]), __uint_as_float(dp[c + 1])), dl_pair)),
                           da, db);
                 dw[c / 2] = pack2<BF16>(da, db);
+                if (W::kWindow) {
+                    const float2 low = unpack2<BF16>(dw[c / 2]);
+                    row_sum = f2_add(row_sum, f2_pack(low.x, low.y));
+                }
             }
         }
         PH(7);
@@ -211,12 +228,28 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
     // end are not written by the store.
     const uint32_t acc = lane_base + kColGrad + ch0;
     const float mul = p.scale;
+    float rest = 0.f;  // windowed calls: minus the row sum of dS_low
+    if (W::kWindow) {
+        float* sums = reinterpret_cast<float*>(s_owner + Cfg<D>::kTileBytes);  // the dO tile is dead
+        float x0, x1;
+        f2_unpack(row_sum, x0, x1);
+        sums[wg * kTile + r] = x0 + x1;
+        mbar_arrive(&sh.sums_staged);
+        if (!mbar_wait(&sh.sums_staged, 0, abort_word, 152)) return;
+        if (!mbar_wait(&sh.mean_ready, 0, abort_word, 153)) return;
+        rest = -(sums[r] + sums[kTile + r]);
+    }
     constexpr int kStep = kHalf < 32 ? 16 : 32;
 #pragma unroll
     for (int c = 0; c < kHalf; c += kStep) {
         uint32_t v[kStep];
         tmem_ld(acc + c, v);
         tmem_wait_ld();
+        if (W::kWindow) {
+#pragma unroll
+            for (int e = 0; e < kStep; ++e)
+                v[e] = __float_as_uint(fmaf(rest, sh.mean[ch0 + c + e], __uint_as_float(v[e])));
+        }
 #pragma unroll
         for (int e = 0; e < kStep; e += 8) {
             uint4 o;

@@ -28,7 +28,7 @@ struct Cfg {
     static constexpr int kTileBytes = kTile * D * 2;
     static constexpr int kKeySlots = D == 128 ? 3 : 4;
     static constexpr int kValueSlots = D == 128 ? 2 : 4;
-    static constexpr int kSmemBytes = (2 + kKeySlots + kValueSlots) * kTileBytes + 1024 + 512;
+    static constexpr int kSmemBytes = (2 + kKeySlots + kValueSlots) * kTileBytes + 1024 + 1024;
 };
 
 struct Shared {
@@ -42,11 +42,50 @@ struct Shared {
     uint64_t ds_done;      // every consumer stored its dS_low
     uint64_t final_done;
     uint64_t out_staged;   // every consumer has put its part of the gradient tile into shared memory
+    uint64_t mean_ready;   // windowed calls: `mean` holds the sampled mean key
+    uint64_t sums_staged;  // windowed calls: every consumer has stored its row sum
     uint32_t tmem_base;
     int abort_word;
+    float mean[128];       // windowed calls: mean key of the tile, by channel
 };
 
 constexpr uint32_t kColS = 0, kColDp = 256, kColGrad = 384;
+
+// Windowed calls: the mean of 32 keys spread evenly over those the tile's rows see, by an otherwise idle warp while the
+// pipeline fills.  The exact dS of a row sums to zero, so dQ = sum dS K = sum dS (K - c) for any c; the rounded dS sums
+// to some R instead, and the epilogue takes R c off again.  Without that a per-channel offset of the keys multiplies
+// every rounding of dS (and the rounding of O inside delta): with offsets of 1.2 standard deviations the BF16 dQ was
+// 5.8e-3 from 64 bits.
+template <int D, class T, class W>
+__device__ __forceinline__ void mean_role(const AttnParams& p, const W& w, Shared& sh, int lane) {
+    int g, i;
+    w.begin(p, g, i);
+    if (!w.valid(g)) return;
+    int lo = window_span(w.start, w.owner0, p.window, p.Sk).lo;
+    int hi = window_span(w.start, min(p.Sq, w.owner0 + kTile) - 1, p.window, p.Sk).hi;
+    if (lo >= hi) lo = 0;  // the tile sees sinks only: at least key 0
+    hi = max(hi, 1);
+    constexpr int kVec = D / 32;  // channels per lane
+    const int d = lane * kVec;
+    const T* k = reinterpret_cast<const T*>(p.k) + (int64_t)w.b * p.ks[0] + (int64_t)(w.head / p.group) * p.ks[1] + d;
+    float sum[kVec] = {};
+#pragma unroll 8
+    for (int n = 0; n < 32; ++n) {
+        const T* row = k + (lo + (int64_t)(hi - lo) * n / 32) * p.ks[2];
+#pragma unroll
+        for (int e = 0; e < kVec; e += 2) {
+            if (d + e >= p.D) continue;
+            const uint32_t word = *reinterpret_cast<const uint32_t*>(row + e);
+            const float2 x = unpack2<std::is_same<T, __nv_bfloat16>::value>(word);
+            sum[e] += x.x;
+            sum[e + 1] += x.y;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) sh.mean[d + e] = sum[e] * (1.f / 32.f);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.mean_ready);
+}
 
 template <int D, class W>
 __device__ __forceinline__ void loader_role(const Maps& maps, const AttnParams& p, const W& w, Shared& sh,
