@@ -251,6 +251,39 @@ KFA_API int kfa_window_backward(const kfa_tensor* q, const kfa_tensor* k, const 
                        kfa_tensor* dk, kfa_tensor* dv, void* workspace, size_t workspace_bytes, int64_t start,
                        int64_t window, int64_t sinks, float scale, void* stream);
 
+/*
+ * Key/value cache held in 4 bits (no counterpart in the reference).  Keys and values are two tensors each:
+ *   codes  uint8 [B,H,capacity,D/2]     byte i of a row: channels 2i (low half) and 2i+1 (high half)
+ *   params 16-bit type [B,H,capacity,D/64,2]   per group of 64 channels: (scale, zero); value = zero + scale * code
+ * D is a multiple of 64 up to 512.  Strides are free except that the last axis of codes and the last two of params are
+ * dense and every row starts on a 16-byte (codes) / 4*(D/64)-byte (params) boundary.
+ *
+ * kfa_cache_write quantises k, v [B,H,n,D] (16-byte addressable rows) into the rows start_b + r, r < lengths[b]
+ * (lengths NULL: all n): scale = round16((max - min) / 15), zero = min, code = round_half_even((x - zero) / scale).  A
+ * group with a value that is not finite gets a NaN scale.  Rows that fall outside [0, capacity), and rows at or behind
+ * a sequence's length, are not written.  start_b is `start` or, where `starts` is given, starts[b] (int32 [B], device).
+ * kfa_cache_read writes the values of the rows start_b + r to k, v [B,H,n,D] (rounded once); rows outside the cache
+ * read as zeros.
+ *
+ * kfa_cache_attention is the attention of q [B,Hq,Sq,D] (unit channel stride, 16-byte addressable rows) to such a
+ * cache, D = 64 or 128: query row r stands at position start_b + r and sees the keys c <= start_b + r, and, with
+ * window > 0, of these only c > start_b + r - window or c < sinks.  Meant for the few rows of decoding (work is
+ * divided by keys; rows are taken 16 per K/V head at a time).  A row that sees no key is zero.  Values that no row sees
+ * are never looked at.  `workspace` holds kfa_cache_attention_workspace_bytes() bytes, 16-byte aligned.
+ */
+KFA_API int kfa_cache_write(const kfa_tensor* k, const kfa_tensor* v, kfa_tensor* k_codes, kfa_tensor* k_params,
+                    kfa_tensor* v_codes, kfa_tensor* v_params, const kfa_tensor* starts, const kfa_tensor* lengths,
+                    int64_t start, void* stream);
+KFA_API int kfa_cache_read(const kfa_tensor* k_codes, const kfa_tensor* k_params, const kfa_tensor* v_codes,
+                   const kfa_tensor* v_params, const kfa_tensor* starts, kfa_tensor* k, kfa_tensor* v, int64_t start,
+                   void* stream);
+KFA_API size_t kfa_cache_attention_workspace_bytes(const kfa_tensor* q, const kfa_tensor* k_codes, int64_t window,
+                   int64_t sinks);
+KFA_API int kfa_cache_attention(const kfa_tensor* q, const kfa_tensor* k_codes, const kfa_tensor* k_params,
+                   const kfa_tensor* v_codes, const kfa_tensor* v_params, const kfa_tensor* starts, kfa_tensor* out,
+                   void* workspace, size_t workspace_bytes, int64_t start, int64_t window, int64_t sinks, float scale,
+                   void* stream);
+
 /* Number of kernel variants configured so far / forget them.  Replace `cache_size`
  * and `clear_cache` (native.cpp:1055-1065). */
 KFA_API int kfa_cache_size(void);

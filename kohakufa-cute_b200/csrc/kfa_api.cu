@@ -1201,6 +1201,195 @@ int kfa_window_backward(const kfa_tensor* q, const kfa_tensor* k, const kfa_tens
     return 0;
 }
 
+}  // extern "C"
+
+namespace {
+
+// One half of a 4-bit cache (format: quantized_cache.cuh) against the first half's shape.
+int fill_cache_half(kfa::CacheView& view, const kfa_tensor* codes, const kfa_tensor* params, const kfa_tensor* like,
+                    int dtype) {
+    if (!codes || !params || !codes->data || !params->data || codes->dtype != KFA_U8 || codes->ndim != 4 ||
+        params->ndim != 5 || params->dtype != dtype)
+        return fail(KFA_INVALID_ARGUMENT,
+                    "quantized cache requires uint8 codes [B,H,capacity,D/2] and params [B,H,capacity,D/64,2] of the "
+                    "FP16/BF16 model type");
+    const int64_t bytes = codes->sizes[3], groups = bytes / 32;
+    for (int i = 0; i < 4; ++i)
+        if (codes->sizes[i] <= 0 || codes->sizes[i] > INT32_MAX || codes->sizes[i] != like->sizes[i])
+            return fail(KFA_INVALID_ARGUMENT, "quantized cache: K and V codes must be nonempty and of one shape");
+    if (bytes % 32 != 0 || groups > 8)
+        return fail(KFA_INVALID_ARGUMENT, "quantized cache requires head dimensions that are multiples of 64 up to 512");
+    for (int i = 0; i < 3; ++i)
+        if (params->sizes[i] != codes->sizes[i])
+            return fail(KFA_INVALID_ARGUMENT, "quantized cache: params do not match the codes");
+    if (params->sizes[3] != groups || params->sizes[4] != 2)
+        return fail(KFA_INVALID_ARGUMENT, "quantized cache: params do not match the codes");
+    bool ok = codes->strides[3] == 1 && reinterpret_cast<uintptr_t>(codes->data) % 16 == 0 && params->strides[4] == 1 &&
+              (groups == 1 || params->strides[3] == 2) && reinterpret_cast<uintptr_t>(params->data) % (4 * groups) == 0;
+    for (int i = 0; i < 3; ++i) {
+        view.cs[i] = codes->strides[i];
+        view.ps[i] = params->strides[i];
+        if (codes->sizes[i] > 1) ok = ok && view.cs[i] % 16 == 0 && view.ps[i] % (2 * groups) == 0;
+    }
+    if (!ok)
+        return fail(KFA_INVALID_ARGUMENT, "quantized cache: rows must be dense and aligned (codes 16 bytes, params one token)");
+    view.codes = static_cast<uint8_t*>(codes->data);
+    view.params = static_cast<uint16_t*>(params->data);
+    return 0;
+}
+
+int check_positions(const kfa_tensor* t, int64_t batch, const char* name) {
+    if (t && (!t->data || t->dtype != KFA_I32 || t->ndim != 1 || t->sizes[0] != batch || (batch > 1 && t->strides[0] != 1)))
+        return fail(KFA_INVALID_ARGUMENT, "quantized cache: %s must be contiguous int32 [batch]", name);
+    return 0;
+}
+
+// 16-bit rows [B, H, n, D] of a cache call: k or v.
+int check_cache_rows(const kfa_tensor* t, const kfa_tensor* codes) {
+    if (!t || !t->data || t->ndim != 4 || !is_half_type(t))
+        return fail(KFA_INVALID_ARGUMENT, "quantized cache requires 4D FP16/BF16 K/V rows");
+    if (t->sizes[0] != codes->sizes[0] || t->sizes[1] != codes->sizes[1] || t->sizes[3] != 2 * codes->sizes[3] ||
+        t->sizes[2] <= 0 || t->sizes[2] > INT32_MAX)
+        return fail(KFA_INVALID_ARGUMENT, "quantized cache: K/V rows do not match the cache's batch, heads and channels");
+    bool ok = t->strides[3] == 1 && reinterpret_cast<uintptr_t>(t->data) % 16 == 0;
+    for (int i = 0; i < 3; ++i) ok = ok && (t->sizes[i] == 1 || t->strides[i] % 8 == 0);
+    if (!ok) return fail(KFA_INVALID_ARGUMENT, "quantized cache requires 16-byte addressable K/V rows");
+    return 0;
+}
+
+int fill_cache_call(kfa::CacheCall& p, const kfa_tensor* k, const kfa_tensor* v, const kfa_tensor* k_codes,
+                    const kfa_tensor* k_params, const kfa_tensor* v_codes, const kfa_tensor* v_params,
+                    const kfa_tensor* starts, int64_t start) {
+    std::memset(&p, 0, sizeof(p));
+    if (!k_codes || k_codes->ndim != 4) return fail(KFA_INVALID_ARGUMENT, "quantized cache: null codes");
+    if (int e = check_cache_rows(k, k_codes)) return e;
+    if (int e = check_cache_rows(v, k_codes)) return e;
+    if (!same_shape(k, v) || k->dtype != v->dtype)
+        return fail(KFA_INVALID_ARGUMENT, "quantized cache requires K and V rows of one shape and type");
+    if (int e = fill_cache_half(p.half[0], k_codes, k_params, k_codes, k->dtype)) return e;
+    if (int e = fill_cache_half(p.half[1], v_codes, v_params, k_codes, k->dtype)) return e;
+    p.B = (int)k->sizes[0];
+    p.H = (int)k->sizes[1];
+    p.n = (int)k->sizes[2];
+    p.D = (int)k->sizes[3];
+    p.capacity = (int)k_codes->sizes[2];
+    if (int e = check_positions(starts, p.B, "starts")) return e;
+    if (2 * k->sizes[0] * k->sizes[1] * k->sizes[2] * (p.D / 8) / 256 > INT32_MAX - 1 || k->sizes[0] * k->sizes[1] > INT32_MAX)
+        return fail(KFA_TOO_LARGE, "quantized cache: too many rows in one call");
+    p.starts = starts ? static_cast<const int32_t*>(starts->data) : nullptr;
+    p.start = start;
+    for (int i = 0; i < 3; ++i) {
+        p.rs[0][i] = k->strides[i];
+        p.rs[1][i] = v->strides[i];
+    }
+    return 0;
+}
+
+int fill_cache_attention(kfa::CacheAttentionCall& p, const kfa_tensor* q, const kfa_tensor* codes, int64_t window,
+                         int64_t sinks) {
+    std::memset(&p, 0, sizeof(p));
+    if (!q || !codes || q->ndim != 4 || codes->ndim != 4 || !is_half_type(q))
+        return fail(KFA_INVALID_ARGUMENT, "cache attention requires 4D FP16/BF16 queries and a quantized cache");
+    for (int i = 0; i < 4; ++i)
+        if (q->sizes[i] <= 0 || q->sizes[i] > INT32_MAX || codes->sizes[i] <= 0 || codes->sizes[i] > INT32_MAX)
+            return fail(KFA_INVALID_ARGUMENT, "cache attention requires nonempty operands");
+    if (q->sizes[0] != codes->sizes[0] || q->sizes[1] % codes->sizes[1] != 0 || q->sizes[3] != 2 * codes->sizes[3])
+        return fail(KFA_INVALID_ARGUMENT,
+                    "cache attention requires matching batch and channels, and query heads divisible by K/V heads");
+    if (q->sizes[3] != 64 && q->sizes[3] != 128)
+        return fail(KFA_INVALID_ARGUMENT, "cache attention requires head dimensions 64 or 128");
+    if (q->sizes[0] * q->sizes[1] * q->sizes[2] > INT32_MAX / 64)
+        return fail(KFA_TOO_LARGE, "cache attention: too many query rows in one call");
+    if (window < 0 || sinks < 0) return fail(KFA_INVALID_ARGUMENT, "cache attention requires window >= 0 and sinks >= 0");
+    p.B = (int)q->sizes[0];
+    p.Hq = (int)q->sizes[1];
+    p.Hkv = (int)codes->sizes[1];
+    p.Sq = (int)q->sizes[2];
+    p.Sk = (int)codes->sizes[2];
+    p.D = (int)q->sizes[3];
+    p.group = p.Hq / p.Hkv;
+    // no window: longer than every position a 32-bit start can reach
+    p.window = window == 0 ? int64_t(1) << 40 : std::min<int64_t>(window, int64_t(1) << 40);
+    p.sinks = (int)std::min<int64_t>(sinks, p.Sk);
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int kfa_cache_write(const kfa_tensor* k, const kfa_tensor* v, kfa_tensor* k_codes, kfa_tensor* k_params,
+                    kfa_tensor* v_codes, kfa_tensor* v_params, const kfa_tensor* starts, const kfa_tensor* lengths,
+                    int64_t start, void* stream) {
+    if (int e = check_device_ok()) return e;
+    kfa::CacheCall p;
+    if (int e = fill_cache_call(p, k, v, k_codes, k_params, v_codes, v_params, starts, start)) return e;
+    if (int e = check_positions(lengths, p.B, "lengths")) return e;
+    p.lengths = lengths ? static_cast<const int32_t*>(lengths->data) : nullptr;
+    p.in[0] = k->data;
+    p.in[1] = v->data;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaError_t ce = timed("cache_write", st, [&] { return kfa::launch_cache_write(p, k->dtype == KFA_BF16, st); });
+    if (ce != cudaSuccess) return cuda_fail(ce, "cache write launch");
+    return 0;
+}
+
+int kfa_cache_read(const kfa_tensor* k_codes, const kfa_tensor* k_params, const kfa_tensor* v_codes,
+                   const kfa_tensor* v_params, const kfa_tensor* starts, kfa_tensor* k, kfa_tensor* v, int64_t start,
+                   void* stream) {
+    if (int e = check_device_ok()) return e;
+    kfa::CacheCall p;
+    if (int e = fill_cache_call(p, k, v, k_codes, k_params, v_codes, v_params, starts, start)) return e;
+    p.out[0] = k->data;
+    p.out[1] = v->data;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaError_t ce = timed("cache_read", st, [&] { return kfa::launch_cache_read(p, k->dtype == KFA_BF16, st); });
+    if (ce != cudaSuccess) return cuda_fail(ce, "cache read launch");
+    return 0;
+}
+
+size_t kfa_cache_attention_workspace_bytes(const kfa_tensor* q, const kfa_tensor* k_codes, int64_t window,
+                                           int64_t sinks) {
+    kfa::CacheAttentionCall p;
+    if (fill_cache_attention(p, q, k_codes, window, sinks)) return 0;
+    return kfa::cache_attention_workspace_bytes(p);
+}
+
+int kfa_cache_attention(const kfa_tensor* q, const kfa_tensor* k_codes, const kfa_tensor* k_params,
+                        const kfa_tensor* v_codes, const kfa_tensor* v_params, const kfa_tensor* starts, kfa_tensor* out,
+                        void* workspace, size_t workspace_bytes, int64_t start, int64_t window, int64_t sinks, float scale,
+                        void* stream) {
+    if (int e = check_device_ok()) return e;
+    kfa::CacheAttentionCall p;
+    if (int e = fill_cache_attention(p, q, k_codes, window, sinks)) return e;
+    if (int e = fill_cache_half(p.half[0], k_codes, k_params, k_codes, q->dtype)) return e;
+    if (int e = fill_cache_half(p.half[1], v_codes, v_params, k_codes, q->dtype)) return e;
+    if (int e = check_positions(starts, p.B, "starts")) return e;
+    if (int e = check_like(out, q, "out")) return e;
+    for (const kfa_tensor* t : {q, static_cast<const kfa_tensor*>(out)}) {
+        bool ok = t->data && t->strides[3] == 1 && reinterpret_cast<uintptr_t>(t->data) % 16 == 0;
+        for (int i = 0; i < 3; ++i) ok = ok && (t->sizes[i] == 1 || t->strides[i] % 8 == 0);
+        if (!ok) return fail(KFA_INVALID_ARGUMENT, "cache attention requires 16-byte addressable query rows");
+    }
+    const size_t need = kfa::cache_attention_workspace_bytes(p);
+    if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))
+        return fail(KFA_INVALID_ARGUMENT, "cache attention workspace too small or not 16-byte aligned");
+    p.q = q->data;
+    p.out = out->data;
+    for (int i = 0; i < 3; ++i) {
+        p.qs[i] = q->strides[i];
+        p.os[i] = out->strides[i];
+    }
+    p.starts = starts ? static_cast<const int32_t*>(starts->data) : nullptr;
+    p.start = start;
+    p.scale = scale;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaError_t ce = timed("cache_attention", st,
+                           [&] { return kfa::launch_cache_attention(p, q->dtype == KFA_BF16, workspace, st); });
+    if (ce != cudaSuccess) return cuda_fail(ce, "cache attention launch");
+    return 0;
+}
+
 int kfa_merge_splits(kfa_tensor* out, kfa_tensor* maximum, kfa_tensor* logsum, const kfa_tensor* part_out,
                      const kfa_tensor* part_maximum, const kfa_tensor* part_logsum, float scale, void* stream) {
     if (!out || !out->data || out->ndim != 4 || !is_half_type(out))

@@ -1,6 +1,7 @@
 // Host-side launch functions implemented by the kernel translation units.
 #pragma once
 #include "kfa_common.cuh"
+#include "quantized_cache.cuh"
 
 namespace kfa {
 
@@ -36,6 +37,12 @@ cudaError_t launch_finish_running(void* out, float* maximum, float* logsum, cons
 bool decode_forward_supported(const AttnParams& p);
 size_t decode_forward_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D);
 cudaError_t launch_decode_forward(const AttnParams& p, bool bf16, void* workspace, int* launches, cudaStream_t st);
+
+// 4-bit key/value cache: rows quantised into it, read back, attended to.
+cudaError_t launch_cache_write(const CacheCall& p, bool bf16, cudaStream_t st);
+cudaError_t launch_cache_read(const CacheCall& p, bool bf16, cudaStream_t st);
+size_t cache_attention_workspace_bytes(const CacheAttentionCall& p);
+cudaError_t launch_cache_attention(const CacheAttentionCall& p, bool bf16, void* workspace, cudaStream_t st);
 
 cudaError_t launch_neighborhood_forward(const AttnParams& p, bool bf16, cudaStream_t st);
 cudaError_t launch_neighborhood_backward(const AttnParams& p, bool bf16, int which, cudaStream_t st);

@@ -14,6 +14,14 @@ from .api import (
     sliding_window_attention,
 )
 
+from .cache import (
+    QuantizedCache,
+    quantized_cache,
+    quantized_cache_attention,
+    quantized_cache_read,
+    quantized_cache_write,
+)
+
 __version__ = "0.1.0"
 __all__ = [
     "attention",
@@ -22,4 +30,9 @@ __all__ = [
     "neighborhood_attention",
     "neighborhood_attention_3d",
     "sliding_window_attention",
+    "QuantizedCache",
+    "quantized_cache",
+    "quantized_cache_attention",
+    "quantized_cache_read",
+    "quantized_cache_write",
 ]

@@ -74,6 +74,11 @@ SIGNATURES = {
     "kfa_window_backward_workspace_bytes": (ctypes.c_size_t, [_TP, _TP] + [ctypes.c_int64] * 3),
     "kfa_window_backward": (ctypes.c_int, [_TP] * 10 + [ctypes.c_void_p, ctypes.c_size_t] + [ctypes.c_int64] * 3 +
                             [ctypes.c_float, ctypes.c_void_p]),
+    "kfa_cache_write": (ctypes.c_int, [_TP] * 8 + [ctypes.c_int64, ctypes.c_void_p]),
+    "kfa_cache_read": (ctypes.c_int, [_TP] * 7 + [ctypes.c_int64, ctypes.c_void_p]),
+    "kfa_cache_attention_workspace_bytes": (ctypes.c_size_t, [_TP, _TP, ctypes.c_int64, ctypes.c_int64]),
+    "kfa_cache_attention": (ctypes.c_int, [_TP] * 7 + [ctypes.c_void_p, ctypes.c_size_t] + [ctypes.c_int64] * 3 +
+                            [ctypes.c_float, ctypes.c_void_p]),
     "kfa_cache_size": (ctypes.c_int, []),
     "kfa_clear_cache": (None, []),
     "kfa_launch_count": (ctypes.c_uint64, []),
@@ -470,6 +475,45 @@ def window_backward(q, k, v, out, maximum, logsum, dout, start, window, sinks, s
         _check(lib.kfa_window_backward(*[_ref(r) for r in records], ctypes.c_void_p(workspace.data_ptr()), need, start,
                                        window, sinks, float(scale), _stream(q.device)))
     return dq, dk, dv
+
+
+def cache_write(k, v, k_codes, k_params, v_codes, v_params, starts, lengths, start):
+    """Quantises the rows of ``k`` and ``v`` into a 4-bit cache in place (``kfa_cache_write``)."""
+    lib = library()
+    k, v = (t if _rows_16_byte_addressable(t) else t.contiguous() for t in (_plain(k), _plain(v)))
+    with torch.cuda.device(k.device):
+        records = [describe(t) for t in (k, v, k_codes, k_params, v_codes, v_params, starts, lengths)]
+        _check(lib.kfa_cache_write(*[_ref(r) for r in records], start, _stream(k.device)))
+
+
+def cache_read(k_codes, k_params, v_codes, v_params, starts, start, length):
+    """(k, v) ``[B, H, length, D]``: the values of a 4-bit cache's rows (``kfa_cache_read``)."""
+    lib = library()
+    shape = (k_codes.shape[0], k_codes.shape[1], length, 2 * k_codes.shape[3])
+    with torch.cuda.device(k_codes.device):
+        k = torch.empty(shape, device=k_codes.device, dtype=k_params.dtype)
+        v = torch.empty_like(k)
+        records = [describe(t) for t in (k_codes, k_params, v_codes, v_params, starts, k, v)]
+        _check(lib.kfa_cache_read(*[_ref(r) for r in records], start, _stream(k.device)))
+    return k, v
+
+
+def cache_attention(q, k_codes, k_params, v_codes, v_params, starts, start, window, sinks, scale):
+    """Attention of a few query rows to a 4-bit cache (``kfa_cache_attention``); ``window`` 0 means none."""
+    lib = library()
+    q = _plain(q)
+    if not _rows_16_byte_addressable(q):
+        q = q.contiguous()
+    with torch.cuda.device(q.device):
+        out = torch.empty_like(q)
+        rq, rc = describe(q), describe(k_codes)
+        need = lib.kfa_cache_attention_workspace_bytes(_ref(rq), _ref(rc), window, sinks)
+        workspace = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
+        records = [rq, rc] + [describe(t) for t in (k_params, v_codes, v_params, starts, out)]
+        _check(lib.kfa_cache_attention(*[_ref(r) for r in records],
+                                       ctypes.c_void_p(workspace.data_ptr() if need else None), need, start, window,
+                                       sinks, float(scale), _stream(q.device)))
+    return out
 
 
 def running_state(q):

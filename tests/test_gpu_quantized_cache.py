@@ -1,0 +1,366 @@
+"""The 4-bit key/value cache: written bits against the definition, what stays untouched, reading back, and attention
+to it against FP64 mathematics on the values it holds."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+TYPES = (torch.bfloat16, torch.float16)
+
+
+def api():
+    import kohakufa_cute
+
+    return kohakufa_cute
+
+
+def native():
+    from kohakufa_cute import native as module
+
+    return module
+
+
+def rows(*shape, dtype, seed, offset=True):
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn(shape, generator=gen)
+    if offset:
+        x = x + 2 * torch.randn((1, shape[1], 1, shape[3]), generator=gen)
+    return x.to(dtype).cuda()
+
+
+def quantise(x):
+    """The definition, on the CPU in IEEE FP32: (codes as bytes, params) of x [..., D]."""
+    g = x.cpu().float().unflatten(-1, (-1, 64))
+    low, high = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
+    scale = ((high - low) / 15).to(x.dtype)
+    step = scale.float()
+    code = torch.where(step > 0, torch.round((g - low) / torch.where(step > 0, step, 1.0)), 0.0).clamp(0, 15)
+    code = code.flatten(-2).to(torch.uint8)
+    return code[..., 0::2] | (code[..., 1::2] << 4), torch.cat((scale, low.to(x.dtype)), -1)
+
+
+def values(codes, params):
+    """FP64 values of a cache half."""
+    codes, params = codes.cpu(), params.cpu().double()
+    code = torch.stack((codes & 15, codes >> 4), -1).flatten(-2).double().unflatten(-1, (-1, 64))
+    return (params[..., 1:2] + params[..., 0:1] * code).flatten(-2)
+
+
+def filled(B, H, capacity, D, dtype, seed):
+    """A cache whose every row holds something, and clones of its tensors."""
+    cache = api().quantized_cache(B, H, capacity, D, dtype=dtype)
+    api().quantized_cache_write(cache, rows(B, H, capacity, D, dtype=dtype, seed=seed),
+                                rows(B, H, capacity, D, dtype=dtype, seed=seed + 1, offset=False))
+    return cache
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", ((1, 1, 1, 64), (2, 3, 37, 128), (1, 2, 5, 256), (2, 1, 300, 512), (3, 2, 129, 64)))
+def test_written_bits_equal_the_definition(shape, dtype):
+    B, H, n, D = shape
+    k, v = rows(*shape, dtype=dtype, seed=n), rows(*shape, dtype=dtype, seed=n + 1, offset=False)
+    k[0, 0, 0, :64] = 3.0  # a group of equal values
+    v[0, 0, 0, :64] = 0.0
+    v[0, 0, 0, 5] = torch.finfo(dtype).tiny / 4  # the scale underflows, or nearly
+    cache = api().quantized_cache(B, H, n + 3, D, dtype=dtype)
+    api().quantized_cache_write(cache, k, v, start=2)
+    for x, codes, params in ((k, cache.k_codes, cache.k_params), (v, cache.v_codes, cache.v_params)):
+        want_codes, want_params = quantise(x)
+        assert torch.equal(codes[:, :, 2:n + 2].cpu(), want_codes)
+        assert torch.equal(params[:, :, 2:n + 2].cpu(), want_params)
+        for t in (codes, params):
+            assert not t[:, :, :2].any() and not t[:, :, n + 2:].any()
+    got = api().quantized_cache_read(cache, start=2, length=n)
+    for x, half, params in ((k, got[0], cache.k_params), (v, got[1], cache.v_params)):
+        want = values(*quantise(x))
+        u = torch.finfo(dtype).eps / 2
+        # reading rounds once; the product and the sum before it are one FP32 fused multiply-add
+        assert bool(((half.cpu().double() - want).abs() <= (u + 2**-22) * want.abs() + torch.finfo(dtype).tiny).all())
+        # a code is at most half a step from its value; the rounded scale adds 15 times its own rounding, at the top
+        # of the group, and a scale below the normal range is rounded in absolute steps
+        scale = params[:, :, 2:n + 2, :, :1].cpu().double().expand(*params.shape[:2], n, D // 64, 64).flatten(-2)
+        slack = scale * 0.5 + 15 * (u * scale + torch.finfo(dtype).tiny * torch.finfo(dtype).eps)
+        assert bool(((x.cpu().double() - want).abs() <= slack + 2**-22 * x.cpu().double().abs()).all())
+    assert native().device_status(reset=True) == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_ragged_rows_leave_the_rest_as_it_was(dtype):
+    B, H, n, D, capacity = 5, 2, 33, 128, 100
+    cache = filled(B, H, capacity, D, dtype, seed=3)
+    before = [t.clone() for t in cache]
+    k, v = rows(B, H, n, D, dtype=dtype, seed=8), rows(B, H, n, D, dtype=dtype, seed=9)
+    starts, lengths = [0, 67, 90, -10, 2**31 - 5], [33, 20, 33, 33, 0]
+    at = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    many = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    api().quantized_cache_write(cache, k, v, start=at, lengths=many)
+    want = [t.cpu().clone() for t in before]
+    for x, codes, params in ((k, want[0], want[1]), (v, want[2], want[3])):
+        new_codes, new_params = quantise(x)
+        for b in range(B):
+            for r in range(lengths[b]):
+                if 0 <= starts[b] + r < capacity:
+                    codes[b, :, starts[b] + r], params[b, :, starts[b] + r] = new_codes[b, :, r], new_params[b, :, r]
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(cache, want))
+    got = api().quantized_cache_read(cache, start=at, length=n)
+    for half, codes, params in ((got[0], want[0], want[1]), (got[1], want[2], want[3])):
+        whole = values(codes, params).to(dtype)
+        for b in range(B):
+            for r in range(n):
+                inside = 0 <= starts[b] + r < capacity
+                row = half[b, :, r].cpu()
+                if inside:
+                    torch.testing.assert_close(row, whole[b, :, starts[b] + r], atol=0, rtol=torch.finfo(dtype).eps)
+                else:
+                    assert not row.any()
+    long = torch.full((B,), 1000, dtype=torch.int32, device="cuda")  # longer than the rows given: all of them
+    api().quantized_cache_write(cache, k, v, start=0, lengths=long)
+    assert torch.equal(cache.k_codes[:, :, :n].cpu(), quantise(k)[0])
+
+
+def test_values_that_are_not_finite():
+    for dtype in TYPES:
+        k = rows(1, 1, 4, 128, dtype=dtype, seed=1)
+        k[0, 0, 0, 3], k[0, 0, 1, 70], k[0, 0, 2, 127] = float("nan"), float("inf"), -float("inf")
+        v = torch.full_like(k, torch.finfo(dtype).max)
+        v[..., ::2] = -torch.finfo(dtype).max
+        cache = api().quantized_cache(1, 1, 4, 128, dtype=dtype)
+        api().quantized_cache_write(cache, k, v)
+        got, wide = api().quantized_cache_read(cache)
+        want = values(*quantise(k)).to(dtype)
+        for r, group in ((0, 0), (1, 1), (2, 1)):
+            assert bool(torch.isnan(got[0, 0, r, group * 64:(group + 1) * 64]).all())
+            other = slice((1 - group) * 64, (2 - group) * 64)
+            torch.testing.assert_close(got[0, 0, r, other].cpu(), want[0, 0, r, other], atol=0, rtol=torch.finfo(dtype).eps)
+        if dtype == torch.float16:  # the widest range of FP16 is held
+            assert bool(torch.isfinite(wide).all()) and float((wide.float() - v.float()).abs().max()) <= 65504 * 2**-9
+        else:  # a range beyond FP32 is not
+            assert bool(torch.isnan(wide).all())
+
+
+def test_layouts_of_rows_and_cache():
+    B, H, n, D = 2, 4, 50, 128
+    k, v = rows(B, H, n, D, dtype=torch.bfloat16, seed=4), rows(B, H, n, D, dtype=torch.bfloat16, seed=5)
+    plain = api().quantized_cache(B, H, 64, D)
+    api().quantized_cache_write(plain, k, v, start=7)
+    seen = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (k, v)]  # [B, n, H, D] in memory
+    odd = torch.zeros(B, H, n, D + 1, device="cuda", dtype=torch.bfloat16)
+    odd[..., 1:] = v
+    big = api().quantized_cache(B + 1, H + 2, 80, D)
+    view = type(big)(*(t[1:, 1:H + 1, 8:72] for t in big))
+    api().quantized_cache_write(view, seen[0], odd[..., 1:], start=7)
+    for a, b in zip(plain, view):
+        assert torch.equal(a, b)
+    assert all(torch.equal(a, b) for a, b in zip(api().quantized_cache_read(plain), api().quantized_cache_read(view)))
+    assert not big.k_codes[0].any() and not big.k_codes[:, 0].any() and not big.k_codes[:, :, 72:].any()
+    q = rows(B, 2 * H, 1, D, dtype=torch.bfloat16, seed=6)
+    want = api().quantized_cache_attention(q, plain, query_start=50)
+    assert torch.equal(want, api().quantized_cache_attention(q, view, query_start=50))
+    spread = torch.zeros(B, 2 * H, 1, 2 * D, device="cuda", dtype=torch.bfloat16)
+    spread[..., ::2] = q
+    assert torch.equal(want, api().quantized_cache_attention(spread[..., ::2], view, query_start=50))
+
+
+def reference(q, cache, starts, window, sinks, scale=None):
+    """(out, bound) in FP64.  The bound: the output's rounding, and the probabilities' (each enters the product
+    multiplied by its key's scale and rounded, against codes less 8) - u |O| + u sum_c P 8 scale_c; FP32 steps (score
+    sums, ex2, normaliser) below 3e-5 of sum_c P |V| are covered by a tenth of u of it."""
+    B, Hq, Sq, D = q.shape
+    k, v = values(cache.k_codes, cache.k_params), values(cache.v_codes, cache.v_params)
+    steps = cache.v_params[..., 0].cpu().double().repeat_interleave(64, -1)
+    group, Sk = Hq // k.shape[1], k.shape[2]
+    pos = torch.tensor(starts)[:, None, None] + torch.arange(Sq)[None, :, None]
+    key = torch.arange(Sk)[None, None]
+    seen = key <= pos
+    if window:
+        seen = seen & ((key > pos - window) | (key < sinks))
+    seen = seen[:, None]
+    k, v, steps = (t.nan_to_num(0.0, 0.0, 0.0).repeat_interleave(group, 1) for t in (k, v, steps))
+    s = q.cpu().double() @ k.transpose(-1, -2) * (D**-0.5 if scale is None else scale)
+    blind = ~seen.any(-1, keepdim=True)
+    s = s.masked_fill(~seen, float("-inf")).masked_fill(blind, 0.0)
+    p = torch.softmax(s, -1).masked_fill(~seen, 0.0)
+    u = torch.finfo(q.dtype).eps / 2
+    out = p @ v
+    bound = u * out.abs() + u * 8 * (p @ steps) + 0.1 * u * (p @ v.abs()) + torch.finfo(q.dtype).tiny
+    return out, bound
+
+
+CASES = (
+    # Hq, Hkv, Sq, capacity, D, window, sinks, starts
+    (8, 8, 1, 1, 64, 0, 0, (0,)),
+    (8, 8, 1, 777, 64, 0, 0, (776,)),
+    (32, 8, 1, 2000, 128, 0, 0, (1999, 0, 31, 32, 1000)),
+    (8, 1, 4, 1500, 128, 0, 0, (1496, 5, -2, 2**31 - 1)),     # 32 rows per cache head, rows before the first key
+    (6, 2, 3, 900, 128, 100, 4, (897, 99, 0, 950)),           # nine rows; behind the cache: sinks and a part of the window
+    (16, 2, 1, 3000, 64, 256, 130, (2999, 385, 200)),
+    (4, 4, 2, 700, 128, 33, 0, (698, 64, 800)),               # the last sequence sees nothing
+    (5, 1, 7, 513, 64, 1, 1, (506, 0)),
+    (64, 8, 4, 1100, 128, 4096, 4, (1096, 512)),
+    (2, 1, 40, 400, 128, 64, 16, (360, 17)),                  # a longer piece
+)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", CASES)
+def test_attention_matches_fp64(case, dtype):
+    Hq, Hkv, Sq, capacity, D, window, sinks, starts = case
+    B = len(starts)
+    cache = filled(B, Hkv, capacity, D, dtype, seed=capacity)
+    q = rows(B, Hq, Sq, D, dtype=dtype, seed=capacity + 7, offset=False) * 1.5
+    for b, start in enumerate(starts):  # behind the last position there may be anything
+        end = min(capacity, max(0, start + Sq))
+        for codes, params in (cache[:2], cache[2:]):
+            codes[b, :, end:], params[b, :, end:] = 255, float("nan")
+    at = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    for scale in (None, -0.2):
+        want, bound = reference(q, cache, starts, window, sinks, scale)
+        got = api().quantized_cache_attention(q, cache, query_start=at, window=window or None, sinks=sinks, scale=scale)
+        assert got.shape == q.shape and got.dtype == dtype and bool(torch.isfinite(got).all())
+        far = ((got.cpu().double() - want).abs() - bound).max()
+        assert float(far) <= 0, f"an element is {float(far):.3e} beyond its roundings"
+        again = api().quantized_cache_attention(q, cache, query_start=at, window=window or None, sinks=sinks, scale=scale)
+        assert torch.equal(got, again)
+    if 0 <= starts[0] < 2**31 - 1:
+        one = type(cache)(*(t[:1] for t in cache))
+        same = api().quantized_cache_attention(q[:1], one, query_start=starts[0], window=window or None, sinks=sinks,
+                                               scale=-0.2)
+        want, bound = reference(q[:1], one, starts[:1], window, sinks, -0.2)
+        assert bool(((same.cpu().double() - want).abs() <= bound).all())
+    assert native().device_status(reset=True) == 0
+
+
+def test_a_zero_scale_averages_the_visible_values():
+    cache = filled(1, 2, 300, 128, torch.bfloat16, seed=5)
+    q = rows(1, 4, 1, 128, dtype=torch.bfloat16, seed=6)
+    want, bound = reference(q, cache, (200,), 40, 3, 0.0)
+    got = api().quantized_cache_attention(q, cache, query_start=200, window=40, sinks=3, scale=0.0)
+    assert bool(((got.cpu().double() - want).abs() <= bound).all())
+
+
+def test_large_logits_pick_one_key():
+    """Scores that differ by hundreds: the softmax is a copy of one value row."""
+    for dtype in TYPES:
+        cache = filled(1, 1, 2000, 128, dtype, seed=11)
+        q = (rows(1, 8, 1, 128, dtype=dtype, seed=12) * 100).to(dtype)
+        want, bound = reference(q, cache, (1999,), 0, 0)
+        got = api().quantized_cache_attention(q, cache, query_start=1999)
+        # FP32 score sums of magnitude up to 100 * 128 * 10 are off by 2^-22 of that: 0.03, a factor 1.03 in P where a
+        # second key comes close (bounded by the values' own size), nothing where it does not
+        slack = 0.03 * values(cache.v_codes, cache.v_params).abs().max()
+        assert bool(((got.cpu().double() - want).abs() <= bound + slack).all())
+
+
+def test_captured_decoding_follows_new_positions():
+    """Write one token, attend, in a graph; replayed with other rows and positions it equals eager calls."""
+    B, Hq, Hkv, D, capacity = 3, 8, 2, 128, 1200
+    eager, held = filled(B, Hkv, capacity, D, torch.bfloat16, 1), filled(B, Hkv, capacity, D, torch.bfloat16, 1)
+    k, v = rows(B, Hkv, 1, D, dtype=torch.bfloat16, seed=2), rows(B, Hkv, 1, D, dtype=torch.bfloat16, seed=3)
+    q = rows(B, Hq, 1, D, dtype=torch.bfloat16, seed=4)
+    at = torch.tensor([700, 3, 0], dtype=torch.int32, device="cuda")
+
+    def step(cache, window):
+        api().quantized_cache_write(cache, k, v, start=at)
+        return api().quantized_cache_attention(q, cache, query_start=at, window=window, sinks=4 if window else 0)
+
+    graphs = []
+    for window in (None, 300):
+        step(held, window)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(held, window)
+        graphs.append((graph, out, window))
+    step(eager, None)
+    for i, positions in enumerate(([701, 4, 1], [1199, 600, 0], [20, 1198, 333])):
+        at.copy_(torch.tensor(positions, dtype=torch.int32))
+        for t in (k, v, q):
+            t.copy_(torch.randn(t.shape, generator=torch.Generator().manual_seed(i)).to(t.dtype))
+        for graph, out, window in graphs:
+            want = step(eager, window)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+    assert all(torch.equal(a, b) for a, b in zip(eager, held))
+
+
+def test_another_stream_and_two_calls_at_once():
+    cache = filled(2, 2, 4000, 128, torch.bfloat16, 21)
+    q = rows(2, 8, 1, 128, dtype=torch.bfloat16, seed=22)
+    want = api().quantized_cache_attention(q, cache, query_start=3999)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    results = []
+    for _ in range(10):
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                results.append(api().quantized_cache_attention(q, cache, query_start=3999))
+    torch.cuda.synchronize()
+    assert all(torch.equal(want, r) for r in results)
+
+
+def test_decoding_steps_follow_a_prompt():
+    """A prompt written and attended to, then tokens one by one: each step equals attention on what was read back."""
+    B, Hq, Hkv, D, prompt, steps, window, sinks = 2, 8, 2, 128, 300, 4, 128, 4
+    cache = api().quantized_cache(B, Hkv, prompt + steps, D)
+    k, v = (rows(B, Hkv, prompt + steps, D, dtype=torch.bfloat16, seed=s) for s in (31, 32))
+    q = rows(B, Hq, prompt + steps, D, dtype=torch.bfloat16, seed=33)
+    api().quantized_cache_write(cache, k[:, :, :prompt], v[:, :, :prompt])
+    kq, vq = api().quantized_cache_read(cache, length=prompt)
+    out = api().sliding_window_attention(q[:, :, :prompt], kq, vq, window=window, sinks=sinks)
+    want, bound = reference(q[:, :, :prompt], type(cache)(*(t[:, :, :prompt] for t in cache)), (0, 0), window, sinks)
+    # the window operator reads K and V rounded to 16 bits, which the direct definition does not: one more rounding of
+    # V (u sum P |V|), and scores off by u sum |q| |k| / sqrt(D), i.e. P off by that factor
+    u = torch.finfo(torch.bfloat16).eps / 2
+    kd, vd = (t.cpu().double().repeat_interleave(Hq // Hkv, 1) for t in (kq, vq))
+    factor = u * (q[:, :, :prompt].cpu().double().abs() @ kd.abs().transpose(-1, -2)).amax(-1, keepdim=True) * D**-0.5
+    slack = (2 * u + 2 * factor) * vd.abs().amax(2, keepdim=True)
+    assert bool(((out.cpu().double() - want).abs() <= bound + slack).all())
+    for t in range(prompt, prompt + steps):
+        api().quantized_cache_write(cache, k[:, :, t:t + 1], v[:, :, t:t + 1], start=t)
+        got = api().quantized_cache_attention(q[:, :, t:t + 1], cache, query_start=t, window=window, sinks=sinks)
+        want, bound = reference(q[:, :, t:t + 1], cache, (t, t), window, sinks)
+        assert bool(((got.cpu().double() - want).abs() <= bound).all())
+    assert native().device_status(reset=True) == 0
+
+
+def test_compiled_route():
+    cache, other = (filled(2, 2, 200, 64, torch.float16, 41) for _ in range(2))
+    k, v = rows(2, 2, 3, 64, dtype=torch.float16, seed=42), rows(2, 2, 3, 64, dtype=torch.float16, seed=43)
+    q = rows(2, 4, 3, 64, dtype=torch.float16, seed=44)
+
+    def step(q, k, v, cache):
+        api().quantized_cache_write(cache, k, v, start=100)
+        out = api().quantized_cache_attention(q, cache, query_start=100, window=50, sinks=2)
+        return out, *api().quantized_cache_read(cache, start=90, length=13)
+
+    want = step(q, k, v, cache)
+    got = torch.compile(step, fullgraph=True, backend="aot_eager")(q, k, v, other)
+    assert all(torch.equal(a, b) for a, b in zip((*want, *cache), (*got, *other)))
+
+
+def test_refusals():
+    cache = api().quantized_cache(2, 2, 16, 64)
+    k = rows(2, 2, 4, 64, dtype=torch.bfloat16, seed=1)
+    q = rows(2, 4, 1, 64, dtype=torch.bfloat16, seed=1)
+    write, read, attend = api().quantized_cache_write, api().quantized_cache_read, api().quantized_cache_attention
+    for call in (lambda: write(cache, k, k, start=13), lambda: write(cache, k, k[:, :, :3]),
+                 lambda: write(cache, k.half(), k.half()), lambda: write(cache, k[:1], k[:1]),
+                 lambda: write(cache, k.cpu(), k.cpu()), lambda: write(cache, k, k, lengths=4),
+                 lambda: write(cache, k.clone().requires_grad_(True), k),
+                 lambda: read(cache, start=10, length=7), lambda: read(cache, length=0), lambda: read(cache, start=16),
+                 lambda: read(cache, start=torch.zeros(2, dtype=torch.int32, device="cuda")),
+                 lambda: attend(q[:, :3], cache, query_start=0), lambda: attend(q.half(), cache, query_start=0),
+                 lambda: attend(q, cache, query_start=0, sinks=2), lambda: attend(q, cache, query_start=0, window=0),
+                 lambda: attend(q.clone().requires_grad_(True), cache, query_start=0),
+                 lambda: attend(q, cache, query_start=0, scale=float("inf")),
+                 lambda: attend(q, cache, query_start=torch.zeros(2, dtype=torch.int64, device="cuda"))):
+        with pytest.raises(ValueError):
+            call()
+    wide = api().quantized_cache(1, 1, 4, 256)
+    with pytest.raises(ValueError, match="64 and 128"):
+        attend(rows(1, 1, 1, 256, dtype=torch.bfloat16, seed=1), wide, query_start=0)
+    shifted = torch.zeros(2 * 2 * 16 * 32 + 8, dtype=torch.uint8, device="cuda")[8:].view(2, 2, 16, 32)
+    with pytest.raises(ValueError, match="aligned"):
+        write(cache._replace(k_codes=shifted), k, k)
+    assert all(not t.any() for t in cache)
+    assert native().device_status(reset=True) == 0
