@@ -1,0 +1,738 @@
+// Attention of a few query rows per K/V head to a long key/value cache, held in 16 bits or in 4 (quantized_cache.cuh),
+// with positions per sequence and the sliding window and sinks of window.cuh.
+//
+// Such a call is bound by the HBM time of the keys and values that some row sees.  To keep the arithmetic below that,
+// the two products run on the tensor cores' register path (mma m16n8k16), where a fragment of eight query rows costs
+// nothing extra and the cache goes from shared memory to registers once:
+//   S^T = K q^T     A = 16 tokens x 16 channels, B = 16 channels x 8 query rows
+//   O^T = V^T P^T   A = 16 channels x 16 tokens, B = 16 tokens x 8 query rows (P^T by two 8x8 register transposes)
+// (tcgen05 wants 128 rows of operand A in shared memory: the 4-bit cache would have to be widened into it, 4 x the
+// bytes, and its rows are tokens only in one of the two products.)
+//
+// 4-bit caches are never widened to values.  Codes become 16-bit floats in two instructions per pair (shift, and one
+// logic operation that masks the code into the mantissa of 16.0: 16 + code), and scale and zero of a token's group of
+// 64 channels are applied to sums, in FP32:
+//   s    = sum_g  scale_g * (sum_d q_d (16 + code_d))  +  (zero_g - 16 scale_g) * (sum_d q_d)
+//   o_d  = sum_t  round16(p_t scale_g) * (code_d - 8)  +  sum_t p_t (zero_g + 8 scale_g)
+// The codes less 8 are centred, so the one rounding, of p * scale, weighs like the rounding of p against 16-bit values.
+//
+// Work is cut evenly however ragged the batch is: the blocks of tokens that the units (sequence, K/V head, chunk of
+// query rows) have to read are numbered through, and each CTA takes an equal piece of that line; where a unit spans
+// several CTAs their partial (maximum, sum, accumulator) are merged by a second, dependent launch.  The lengths come
+// from device memory, so a captured call follows new positions.  Within a CTA the warps take blocks in turn, each with
+// its own ring of asynchronous copies.
+#pragma once
+#include "kfa_common.cuh"
+#include "quantized_cache.cuh"
+#include "sm100_ptx.cuh"
+#include "window.cuh"
+
+#include <type_traits>
+
+namespace kfa {
+
+struct RowsCall {
+    CacheAttentionCall c;
+    const void* kv[2];    // 16-bit cache: keys, values
+    int64_t kvs[2][3];    // batch, head, token strides (elements)
+    int rows, chunks;     // query rows per K/V head, pieces of 8 * NT of them
+    int ctas;
+    float* part_o;        // [ctas][2][8 NT][D]: a CTA's first and last piece of a unit
+    float* part_ml;       // [ctas][2][8 NT][2]: maximum, sum
+};
+
+namespace rows {
+
+constexpr int kWarps = 4;
+
+// CTAs per SM that registers and shared memory allow (the launch bounds hold the compiler to it).
+template <int D, bool Q4, int NT>
+constexpr int resident() {
+    return Q4 ? (D == 64 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 3 : 2)) : (D == 64 ? 3 : 2);
+}
+
+template <int D, bool Q4>
+struct Cfg {
+    static constexpr int kGroups = D / kCacheGroup;
+    static constexpr int kBlock = Q4 ? 32 : 16;                // tokens per block
+    static constexpr int kRow = Q4 ? D / 2 : D * 2;            // bytes of a token's codes or channels
+    static constexpr int kParam = Q4 ? 4 * kGroups : 0;        // bytes of a token's scales and zeros
+    static constexpr int kHalf = kBlock * (kRow + kParam);     // one block of keys or of values
+    static constexpr int kStage = 2 * kHalf;
+    static constexpr int kStages = Q4 ? (D == 64 ? 4 : 3) : (D == 64 ? 4 : 3);
+    static constexpr int kRing = kWarps * kStages * kStage;
+};
+
+// ------------------------------------------------------------------ the line of blocks
+struct Blocks {
+    int sinks, first, count;  // blocks [0, sinks), then `count - sinks` blocks from `first` on
+    __device__ __forceinline__ int block(int i) const { return i < sinks ? i : first + (i - sinks); }
+};
+
+__device__ __forceinline__ Blocks blocks_of(const CacheAttentionCall& c, int64_t start, int size) {
+    const WindowSpan a = window_span(start, 0, c.window, c.Sk), z = window_span(start, c.Sq - 1, c.window, c.Sk);
+    Blocks n;
+    n.sinks = (min(c.sinks, z.hi) + size - 1) / size;
+    n.first = max(a.lo / size, n.sinks);
+    n.count = n.sinks + (a.lo < z.hi ? max((z.hi + size - 1) / size - n.first, 0) : 0);
+    return n;
+}
+
+__device__ __forceinline__ int64_t start_of(const CacheAttentionCall& c, int b) {
+    return c.starts ? (int64_t)c.starts[b] : c.start;
+}
+
+// Blocks of the whole call; every lane of the (converged) warp returns the sum.
+__device__ __forceinline__ int64_t total_blocks(const CacheAttentionCall& c, int64_t units, int size) {
+    int64_t sum = 0;
+    for (int b = threadIdx.x & 31; b < c.B; b += 32) sum += blocks_of(c, start_of(c, b), size).count;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum * units;
+}
+
+// The sequence that position `at` of the line falls into and the position of its first block.
+__device__ __forceinline__ int sequence_at(const CacheAttentionCall& c, int64_t units, int size, int64_t at, int64_t& base) {
+    const int lane = threadIdx.x & 31;
+    int64_t before = 0;
+    for (int b0 = 0; b0 < c.B; b0 += 32) {
+        int64_t sum = b0 + lane < c.B ? blocks_of(c, start_of(c, b0 + lane), size).count * units : 0;
+        const int64_t mine = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += up;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, at < before + sum);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            base = before + __shfl_sync(0xffffffffu, sum - mine, src);
+            return b0 + src;
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    base = before;
+    return c.B;  // behind the line
+}
+
+// CTAs that get blocks (every one of them at least one), the first block of CTA `i`, and the CTA that owns block `at`.
+__device__ __forceinline__ int used_ctas(int64_t total, int ctas) { return (int)min((int64_t)ctas, total); }
+__device__ __forceinline__ int64_t cta_begin(int64_t total, int ctas, int i) { return total * i / ctas; }
+__device__ __forceinline__ int cta_of(int64_t total, int ctas, int64_t at) { return (int)(((at + 1) * ctas - 1) / total); }
+
+// ------------------------------------------------------------------ instructions
+template <bool BF16>
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+    if constexpr (BF16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+template <bool TRANS>
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    if constexpr (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// Asynchronous copy of N bytes (zeros when `live` is false: nothing is read then).
+template <int N>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool live) {
+    const int bytes = live ? N : 0;
+    if constexpr (N == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Code t (0..3) of both halves of a word as a pair of 16-bit floats 16 + code.
+template <bool BF16, int t>
+__device__ __forceinline__ uint32_t widen(uint32_t w) {
+    constexpr int to = BF16 ? 3 : 6, shift = to - 4 * t;  // where the four bits go in the mantissa
+    constexpr uint32_t mask = BF16 ? 0x00780078u : 0x03c003c0u, sixteen = BF16 ? 0x41804180u : 0x4c004c00u;
+    const uint32_t x = shift >= 0 ? w << (shift >= 0 ? shift : 0) : w >> (shift < 0 ? -shift : 0);
+    return (x & mask) | sixteen;
+}
+// The same less 24: code - 8, exactly.
+template <bool BF16, int t>
+__device__ __forceinline__ uint32_t centred(uint32_t w) {
+    const uint32_t x = widen<BF16, t>(w);
+    uint32_t y;
+    if constexpr (BF16) asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x41c041c0u));
+    else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x4e004e00u));
+    return y;
+}
+
+// ------------------------------------------------------------------ one unit's piece, one warp
+// Running state of a warp over its blocks: thread (g, i) = (lane / 4, lane % 4) holds the maximum of query rows 2i and
+// 2i + 1, its own part of their sums, and the accumulator of those rows at its channels (channel_of).
+template <int D, bool Q4, int NT>
+struct State {
+    static constexpr int kTiles = D / 16;
+    float m[NT][2], l[NT][2], z[NT][2][Q4 ? D / kCacheGroup : 1];
+    float o[kTiles][NT][4];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                m[n][e] = -INFINITY;
+                l[n][e] = 0.f;
+#pragma unroll
+                for (int g = 0; g < (Q4 ? D / kCacheGroup : 1); ++g) z[n][e][g] = 0.f;
+            }
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[t][n][e] = 0.f;
+    }
+};
+
+// Channel of accumulator row `upper` * 8 + g of tile t.
+template <bool Q4>
+__device__ __forceinline__ int channel_of(int t, int g, int upper) {
+    return Q4 ? (t >> 2) * kCacheGroup + 8 * g + (t & 3) + 4 * upper : 16 * t + g + 8 * upper;
+}
+
+// Scores of a block in S[mt][n][e] (token mt * 16 + g + 8 * (e >> 1), query row 2i + (e & 1) of row tile n).
+template <typename T, int D, int NT>
+__device__ __forceinline__ void scores_q4(float (&s)[2][NT][4], const uint8_t* codes, const uint8_t* params,
+                                          const uint32_t (&qf)[NT][D / 16][2], const float (&qsum)[NT][2][D / 64], int g,
+                                          int i) {
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    using C = Cfg<D, true>;
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[mt][n][e] = 0.f;
+        const int t0 = mt * 16 + g;
+#pragma unroll
+        for (int grp = 0; grp < C::kGroups; ++grp) {
+            uint32_t w[2][2], pr[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint2 pair = *reinterpret_cast<const uint2*>(codes + (t0 + 8 * u) * C::kRow + grp * 32 + i * 8);
+                w[u][0] = pair.x;
+                w[u][1] = pair.y;
+                pr[u] = *reinterpret_cast<const uint32_t*>(params + (t0 + 8 * u) * C::kParam + grp * 4);
+            }
+            float acc[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const uint32_t a = w[0][x], b = w[1][x];
+                const uint32_t a0 = widen<BF16, 0>(a), a1 = widen<BF16, 1>(a), a2 = widen<BF16, 2>(a), a3 = widen<BF16, 3>(a);
+                const uint32_t b0 = widen<BF16, 0>(b), b1 = widen<BF16, 1>(b), b2 = widen<BF16, 2>(b), b3 = widen<BF16, 3>(b);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    mma<BF16>(acc[n], a0, b0, a1, b1, qf[n][grp * 4 + x * 2][0], qf[n][grp * 4 + x * 2][1]);
+                    mma<BF16>(acc[n], a2, b2, a3, b3, qf[n][grp * 4 + x * 2 + 1][0], qf[n][grp * 4 + x * 2 + 1][1]);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const float2 sz = unpack2<BF16>(pr[u]);
+                const float off = fmaf(sz.x, -16.f, sz.y);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        s[mt][n][2 * u + e] = fmaf(sz.x, acc[n][2 * u + e], fmaf(off, qsum[n][e][grp], s[mt][n][2 * u + e]));
+            }
+        }
+    }
+}
+
+template <typename T, int D, int NT>
+__device__ __forceinline__ void scores_16(float (&s)[1][NT][4], uint32_t tile, const uint32_t (&qf)[NT][D / 16][2], int lane) {
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[0][n][e] = 0.f;
+    const int row = (lane & 7) + (lane & 8);
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+        uint32_t a[4];
+        const int chunk = 2 * ks + (lane >> 4);
+        ldmatrix4<false>(a, tile + row * (D * 2) + ((chunk ^ (row & 7)) << 4));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma<BF16>(s[0][n], a[0], a[1], a[2], a[3], qf[n][ks][0], qf[n][ks][1]);
+    }
+}
+
+// One block: softmax and both products.  CLEAN: every row sees every token of it.
+template <typename T, int D, bool Q4, int NT, bool CLEAN>
+__device__ __forceinline__ void block_step(State<D, Q4, NT>& st, const uint8_t* stage, const uint32_t (&qf)[NT][D / 16][2],
+                                           const float (&qsum)[NT][2][D / 64], const CacheAttentionCall& c, int64_t start,
+                                           int key0, int row0, float c2, int lane) {
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    using C = Cfg<D, Q4>;
+    constexpr int MT = C::kBlock / 16;
+    const int g = lane >> 2, i = lane & 3;
+    float s[MT][NT][4];
+    if constexpr (Q4) scores_q4<T, D, NT>(s, stage, stage + C::kBlock * C::kRow, qf, qsum, g, i);
+    else scores_16<T, D, NT>(s, smem_u32(stage), qf, lane);
+
+    bool grown = false;
+    float mn[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            if (!CLEAN) {
+                const WindowSpan span = window_span(start, (row0 + n * 8 + 2 * i + e) % c.Sq, c.window, c.Sk);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        if (!window_sees(span, c.sinks, key0 + mt * 16 + g + 8 * u)) s[mt][n][2 * u + e] = -INFINITY;
+            }
+            float mx = st.m[n][e];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) mx = max3(mx, s[mt][n][e], s[mt][n][2 + e]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            mn[n][e] = mx;
+            grown = grown || mx > st.m[n][e];
+        }
+    if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float alpha = st.m[n][e] == -INFINITY ? 0.f : ex2((st.m[n][e] - mn[n][e]) * c2);
+                st.m[n][e] = mn[n][e];
+                st.l[n][e] *= alpha;
+                if (Q4) {
+#pragma unroll
+                    for (int grp = 0; grp < C::kGroups; ++grp) st.z[n][e][Q4 ? grp : 0] *= alpha;
+                }
+#pragma unroll
+                for (int t = 0; t < D / 16; ++t) {
+                    st.o[t][n][e] *= alpha;
+                    st.o[t][n][2 + e] *= alpha;
+                }
+            }
+    }
+    // probabilities, in place of the scores
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float m = !CLEAN && st.m[n][e] == -INFINITY ? 0.f : st.m[n][e];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float& x = s[mt][n][2 * u + e];
+                    const float p = ex2((x - m) * c2);
+                    x = !CLEAN && x == -INFINITY ? 0.f : p;
+                    st.l[n][e] += x;
+                }
+        }
+
+    const uint8_t* values = stage + C::kHalf;
+    if constexpr (Q4) {
+        const uint8_t* params = values + C::kBlock * C::kRow;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+            for (int grp = 0; grp < C::kGroups; ++grp) {
+                uint32_t bf[NT][2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const float2 sz = unpack2<BF16>(*reinterpret_cast<const uint32_t*>(params + (mt * 16 + g + 8 * u) * C::kParam + grp * 4));
+                    const float off = fmaf(sz.x, 8.f, sz.y);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const float p0 = s[mt][n][2 * u], p1 = s[mt][n][2 * u + 1];
+                        float w0 = p0 * sz.x, w1 = p1 * sz.x;
+                        if (CLEAN) {
+                            st.z[n][0][grp] = fmaf(p0, off, st.z[n][0][grp]);
+                            st.z[n][1][grp] = fmaf(p1, off, st.z[n][1][grp]);
+                        } else {  // a token this row does not see may hold anything
+                            w0 = p0 == 0.f ? 0.f : w0;
+                            w1 = p1 == 0.f ? 0.f : w1;
+                            st.z[n][0][grp] += p0 == 0.f ? 0.f : p0 * off;
+                            st.z[n][1][grp] += p1 == 0.f ? 0.f : p1 * off;
+                        }
+                        bf[n][u] = transpose8(pack2<BF16>(w0, w1));
+                    }
+                }
+                uint32_t w[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int token = mt * 16 + 2 * i + (x & 1) + (x >> 1) * 8;
+                    w[x] = *reinterpret_cast<const uint32_t*>(values + token * C::kRow + grp * 32 + g * 4);
+                }
+                const uint32_t lo0 = __byte_perm(w[0], w[1], 0x5410), hi0 = __byte_perm(w[0], w[1], 0x7632);
+                const uint32_t lo1 = __byte_perm(w[2], w[3], 0x5410), hi1 = __byte_perm(w[2], w[3], 0x7632);
+                auto tile = [&](auto t_) {
+                    constexpr int t = decltype(t_)::value;
+                    const uint32_t a0 = centred<BF16, t>(lo0), a1 = centred<BF16, t>(hi0);
+                    const uint32_t a2 = centred<BF16, t>(lo1), a3 = centred<BF16, t>(hi1);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma<BF16>(st.o[grp * 4 + t][n], a0, a1, a2, a3, bf[n][0], bf[n][1]);
+                };
+                tile(std::integral_constant<int, 0>{});
+                tile(std::integral_constant<int, 1>{});
+                tile(std::integral_constant<int, 2>{});
+                tile(std::integral_constant<int, 3>{});
+            }
+        }
+    } else {
+        uint32_t bf[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) bf[n][u] = transpose8(pack2<BF16>(s[0][n][2 * u], s[0][n][2 * u + 1]));
+        const int row = (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) {
+            uint32_t a[4];
+            const int chunk = 2 * t + ((lane >> 3) & 1);
+            ldmatrix4<true>(a, smem_u32(values) + row * (D * 2) + ((chunk ^ (row & 7)) << 4));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma<BF16>(st.o[t][n], a[0], a[1], a[2], a[3], bf[n][0], bf[n][1]);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ kernels
+template <typename T, int D, bool Q4, int NT>
+__global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_rows(const RowsCall p) {
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    using C = Cfg<D, Q4>;
+    constexpr int R = 8 * NT;
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ float sm_m[kWarps][R], sm_l[kWarps][R];
+    const CacheAttentionCall& c = p.c;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may be scheduled; it waits for this grid
+    const int64_t units = (int64_t)c.Hkv * p.chunks;
+    const int64_t total = total_blocks(c, units, C::kBlock);
+    const int ctas = used_ctas(total, p.ctas);
+    if ((int)blockIdx.x >= ctas) return;
+    const int64_t begin = cta_begin(total, ctas, blockIdx.x), end = cta_begin(total, ctas, blockIdx.x + 1);
+    uint8_t* my_ring = ring + warp * C::kStages * C::kStage;
+    const float c2 = fabsf(c.scale) * kLog2e;
+    State<D, Q4, NT> st;
+
+    for (int64_t at = begin; at < end;) {
+        int64_t base;
+        const int b = sequence_at(c, units, C::kBlock, at, base);
+        const int64_t start = start_of(c, b);
+        const Blocks blocks = blocks_of(c, start, C::kBlock);
+        const int unit = (int)((at - base) / blocks.count), from = (int)((at - base) - (int64_t)unit * blocks.count);
+        const int count = (int)min(end - at, (int64_t)(blocks.count - from));
+        const int kvh = unit / p.chunks, row0 = unit % p.chunks * R;
+        const WindowSpan low = window_span(start, 0, c.window, c.Sk), high = window_span(start, c.Sq - 1, c.window, c.Sk);
+
+        // the copies of this warp's block `n` (blocks warp, warp + kWarps, ... of the piece) into its ring
+        const int mine = count > warp ? (count - warp + kWarps - 1) / kWarps : 0;
+        auto request = [&](int n) {
+            if (n < mine) {
+                const int key0 = blocks.block(from + warp + n * kWarps) * C::kBlock;
+                const uint32_t dst = smem_u32(my_ring + (n % C::kStages) * C::kStage);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    constexpr int kChunks = C::kRow / 16;
+                    const uint8_t* src;
+                    int64_t step;
+                    if constexpr (Q4) {
+                        const CacheView& v = c.half[half];
+                        src = v.codes + b * v.cs[0] + kvh * v.cs[1];
+                        step = v.cs[2];
+                    } else {
+                        src = static_cast<const uint8_t*>(p.kv[half]) + 2 * (b * p.kvs[half][0] + kvh * p.kvs[half][1]);
+                        step = 2 * p.kvs[half][2];
+                    }
+#pragma unroll
+                    for (int x = 0; x < C::kBlock * kChunks / 32; ++x) {
+                        const int idx = x * 32 + lane, token = idx / kChunks, chunk = idx % kChunks, key = key0 + token;
+                        const bool live = key < high.hi && (key >= low.lo || key < c.sinks);
+                        const int to = Q4 ? chunk : chunk ^ (token & 7);
+                        copy_async<16>(dst + half * C::kHalf + token * C::kRow + to * 16, src + (live ? key * step : 0) + chunk * 16, live);
+                    }
+                    if constexpr (Q4) {
+                        const CacheView& v = c.half[half];
+                        const int key = key0 + lane;
+                        const bool live = key < high.hi && (key >= low.lo || key < c.sinks);
+                        copy_async<C::kParam>(dst + half * C::kHalf + C::kBlock * C::kRow + lane * C::kParam,
+                                              v.params + b * v.ps[0] + kvh * v.ps[1] + (live ? key * v.ps[2] : 0), live);
+                    }
+                }
+            }
+            copy_commit();
+        };
+#pragma unroll
+        for (int n = 0; n < C::kStages - 1; ++n) request(n);
+
+        // the query rows as operand B, and their sums over the groups
+        uint32_t qf[NT][D / 16][2];
+        float qsum[NT][2][D / 64];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int r = row0 + n * 8 + g;
+            const bool live = r < p.rows;
+            const int head = kvh * c.group + r / c.Sq, sq = r % c.Sq;
+            const T* qrow = static_cast<const T*>(c.q) + (live ? b * c.qs[0] + head * c.qs[1] + sq * c.qs[2] : 0);
+            const uint32_t flip = c.scale < 0.f ? 0x80008000u : 0u;
+            if constexpr (Q4) {
+#pragma unroll
+                for (int grp = 0; grp < C::kGroups; ++grp) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        uint4 raw = live ? *reinterpret_cast<const uint4*>(qrow + grp * 64 + i * 16 + x * 8) : make_uint4(0, 0, 0, 0);
+                        raw.x ^= flip, raw.y ^= flip, raw.z ^= flip, raw.w ^= flip;
+                        // channels 0..7 in raw.x .. raw.w; a pair is (channel j, channel j + 4)
+                        qf[n][grp * 4 + x * 2][0] = __byte_perm(raw.x, raw.z, 0x5410);
+                        qf[n][grp * 4 + x * 2][1] = __byte_perm(raw.x, raw.z, 0x7632);
+                        qf[n][grp * 4 + x * 2 + 1][0] = __byte_perm(raw.y, raw.w, 0x5410);
+                        qf[n][grp * 4 + x * 2 + 1][1] = __byte_perm(raw.y, raw.w, 0x7632);
+                        const float2 e0 = unpack2<BF16>(raw.x), e1 = unpack2<BF16>(raw.y), e2 = unpack2<BF16>(raw.z),
+                                     e3 = unpack2<BF16>(raw.w);
+                        sum += ((e0.x + e0.y) + (e1.x + e1.y)) + ((e2.x + e2.y) + (e3.x + e3.y));
+                    }
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);  // row g
+                    qsum[n][0][grp] = __shfl_sync(0xffffffffu, sum, 8 * i);
+                    qsum[n][1][grp] = __shfl_sync(0xffffffffu, sum, 8 * i + 4);
+                }
+            } else {
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+                        qf[n][ks][x] = live ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + x * 8 + 2 * i) ^ flip : 0u;
+            }
+        }
+
+        st.clear();
+        for (int n = 0; n < mine; ++n) {
+            copy_wait<C::kStages - 2>();
+            __syncwarp();
+            request(n + C::kStages - 1);  // into the stage that the previous block has left
+            const int key0 = blocks.block(from + warp + n * kWarps) * C::kBlock;
+            const uint8_t* stage = my_ring + (n % C::kStages) * C::kStage;
+            const bool clean = key0 + C::kBlock <= low.hi && (key0 >= high.lo || key0 + C::kBlock <= c.sinks);
+            if (clean) block_step<T, D, Q4, NT, true>(st, stage, qf, qsum, c, start, key0, row0, c2, lane);
+            else block_step<T, D, Q4, NT, false>(st, stage, qf, qsum, c, start, key0, row0, c2, lane);
+            __syncwarp();
+        }
+        copy_wait<0>();
+
+        // the warps of the CTA, merged in a fixed order through the (now idle) ring
+        __syncthreads();
+        float* sm_o = reinterpret_cast<float*>(ring);  // [warp][R][D]
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float l = st.l[n][e];
+                l += __shfl_xor_sync(0xffffffffu, l, 4);
+                l += __shfl_xor_sync(0xffffffffu, l, 8);
+                l += __shfl_xor_sync(0xffffffffu, l, 16);
+                const int r = n * 8 + 2 * i + e;
+                if (g == 0) {
+                    sm_m[warp][r] = st.m[n][e];
+                    sm_l[warp][r] = l;
+                }
+                float z[Q4 ? D / 64 : 1] = {};
+                if (Q4) {
+#pragma unroll
+                    for (int grp = 0; grp < D / 64; ++grp) {
+                        float x = st.z[n][e][Q4 ? grp : 0];
+                        x += __shfl_xor_sync(0xffffffffu, x, 4);
+                        x += __shfl_xor_sync(0xffffffffu, x, 8);
+                        x += __shfl_xor_sync(0xffffffffu, x, 16);
+                        z[Q4 ? grp : 0] = x;
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        sm_o[(warp * R + r) * D + channel_of<Q4>(t, g, u)] = st.o[t][n][2 * u + e] + z[Q4 ? t >> 2 : 0];
+            }
+        __syncthreads();
+        const bool whole = count == blocks.count;
+        const int slot = at == begin ? 0 : 1;
+        for (int idx = threadIdx.x; idx < R * (D / 4); idx += kWarps * 32) {
+            const int r = idx / (D / 4), d = idx % (D / 4) * 4;
+            float mx = sm_m[0][r];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, sm_m[w][r]);
+            float sum = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float weight = sm_m[w][r] == -INFINITY ? 0.f : ex2((sm_m[w][r] - mx) * c2);
+                const float4 x = *reinterpret_cast<const float4*>(sm_o + (w * R + r) * D + d);
+                sum += sm_l[w][r] * weight;
+                acc.x = fmaf(x.x, weight, acc.x), acc.y = fmaf(x.y, weight, acc.y);
+                acc.z = fmaf(x.z, weight, acc.z), acc.w = fmaf(x.w, weight, acc.w);
+            }
+            if (whole) {
+                const int row = row0 + r;
+                if (row < p.rows) {
+                    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+                    T* out = static_cast<T*>(c.out) + b * c.os[0] + (kvh * c.group + row / c.Sq) * c.os[1] + row % c.Sq * c.os[2] + d;
+                    *reinterpret_cast<uint2*>(out) =
+                        make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
+                }
+            } else {
+                const int64_t piece = ((int64_t)blockIdx.x * 2 + slot) * R + r;
+                *reinterpret_cast<float4*>(p.part_o + piece * D + d) = acc;
+                if (d == 0) *reinterpret_cast<float2*>(p.part_ml + piece * 2) = make_float2(mx, sum);
+            }
+        }
+        __syncthreads();
+        at += count;
+    }
+}
+
+// One CTA per unit: units that one CTA served whole are done; the others' pieces are merged in order; a sequence
+// without a visible key gets its zeros here.
+template <typename T, int D, bool Q4, int NT>
+__global__ void __launch_bounds__(256) merge_rows(const RowsCall p) {
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    using C = Cfg<D, Q4>;
+    constexpr int R = 8 * NT;
+    const CacheAttentionCall& c = p.c;
+    const int64_t units = (int64_t)c.Hkv * p.chunks;
+    const int b = (int)(blockIdx.x / units), unit = (int)(blockIdx.x % units);
+    const int kvh = unit / p.chunks, row0 = unit % p.chunks * R;
+    const int64_t total = total_blocks(c, units, C::kBlock);
+    const int count = blocks_of(c, start_of(c, b), C::kBlock).count;
+    const int ctas = used_ctas(total, p.ctas);
+    int first = 0, last = -1;
+    int64_t u0 = 0;
+    if (count > 0) {
+        int64_t base = 0;  // blocks of the sequences before b
+        for (int x = threadIdx.x & 31; x < b; x += 32) base += blocks_of(c, start_of(c, x), C::kBlock).count;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) base += __shfl_xor_sync(0xffffffffu, base, o);
+        u0 = base * units + (int64_t)unit * count;
+        first = cta_of(total, ctas, u0);
+        last = cta_of(total, ctas, u0 + count - 1);
+    }
+    // (also where there is nothing to merge: this grid's end has to mean the end of the other one)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (count > 0 && first == last) return;
+    const float c2 = fabsf(c.scale) * kLog2e;
+    const int slot0 = count > 0 && u0 == cta_begin(total, ctas, first) ? 0 : 1;
+    for (int idx = threadIdx.x; idx < R * (D / 4); idx += 256) {
+        const int r = idx / (D / 4), d = idx % (D / 4) * 4, row = row0 + r;
+        if (row >= p.rows) continue;
+        float mx = -INFINITY, sum = 0.f;
+        for (int i = first; i <= last; ++i)
+            mx = fmaxf(mx, p.part_ml[(((int64_t)i * 2 + (i == first ? slot0 : 0)) * R + r) * 2]);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int i = first; i <= last; ++i) {
+            const int64_t piece = ((int64_t)i * 2 + (i == first ? slot0 : 0)) * R + r;
+            const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + piece * 2);
+            const float4 x = *reinterpret_cast<const float4*>(p.part_o + piece * D + d);
+            const float weight = ml.x == -INFINITY ? 0.f : ex2((ml.x - mx) * c2);
+            sum += ml.y * weight;
+            acc.x = fmaf(x.x, weight, acc.x), acc.y = fmaf(x.y, weight, acc.y);
+            acc.z = fmaf(x.z, weight, acc.z), acc.w = fmaf(x.w, weight, acc.w);
+        }
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        T* out = static_cast<T*>(c.out) + b * c.os[0] + (kvh * c.group + row / c.Sq) * c.os[1] + row % c.Sq * c.os[2] + d;
+        *reinterpret_cast<uint2*>(out) =
+            make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
+    }
+}
+
+// ------------------------------------------------------------------ host
+template <int D, bool Q4>
+int64_t most_blocks(const CacheAttentionCall& c) {  // of one unit
+    constexpr int size = Cfg<D, Q4>::kBlock;
+    const int64_t keys = c.window < c.Sk ? c.window + c.Sq - 1 : c.Sk;
+    const int64_t all = (c.Sk + size - 1) / size, some = (keys + size - 1) / size + 1 + (c.sinks + size - 1) / size;
+    return some < all ? some : all;
+}
+
+inline int row_tiles(const CacheAttentionCall& c) { return (int64_t)c.group * c.Sq <= 8 ? 1 : 2; }
+
+template <int D, bool Q4, int NT>
+int plan_ctas(const CacheAttentionCall& c, int chunks) {
+    // As many CTAs as are resident at once, but no fewer blocks for a CTA than it has warps.
+    const int64_t line = (int64_t)c.B * c.Hkv * chunks * most_blocks<D, Q4>(c);
+    const int64_t most = 148 * resident<D, Q4, NT>();
+    const int64_t want = (line + kWarps - 1) / kWarps;
+    return (int)(want < 1 ? 1 : (want > most ? most : want));
+}
+
+template <int D, bool Q4>
+size_t workspace_bytes(const CacheAttentionCall& c) {
+    const int NT = row_tiles(c), R = 8 * NT, chunks = (c.group * c.Sq + R - 1) / R;
+    const int ctas = NT == 1 ? plan_ctas<D, Q4, 1>(c, chunks) : plan_ctas<D, Q4, 2>(c, chunks);
+    return (size_t)ctas * 2 * R * (D + 2) * sizeof(float);
+}
+
+template <typename T, int D, bool Q4, int NT>
+cudaError_t launch(RowsCall& p, void* workspace, cudaStream_t st) {
+    using C = Cfg<D, Q4>;
+    constexpr int R = 8 * NT;
+    constexpr int kMerge = kWarps * R * D * 4;
+    constexpr int kSmem = C::kRing > kMerge ? C::kRing : kMerge;
+    p.rows = p.c.group * p.c.Sq;
+    p.chunks = (p.rows + R - 1) / R;
+    p.ctas = plan_ctas<D, Q4, NT>(p.c, p.chunks);
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = p.part_o + (size_t)p.ctas * 2 * R * D;
+    cudaError_t e = cudaFuncSetAttribute(decode_rows<T, D, Q4, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return e;
+    decode_rows<T, D, Q4, NT><<<p.ctas, kWarps * 32, kSmem, st>>>(p);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)((int64_t)p.c.B * p.c.Hkv * p.chunks));
+    config.blockDim = dim3(256);
+    config.stream = st;
+    cudaLaunchAttribute dependent[1];
+    dependent[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    dependent[0].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = dependent;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, merge_rows<T, D, Q4, NT>, (const RowsCall)p);
+}
+
+template <typename T, bool Q4>
+cudaError_t dispatch(RowsCall& p, void* workspace, cudaStream_t st) {
+    const bool one = row_tiles(p.c) == 1;
+    if (p.c.D == 128)
+        return one ? launch<T, 128, Q4, 1>(p, workspace, st) : launch<T, 128, Q4, 2>(p, workspace, st);
+    return one ? launch<T, 64, Q4, 1>(p, workspace, st) : launch<T, 64, Q4, 2>(p, workspace, st);
+}
+
+}  // namespace rows
+}  // namespace kfa
