@@ -235,15 +235,20 @@ KFA_API int kfa_merge_splits(kfa_tensor* out, kfa_tensor* maximum, kfa_tensor* l
  * `start` for every batch when `starts` is NULL, else starts[b] (int32 [B] in device memory, read by the kernels: the
  * call can be captured in a graph and replayed with new positions).  Any position is allowed: a row that sees no key
  * yields out = 0, maximum = -inf, logsum = 0.  window >= 1, sinks >= 0, any other operand as for kfa_forward; the
- * statistics may both be NULL.
+ * statistics may both be NULL.  `workspace` holds kfa_window_forward_workspace_bytes() bytes, 16-byte aligned (0: may be
+ * NULL): without statistics, calls of at most 16 query rows per K/V head (positions x grouped heads, 64 or 128
+ * channels) run on the decoding kernels, which need it.
  *
  * kfa_window_backward takes the forward's out/maximum/logsum and one `start` >= 0 for all batches; `workspace` holds
  * kfa_window_backward_workspace_bytes() bytes, 256-byte aligned.  Every gradient has one owner and a fixed order of
  * additions.
  */
+KFA_API size_t kfa_window_forward_workspace_bytes(const kfa_tensor* q, const kfa_tensor* k, int64_t window,
+                       int64_t sinks, int statistics);
 KFA_API int kfa_window_forward(const kfa_tensor* q, const kfa_tensor* k, const kfa_tensor* v, const kfa_tensor* starts,
-                       kfa_tensor* out, kfa_tensor* maximum, kfa_tensor* logsum, int64_t start, int64_t window,
-                       int64_t sinks, float scale, void* stream);
+                       kfa_tensor* out, kfa_tensor* maximum, kfa_tensor* logsum, void* workspace,
+                       size_t workspace_bytes, int64_t start, int64_t window, int64_t sinks, float scale,
+                       void* stream);
 KFA_API size_t kfa_window_backward_workspace_bytes(const kfa_tensor* q, const kfa_tensor* k, int64_t start,
                        int64_t window, int64_t sinks);
 KFA_API int kfa_window_backward(const kfa_tensor* q, const kfa_tensor* k, const kfa_tensor* v, const kfa_tensor* out,

@@ -1115,9 +1115,30 @@ SinkPlan sink_plan(const kfa_tensor* q, const kfa_tensor* k, int64_t window, int
 
 extern "C" {
 
+size_t kfa_window_forward_workspace_bytes(const kfa_tensor* q, const kfa_tensor* k, int64_t window, int64_t sinks,
+                                          int statistics) {
+    if (!q || !k || statistics || q->ndim != 4 || k->ndim != 4 || window < 1 || sinks < 0) return 0;
+    for (int i = 0; i < 4; ++i)
+        if (q->sizes[i] <= 0 || k->sizes[i] <= 0 || q->sizes[i] > INT32_MAX || k->sizes[i] > INT32_MAX) return 0;
+    if (q->sizes[1] % k->sizes[1] != 0) return 0;
+    kfa::AttnParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.B = (int)q->sizes[0];
+    p.Hq = (int)q->sizes[1];
+    p.Hkv = (int)k->sizes[1];
+    p.Sq = (int)q->sizes[2];
+    p.Sk = (int)k->sizes[2];
+    p.D = (int)q->sizes[3];
+    p.group = p.Hq / p.Hkv;
+    p.window = std::min<int64_t>(window, int64_t(1) << 40);
+    p.sinks = (int)std::min<int64_t>(sinks, p.Sk);
+    return kfa::window_decode_shape(p) ? kfa::window_decode_workspace_bytes(p) : 0;
+}
+
 int kfa_window_forward(const kfa_tensor* q, const kfa_tensor* k, const kfa_tensor* v, const kfa_tensor* starts,
-                       kfa_tensor* out, kfa_tensor* maximum, kfa_tensor* logsum, int64_t start, int64_t window,
-                       int64_t sinks, float scale, void* stream) {
+                       kfa_tensor* out, kfa_tensor* maximum, kfa_tensor* logsum, void* workspace,
+                       size_t workspace_bytes, int64_t start, int64_t window, int64_t sinks, float scale,
+                       void* stream) {
     if (int e = check_device_ok()) return e;
     if (int e = check_qkv(q, k, v)) return e;
     kfa::AttnParams p;
@@ -1133,6 +1154,23 @@ int kfa_window_forward(const kfa_tensor* q, const kfa_tensor* k, const kfa_tenso
     p.logsum = keep_statistics ? static_cast<float*>(logsum->data) : nullptr;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool bf16 = q->dtype == KFA_BF16;
+    const size_t need = kfa_window_forward_workspace_bytes(q, k, window, sinks, keep_statistics);
+    if (need > 0) {
+        auto rows_ok = [](const void* ptr, const int64_t* st, const int64_t* sizes) {
+            bool ok = st[3] == 1 && reinterpret_cast<uintptr_t>(ptr) % 16 == 0;
+            for (int i = 0; i < 3; ++i) ok = ok && (sizes[i] == 1 || st[i] % 8 == 0);
+            return ok;
+        };
+        if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+            return fail(KFA_INVALID_ARGUMENT, "window forward workspace too small or not 16-byte aligned");
+        if (rows_ok(p.q, p.qs, q->sizes) && rows_ok(p.k, p.ks, k->sizes) && rows_ok(p.v, p.vs, v->sizes) &&
+            rows_ok(p.out, p.os, out->sizes)) {
+            cudaError_t ce = timed("window_decode", st, [&] { return kfa::launch_window_decode(p, bf16, workspace, st); });
+            if (ce != cudaSuccess) return cuda_fail(ce, "window decode launch");
+            count_kernel("window_decode", 1);  // two launches
+            return 0;
+        }
+    }
     cudaError_t ce = window_on_pipeline(p) && kfa::pipeline_forward_supported(p, bf16)
                          ? timed("pipeline_forward_window", st, [&] { return kfa::launch_pipeline_forward(p, bf16, st); })
                          : timed("general_forward", st, [&] { return kfa::launch_general_forward(p, bf16, st); });
@@ -1387,6 +1425,7 @@ int kfa_cache_attention(const kfa_tensor* q, const kfa_tensor* k_codes, const kf
     cudaError_t ce = timed("cache_attention", st,
                            [&] { return kfa::launch_cache_attention(p, q->dtype == KFA_BF16, workspace, st); });
     if (ce != cudaSuccess) return cuda_fail(ce, "cache attention launch");
+    count_kernel("cache_attention", 1);  // two launches
     return 0;
 }
 

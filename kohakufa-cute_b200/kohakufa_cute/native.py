@@ -70,7 +70,9 @@ SIGNATURES = {
                                                               _I64P, ctypes.c_float, ctypes.c_void_p]),
     "kfa_merge_partial": (ctypes.c_int, [_TP] * 6 + [ctypes.c_float, ctypes.c_void_p]),
     "kfa_merge_splits": (ctypes.c_int, [_TP] * 6 + [ctypes.c_float, ctypes.c_void_p]),
-    "kfa_window_forward": (ctypes.c_int, [_TP] * 7 + [ctypes.c_int64] * 3 + [ctypes.c_float, ctypes.c_void_p]),
+    "kfa_window_forward_workspace_bytes": (ctypes.c_size_t, [_TP, _TP, ctypes.c_int64, ctypes.c_int64, ctypes.c_int]),
+    "kfa_window_forward": (ctypes.c_int, [_TP] * 7 + [ctypes.c_void_p, ctypes.c_size_t] + [ctypes.c_int64] * 3 +
+                           [ctypes.c_float, ctypes.c_void_p]),
     "kfa_window_backward_workspace_bytes": (ctypes.c_size_t, [_TP, _TP] + [ctypes.c_int64] * 3),
     "kfa_window_backward": (ctypes.c_int, [_TP] * 10 + [ctypes.c_void_p, ctypes.c_size_t] + [ctypes.c_int64] * 3 +
                             [ctypes.c_float, ctypes.c_void_p]),
@@ -452,8 +454,11 @@ def window_forward(q, k, v, starts, start, window, sinks, scale, statistics=True
         maximum = torch.empty(q.shape[:-1], device=q.device, dtype=torch.float32) if statistics else None
         logsum = torch.empty_like(maximum) if statistics else None
         records = [describe(t) for t in (q, k, v, starts, out, maximum, logsum)]
-        _check(lib.kfa_window_forward(*[_ref(r) for r in records], start, window, sinks, float(scale),
-                                      _stream(q.device)))
+        need = lib.kfa_window_forward_workspace_bytes(_ref(records[0]), _ref(records[1]), window, sinks, statistics)
+        workspace = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
+        _check(lib.kfa_window_forward(*[_ref(r) for r in records],
+                                      ctypes.c_void_p(workspace.data_ptr() if need else None), need, start, window,
+                                      sinks, float(scale), _stream(q.device)))
     return out, maximum, logsum
 
 
