@@ -27,6 +27,7 @@
 #include "sm100_ptx.cuh"
 #include "window.cuh"
 
+#include <atomic>
 #include <type_traits>
 
 namespace kfa {
@@ -709,8 +710,17 @@ cudaError_t launch(RowsCall& p, void* workspace, cudaStream_t st) {
     p.ctas = plan_ctas<D, Q4, NT>(p.c, p.chunks);
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = p.part_o + (size_t)p.ctas * 2 * R * D;
-    cudaError_t e = cudaFuncSetAttribute(decode_rows<T, D, Q4, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    // the shared-memory opt-in holds per device; a decoding step is short enough for the call to show, so it is made once
+    static std::atomic<uint64_t> opted{0};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return e;
+    const uint64_t bit = uint64_t(1) << (device & 63);
+    if (!(opted.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(decode_rows<T, D, Q4, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        if (e != cudaSuccess) return e;
+        opted.fetch_or(bit, std::memory_order_relaxed);
+    }
     decode_rows<T, D, Q4, NT><<<p.ctas, kWarps * 32, kSmem, st>>>(p);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;

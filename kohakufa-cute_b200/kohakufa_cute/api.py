@@ -16,6 +16,7 @@ Signatures, argument meaning and error behaviour follow the reference package
 Validation errors are ``ValueError``; kernel or library errors propagate unchanged.
 """
 
+from functools import lru_cache
 from math import isfinite, prod
 
 import torch
@@ -25,6 +26,7 @@ _HALF_TYPES = (torch.float16, torch.bfloat16)
 _SUPPORTED_CAPABILITY = (10, 0)
 
 
+@lru_cache(maxsize=None)
 def _device_supported(device):
     return torch.cuda.get_device_capability(device) == _SUPPORTED_CAPABILITY
 

@@ -9,8 +9,10 @@ stream.  There is no fallback: when the library is missing, loading raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -40,6 +42,7 @@ class KfaTensor(ctypes.Structure):
 
 
 _TP = ctypes.POINTER(KfaTensor)
+_VP = ctypes.c_void_p  # a record by its address (see ``_records``)
 _I64P = ctypes.POINTER(ctypes.c_int64)
 
 # name -> (restype, argtypes); must list every symbol declared in include/kfa.h
@@ -70,17 +73,17 @@ SIGNATURES = {
                                                               _I64P, ctypes.c_float, ctypes.c_void_p]),
     "kfa_merge_partial": (ctypes.c_int, [_TP] * 6 + [ctypes.c_float, ctypes.c_void_p]),
     "kfa_merge_splits": (ctypes.c_int, [_TP] * 6 + [ctypes.c_float, ctypes.c_void_p]),
-    "kfa_window_forward_workspace_bytes": (ctypes.c_size_t, [_TP, _TP, ctypes.c_int64, ctypes.c_int64, ctypes.c_int]),
-    "kfa_window_forward": (ctypes.c_int, [_TP] * 7 + [ctypes.c_void_p, ctypes.c_size_t] + [ctypes.c_int64] * 3 +
-                           [ctypes.c_float, ctypes.c_void_p]),
-    "kfa_window_backward_workspace_bytes": (ctypes.c_size_t, [_TP, _TP] + [ctypes.c_int64] * 3),
-    "kfa_window_backward": (ctypes.c_int, [_TP] * 10 + [ctypes.c_void_p, ctypes.c_size_t] + [ctypes.c_int64] * 3 +
-                            [ctypes.c_float, ctypes.c_void_p]),
-    "kfa_cache_write": (ctypes.c_int, [_TP] * 8 + [ctypes.c_int64, ctypes.c_void_p]),
-    "kfa_cache_read": (ctypes.c_int, [_TP] * 7 + [ctypes.c_int64, ctypes.c_void_p]),
-    "kfa_cache_attention_workspace_bytes": (ctypes.c_size_t, [_TP, _TP, ctypes.c_int64, ctypes.c_int64]),
-    "kfa_cache_attention": (ctypes.c_int, [_TP] * 7 + [ctypes.c_void_p, ctypes.c_size_t] + [ctypes.c_int64] * 3 +
-                            [ctypes.c_float, ctypes.c_void_p]),
+    "kfa_window_forward_workspace_bytes": (ctypes.c_size_t, [_VP, _VP, ctypes.c_int64, ctypes.c_int64, ctypes.c_int]),
+    "kfa_window_forward": (ctypes.c_int, [_VP] * 7 + [_VP, ctypes.c_size_t] + [ctypes.c_int64] * 3 +
+                           [ctypes.c_float, _VP]),
+    "kfa_window_backward_workspace_bytes": (ctypes.c_size_t, [_VP, _VP] + [ctypes.c_int64] * 3),
+    "kfa_window_backward": (ctypes.c_int, [_VP] * 10 + [_VP, ctypes.c_size_t] + [ctypes.c_int64] * 3 +
+                            [ctypes.c_float, _VP]),
+    "kfa_cache_write": (ctypes.c_int, [_VP] * 8 + [ctypes.c_int64, _VP]),
+    "kfa_cache_read": (ctypes.c_int, [_VP] * 7 + [ctypes.c_int64, _VP]),
+    "kfa_cache_attention_workspace_bytes": (ctypes.c_size_t, [_VP, _VP, ctypes.c_int64, ctypes.c_int64]),
+    "kfa_cache_attention": (ctypes.c_int, [_VP] * 7 + [_VP, ctypes.c_size_t] + [ctypes.c_int64] * 3 +
+                            [ctypes.c_float, _VP]),
     "kfa_cache_size": (ctypes.c_int, []),
     "kfa_clear_cache": (None, []),
     "kfa_launch_count": (ctypes.c_uint64, []),
@@ -139,6 +142,40 @@ def describe(tensor):
     return record
 
 
+# The fields of a record with n axes (the rest of the six stays zero).
+_RECORDS = [struct.Struct(f"<Qii{n}q{8 * (6 - n)}x{n}q{8 * (6 - n)}x") for n in range(7)]
+_RECORD_BYTES = ctypes.sizeof(KfaTensor)
+
+
+def _records(*tensors):
+    """``(buffer, addresses)``: the records of ``describe`` side by side in one buffer, for the entry points whose host
+    time matters (a decoding step launches for a few microseconds); the buffer has to outlive the call."""
+    buffer = bytearray(_RECORD_BYTES * len(tensors))
+    base = ctypes.addressof(ctypes.c_char.from_buffer(buffer))
+    addresses, offset = [], 0
+    for t in tensors:
+        if t is None:
+            addresses.append(None)
+        else:
+            n = t.dim()
+            _RECORDS[n].pack_into(buffer, offset, t.data_ptr(), _DTYPES[t.dtype], n, *t.shape, *t.stride())
+            addresses.append(base + offset)
+        offset += _RECORD_BYTES
+    return buffer, addresses
+
+
+_NO_CONTEXT = contextlib.nullcontext()
+
+
+def _on(device):
+    """``torch.cuda.device(device)``, or nothing where that device is current already."""
+    return _NO_CONTEXT if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _raw_stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def _ref(record):
     return None if record is None else ctypes.byref(record)
 
@@ -164,13 +201,17 @@ def _stream(device):
 
 def _plain(tensor):
     """Physical storage must equal logical values: resolve lazy conj/neg view flags."""
-    return tensor.resolve_conj().resolve_neg()
+    return tensor.resolve_conj().resolve_neg() if tensor.is_conj() or tensor.is_neg() else tensor
 
 
 def _rows_16_byte_addressable(t):
-    if t.stride(-1) != 1 or t.data_ptr() % 16:
+    *strides, channel = t.stride()
+    if channel != 1 or t.data_ptr() % 16:
         return False
-    return all(size == 1 or (stride > 0 and stride % 8 == 0) for size, stride in zip(t.shape[:-1], t.stride()[:-1]))
+    for size, stride in zip(t.shape, strides):
+        if size != 1 and (stride <= 0 or stride % 8):
+            return False
+    return True
 
 
 def _blocks_shape(q, k, mask):
@@ -449,16 +490,17 @@ def window_forward(q, k, v, starts, start, window, sinks, scale, statistics=True
     if any(a is not b for a, b in zip((q, k, v), originals)):
         out, maximum, logsum = window_forward(q, k, v, starts, start, window, sinks, scale, statistics)
         return _like(originals[0], out), maximum, logsum
-    with torch.cuda.device(q.device):
+    device = q.device
+    with _on(device):
         out = torch.empty_like(q)
-        maximum = torch.empty(q.shape[:-1], device=q.device, dtype=torch.float32) if statistics else None
-        logsum = torch.empty_like(maximum) if statistics else None
-        records = [describe(t) for t in (q, k, v, starts, out, maximum, logsum)]
-        need = lib.kfa_window_forward_workspace_bytes(_ref(records[0]), _ref(records[1]), window, sinks, statistics)
-        workspace = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
-        _check(lib.kfa_window_forward(*[_ref(r) for r in records],
-                                      ctypes.c_void_p(workspace.data_ptr() if need else None), need, start, window,
-                                      sinks, float(scale), _stream(q.device)))
+        maximum = logsum = None
+        if statistics:
+            maximum, logsum = torch.empty((2, *q.shape[:-1]), device=device, dtype=torch.float32).unbind(0)
+        keep, records = _records(q, k, v, starts, out, maximum, logsum)
+        need = lib.kfa_window_forward_workspace_bytes(records[0], records[1], window, sinks, statistics)
+        workspace = torch.empty(need, device=device, dtype=torch.uint8) if need else None
+        _check(lib.kfa_window_forward(*records, workspace.data_ptr() if need else None, need, start, window, sinks,
+                                      scale, _raw_stream(device)))
     return out, maximum, logsum
 
 
@@ -471,14 +513,14 @@ def window_backward(q, k, v, out, maximum, logsum, dout, start, window, sinks, s
     if any(a is not b for a, b in zip((q, k, v), originals)):
         grads = window_backward(q, k, v, out, maximum, logsum, dout, start, window, sinks, scale)
         return tuple(_like(o, g) for o, g in zip(originals, grads))
-    with torch.cuda.device(q.device):
+    device = q.device
+    with _on(device):
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-        rq, rk = describe(q), describe(k)
-        need = lib.kfa_window_backward_workspace_bytes(_ref(rq), _ref(rk), start, window, sinks)
-        workspace = torch.empty(need, device=q.device, dtype=torch.uint8)
-        records = [rq, rk] + [describe(t) for t in (v, out, maximum, logsum, dout, dq, dk, dv)]
-        _check(lib.kfa_window_backward(*[_ref(r) for r in records], ctypes.c_void_p(workspace.data_ptr()), need, start,
-                                       window, sinks, float(scale), _stream(q.device)))
+        keep, records = _records(q, k, v, out, maximum, logsum, dout, dq, dk, dv)
+        need = lib.kfa_window_backward_workspace_bytes(records[0], records[1], start, window, sinks)
+        workspace = torch.empty(need, device=device, dtype=torch.uint8)
+        _check(lib.kfa_window_backward(*records, workspace.data_ptr(), need, start, window, sinks, scale,
+                                       _raw_stream(device)))
     return dq, dk, dv
 
 
@@ -486,20 +528,22 @@ def cache_write(k, v, k_codes, k_params, v_codes, v_params, starts, lengths, sta
     """Quantises the rows of ``k`` and ``v`` into a 4-bit cache in place (``kfa_cache_write``)."""
     lib = library()
     k, v = (t if _rows_16_byte_addressable(t) else t.contiguous() for t in (_plain(k), _plain(v)))
-    with torch.cuda.device(k.device):
-        records = [describe(t) for t in (k, v, k_codes, k_params, v_codes, v_params, starts, lengths)]
-        _check(lib.kfa_cache_write(*[_ref(r) for r in records], start, _stream(k.device)))
+    device = k.device
+    with _on(device):
+        keep, records = _records(k, v, k_codes, k_params, v_codes, v_params, starts, lengths)
+        _check(lib.kfa_cache_write(*records, start, _raw_stream(device)))
 
 
 def cache_read(k_codes, k_params, v_codes, v_params, starts, start, length):
     """(k, v) ``[B, H, length, D]``: the values of a 4-bit cache's rows (``kfa_cache_read``)."""
     lib = library()
-    shape = (k_codes.shape[0], k_codes.shape[1], length, 2 * k_codes.shape[3])
-    with torch.cuda.device(k_codes.device):
-        k = torch.empty(shape, device=k_codes.device, dtype=k_params.dtype)
+    batch, heads, _, half = k_codes.shape
+    device = k_codes.device
+    with _on(device):
+        k = torch.empty((batch, heads, length, 2 * half), device=device, dtype=k_params.dtype)
         v = torch.empty_like(k)
-        records = [describe(t) for t in (k_codes, k_params, v_codes, v_params, starts, k, v)]
-        _check(lib.kfa_cache_read(*[_ref(r) for r in records], start, _stream(k.device)))
+        keep, records = _records(k_codes, k_params, v_codes, v_params, starts, k, v)
+        _check(lib.kfa_cache_read(*records, start, _raw_stream(device)))
     return k, v
 
 
@@ -509,15 +553,14 @@ def cache_attention(q, k_codes, k_params, v_codes, v_params, starts, start, wind
     q = _plain(q)
     if not _rows_16_byte_addressable(q):
         q = q.contiguous()
-    with torch.cuda.device(q.device):
+    device = q.device
+    with _on(device):
         out = torch.empty_like(q)
-        rq, rc = describe(q), describe(k_codes)
-        need = lib.kfa_cache_attention_workspace_bytes(_ref(rq), _ref(rc), window, sinks)
-        workspace = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
-        records = [rq, rc] + [describe(t) for t in (k_params, v_codes, v_params, starts, out)]
-        _check(lib.kfa_cache_attention(*[_ref(r) for r in records],
-                                       ctypes.c_void_p(workspace.data_ptr() if need else None), need, start, window,
-                                       sinks, float(scale), _stream(q.device)))
+        keep, records = _records(q, k_codes, k_params, v_codes, v_params, starts, out)
+        need = lib.kfa_cache_attention_workspace_bytes(records[0], records[1], window, sinks)
+        workspace = torch.empty(need, device=device, dtype=torch.uint8)
+        _check(lib.kfa_cache_attention(*records, workspace.data_ptr(), need, start, window, sinks, scale,
+                                       _raw_stream(device)))
     return out
 
 
