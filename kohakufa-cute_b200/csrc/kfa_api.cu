@@ -1312,7 +1312,7 @@ int fill_cache_call(kfa::CacheCall& p, const kfa_tensor* k, const kfa_tensor* v,
     p.D = (int)k->sizes[3];
     p.capacity = (int)k_codes->sizes[2];
     if (int e = check_positions(starts, p.B, "starts")) return e;
-    if (2 * k->sizes[0] * k->sizes[1] * k->sizes[2] * (p.D / 8) / 256 > INT32_MAX - 1 || k->sizes[0] * k->sizes[1] > INT32_MAX)
+    if (k->sizes[0] * k->sizes[1] > INT32_MAX / 2 || 2 * k->sizes[0] * k->sizes[1] * (k->sizes[2] / 16 + 1) > INT32_MAX)
         return fail(KFA_TOO_LARGE, "quantized cache: too many rows in one call");
     p.starts = starts ? static_cast<const int32_t*>(starts->data) : nullptr;
     p.start = start;

@@ -26,8 +26,14 @@ _HALF_TYPES = (torch.float16, torch.bfloat16)
 _SUPPORTED_CAPABILITY = (10, 0)
 
 
-@lru_cache(maxsize=None)
 def _device_supported(device):
+    if torch.compiler.is_compiling():
+        return torch.cuda.get_device_capability(device) == _SUPPORTED_CAPABILITY
+    return _device_supported_once(device)
+
+
+@lru_cache(maxsize=None)
+def _device_supported_once(device):
     return torch.cuda.get_device_capability(device) == _SUPPORTED_CAPABILITY
 
 
