@@ -10,9 +10,9 @@
 // bytes, and its rows are tokens only in one of the two products.)
 //
 // 4-bit caches are never widened to values.  Codes become 16-bit floats in two instructions per pair (shift, and one
-// logic operation that masks the code into the mantissa of 16.0: 16 + code), and scale and zero of a token's group of
+// logic operation that masks the code into the mantissa of a base, 16 or 128), and scale and zero of a token's group of
 // 64 channels are applied to sums, in FP32:
-//   s    = sum_g  scale_g * (sum_d q_d (16 + code_d))  +  (zero_g - 16 scale_g) * (sum_d q_d)
+//   s    = sum_g  scale_g * (sum_d q_d (base_d + code_d) - sum_d q_d base_d)  +  zero_g * (sum_d q_d)
 //   o_d  = sum_t  round16(p_t scale_g) * (code_d - 8)  +  sum_t p_t (zero_g + 8 scale_g)
 // The codes less 8 are centred, so the one rounding, of p * scale, weighs like the rounding of p against 16-bit values.
 //
@@ -122,6 +122,19 @@ __device__ __forceinline__ int64_t cta_begin(int64_t total, int ctas, int i) { r
 __device__ __forceinline__ int cta_of(int64_t total, int ctas, int64_t at) { return (int)(((at + 1) * ctas - 1) / total); }
 
 // ------------------------------------------------------------------ instructions
+// d = A B + (c0, c1, c0, c1)
+template <bool BF16>
+__device__ __forceinline__ void mma_from(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1, float c0, float c1) {
+    if constexpr (BF16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
 template <bool BF16>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
@@ -157,24 +170,35 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool l
     else
         asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(bytes) : "memory");
 }
+// One contiguous copy, counted in bytes on `bar`.
+__device__ __forceinline__ void copy_bulk(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// Code t (0..3) of both halves of a word as a pair of 16-bit floats 16 + code.
+// Code t (0..3) of both halves of a word as a pair of 16-bit floats base<t> + code: the four bits land in the mantissa of
+// the base (in BF16 the lowest code is in place already: 128 + code).  The integer pipe, which has the masks and the
+// shifts, bounds the kernel; shifting by multiplications on the FMA pipe was slower (169 against 154 us).
+template <bool BF16, int t>
+__host__ __device__ constexpr float base_of() { return BF16 && t == 0 ? 128.f : 16.f; }
 template <bool BF16, int t>
 __device__ __forceinline__ uint32_t widen(uint32_t w) {
+    if constexpr (BF16 && t == 0) return (w & 0x000f000fu) | 0x43004300u;
     constexpr int to = BF16 ? 3 : 6, shift = to - 4 * t;  // where the four bits go in the mantissa
     constexpr uint32_t mask = BF16 ? 0x00780078u : 0x03c003c0u, sixteen = BF16 ? 0x41804180u : 0x4c004c00u;
     const uint32_t x = shift >= 0 ? w << (shift >= 0 ? shift : 0) : w >> (shift < 0 ? -shift : 0);
     return (x & mask) | sixteen;
 }
-// The same less 24: code - 8, exactly.
+// The same less base<t> + 8: code - 8, exactly.
 template <bool BF16, int t>
 __device__ __forceinline__ uint32_t centred(uint32_t w) {
     const uint32_t x = widen<BF16, t>(w);
     uint32_t y;
-    if constexpr (BF16) asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x41c041c0u));
+    if constexpr (BF16) asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(t == 0 ? 0x43084308u : 0x41c041c0u));
     else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x4e004e00u));
     return y;
 }
@@ -215,16 +239,12 @@ __device__ __forceinline__ int channel_of(int t, int g, int upper) {
 // Scores of a block in S[mt][n][e] (token mt * 16 + g + 8 * (e >> 1), query row 2i + (e & 1) of row tile n).
 template <typename T, int D, int NT>
 __device__ __forceinline__ void scores_q4(float (&s)[2][NT][4], const uint8_t* codes, const uint8_t* params,
-                                          const uint32_t (&qf)[NT][D / 16][2], const float (&qsum)[NT][2][D / 64], int g,
-                                          int i) {
+                                          const uint32_t (&qf)[NT][D / 16][2], const float (&qsum)[NT][2][D / 64],
+                                          const float (&qbase)[NT][2][D / 64], int g, int i) {
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     using C = Cfg<D, true>;
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[mt][n][e] = 0.f;
         const int t0 = mt * 16 + g;
 #pragma unroll
         for (int grp = 0; grp < C::kGroups; ++grp) {
@@ -238,29 +258,29 @@ __device__ __forceinline__ void scores_q4(float (&s)[2][NT][4], const uint8_t* c
             }
             float acc[NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-#pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const uint32_t a = w[0][x], b = w[1][x];
                 const uint32_t a0 = widen<BF16, 0>(a), a1 = widen<BF16, 1>(a), a2 = widen<BF16, 2>(a), a3 = widen<BF16, 3>(a);
                 const uint32_t b0 = widen<BF16, 0>(b), b1 = widen<BF16, 1>(b), b2 = widen<BF16, 2>(b), b3 = widen<BF16, 3>(b);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    mma<BF16>(acc[n], a0, b0, a1, b1, qf[n][grp * 4 + x * 2][0], qf[n][grp * 4 + x * 2][1]);
+                    if (x == 0)
+                        mma_from<BF16>(acc[n], a0, b0, a1, b1, qf[n][grp * 4][0], qf[n][grp * 4][1], qbase[n][0][grp], qbase[n][1][grp]);
+                    else
+                        mma<BF16>(acc[n], a0, b0, a1, b1, qf[n][grp * 4 + 2][0], qf[n][grp * 4 + 2][1]);
                     mma<BF16>(acc[n], a2, b2, a3, b3, qf[n][grp * 4 + x * 2 + 1][0], qf[n][grp * 4 + x * 2 + 1][1]);
                 }
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const float2 sz = unpack2<BF16>(pr[u]);
-                const float off = fmaf(sz.x, -16.f, sz.y);
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
-                        s[mt][n][2 * u + e] = fmaf(sz.x, acc[n][2 * u + e], fmaf(off, qsum[n][e][grp], s[mt][n][2 * u + e]));
+                        s[mt][n][2 * u + e] =
+                            fmaf(sz.x, acc[n][2 * u + e],
+                                 grp == 0 ? sz.y * qsum[n][e][0] : fmaf(sz.y, qsum[n][e][grp], s[mt][n][2 * u + e]));
             }
         }
     }
@@ -287,16 +307,20 @@ __device__ __forceinline__ void scores_16(float (&s)[1][NT][4], uint32_t tile, c
 // One block: softmax and both products.  CLEAN: every row sees every token of it.
 template <typename T, int D, bool Q4, int NT, bool CLEAN>
 __device__ __forceinline__ void block_step(State<D, Q4, NT>& st, const uint8_t* stage, const uint32_t (&qf)[NT][D / 16][2],
-                                           const float (&qsum)[NT][2][D / 64], const CacheAttentionCall& c, int64_t start,
+                                           const float (&qsum)[NT][2][D / 64], const float (&qbase)[NT][2][D / 64],
+                                           const CacheAttentionCall& c, int64_t start,
                                            int key0, int row0, float c2, int lane) {
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     using C = Cfg<D, Q4>;
     constexpr int MT = C::kBlock / 16;
     const int g = lane >> 2, i = lane & 3;
     float s[MT][NT][4];
-    if constexpr (Q4) scores_q4<T, D, NT>(s, stage, stage + C::kBlock * C::kRow, qf, qsum, g, i);
+    if constexpr (Q4) scores_q4<T, D, NT>(s, stage, stage + C::kBlock * C::kRow, qf, qsum, qbase, g, i);
     else scores_16<T, D, NT>(s, smem_u32(stage), qf, lane);
 
+    // The reference of the probabilities is re-based only when a score beats it by more than 2^kSlack in probability
+    // terms (which keeps p * scale inside FP16): one vote per block instead of a maximum over the lanes.
+    constexpr float kSlack = BF16 ? 8.f : 2.f;
     bool grown = false;
     float mn[NT][2];
 #pragma unroll
@@ -314,17 +338,16 @@ __device__ __forceinline__ void block_step(State<D, Q4, NT>& st, const uint8_t* 
             float mx = st.m[n][e];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) mx = max3(mx, s[mt][n][e], s[mt][n][2 + e]);
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
             mn[n][e] = mx;
-            grown = grown || mx > st.m[n][e];
+            grown = grown || (mx > st.m[n][e] && !((mx - st.m[n][e]) * c2 <= kSlack));  // (also a first score)
         }
     if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) mn[n][e] = fmaxf(mn[n][e], __shfl_xor_sync(0xffffffffu, mn[n][e], o));
                 const float alpha = st.m[n][e] == -INFINITY ? 0.f : ex2((st.m[n][e] - mn[n][e]) * c2);
                 st.m[n][e] = mn[n][e];
                 st.l[n][e] *= alpha;
@@ -431,6 +454,8 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
     constexpr int R = 8 * NT;
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ float sm_m[kWarps][R], sm_l[kWarps][R];
+    __shared__ uint64_t arrived[kWarps][C::kStages];  // 4-bit caches with dense rows: the stage's codes are there
+    __shared__ int abort_word;
     const CacheAttentionCall& c = p.c;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may be scheduled; it waits for this grid
@@ -442,6 +467,18 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
     uint8_t* my_ring = ring + warp * C::kStages * C::kStage;
     const float c2 = fabsf(c.scale) * kLog2e;
     State<D, Q4, NT> st;
+    // Dense rows of codes come as two contiguous copies per block (32 rows of keys, 32 of values), which cost one thread
+    // a few instructions instead of eight address computations per lane.
+    const bool dense = Q4 && c.half[0].cs[2] == C::kRow && c.half[1].cs[2] == C::kRow;
+    uint32_t phases = 0;  // parity of each stage's next arrival
+    if (threadIdx.x == 0) abort_word = *reinterpret_cast<volatile int*>(c.abort_flag) != 0 ? 90 : 0;
+    if (lane == 0) {
+        for (int n = 0; n < C::kStages; ++n) mbar_init(&arrived[warp][n], 1);
+        mbar_fence_init();
+    }
+    __syncthreads();
+    bool ok = abort_word == 0;
+    if (!ok) return;
 
     for (int64_t at = begin; at < end;) {
         int64_t base;
@@ -455,23 +492,47 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
 
         // the copies of this warp's block `n` (blocks warp, warp + kWarps, ... of the piece) into its ring
         const int mine = count > warp ? (count - warp + kWarps - 1) / kWarps : 0;
-        auto request = [&](int n) {
+        const uint8_t* plane[2];
+        const uint8_t* param_plane[2] = {};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            if constexpr (Q4) {
+                const CacheView& v = c.half[half];
+                plane[half] = v.codes + b * v.cs[0] + kvh * v.cs[1];
+                param_plane[half] = reinterpret_cast<const uint8_t*>(v.params + b * v.ps[0] + kvh * v.ps[1]);
+            } else {
+                plane[half] = static_cast<const uint8_t*>(p.kv[half]) + 2 * (b * p.kvs[half][0] + kvh * p.kvs[half][1]);
+            }
+        }
+        auto request = [&](int n, int into) {
             if (n < mine) {
                 const int key0 = blocks.block(from + warp + n * kWarps) * C::kBlock;
-                const uint32_t dst = smem_u32(my_ring + (n % C::kStages) * C::kStage);
+                const uint32_t dst = smem_u32(my_ring + into * C::kStage);
+                if constexpr (Q4) {
+                    const int key = key0 + lane;
+                    const bool live = key < high.hi && (key >= low.lo || key < c.sinks);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
+                        copy_async<C::kParam>(dst + half * C::kHalf + C::kBlock * C::kRow + lane * C::kParam,
+                                              param_plane[half] + (live ? key * c.half[half].ps[2] * 2 : 0), live);
+                    if (dense) {
+                        // (tokens that no row sees come along; rows behind the cache's end do not, and leave what was
+                        // there before: a code is a finite number whatever it is)
+                        if (lane == 0) {
+                            const uint32_t bytes = min(C::kBlock, c.Sk - key0) * C::kRow;
+                            mbar_expect_tx(&arrived[warp][into], 2 * bytes);
+                            copy_bulk(dst, plane[0] + (int64_t)key0 * C::kRow, bytes, &arrived[warp][into]);
+                            copy_bulk(dst + C::kHalf, plane[1] + (int64_t)key0 * C::kRow, bytes, &arrived[warp][into]);
+                        }
+                        copy_commit();
+                        return;
+                    }
+                }
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     constexpr int kChunks = C::kRow / 16;
-                    const uint8_t* src;
-                    int64_t step;
-                    if constexpr (Q4) {
-                        const CacheView& v = c.half[half];
-                        src = v.codes + b * v.cs[0] + kvh * v.cs[1];
-                        step = v.cs[2];
-                    } else {
-                        src = static_cast<const uint8_t*>(p.kv[half]) + 2 * (b * p.kvs[half][0] + kvh * p.kvs[half][1]);
-                        step = 2 * p.kvs[half][2];
-                    }
+                    const uint8_t* src = plane[half];
+                    const int64_t step = Q4 ? c.half[half].cs[2] : 2 * p.kvs[half][2];
 #pragma unroll
                     for (int x = 0; x < C::kBlock * kChunks / 32; ++x) {
                         const int idx = x * 32 + lane, token = idx / kChunks, chunk = idx % kChunks, key = key0 + token;
@@ -479,23 +540,16 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
                         const int to = Q4 ? chunk : chunk ^ (token & 7);
                         copy_async<16>(dst + half * C::kHalf + token * C::kRow + to * 16, src + (live ? key * step : 0) + chunk * 16, live);
                     }
-                    if constexpr (Q4) {
-                        const CacheView& v = c.half[half];
-                        const int key = key0 + lane;
-                        const bool live = key < high.hi && (key >= low.lo || key < c.sinks);
-                        copy_async<C::kParam>(dst + half * C::kHalf + C::kBlock * C::kRow + lane * C::kParam,
-                                              v.params + b * v.ps[0] + kvh * v.ps[1] + (live ? key * v.ps[2] : 0), live);
-                    }
                 }
             }
             copy_commit();
         };
 #pragma unroll
-        for (int n = 0; n < C::kStages - 1; ++n) request(n);
+        for (int n = 0; n < C::kStages - 1; ++n) request(n, n);
 
         // the query rows as operand B, and their sums over the groups
         uint32_t qf[NT][D / 16][2];
-        float qsum[NT][2][D / 64];
+        float qsum[NT][2][D / 64], qbase[NT][2][D / 64];  // sum_d q_d and -sum_d q_d base_d of query rows 2i, 2i + 1
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int r = row0 + n * 8 + g;
@@ -506,7 +560,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
             if constexpr (Q4) {
 #pragma unroll
                 for (int grp = 0; grp < C::kGroups; ++grp) {
-                    float sum = 0.f;
+                    float sum = 0.f, based = 0.f;
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         uint4 raw = live ? *reinterpret_cast<const uint4*>(qrow + grp * 64 + i * 16 + x * 8) : make_uint4(0, 0, 0, 0);
@@ -518,12 +572,18 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
                         qf[n][grp * 4 + x * 2 + 1][1] = __byte_perm(raw.y, raw.w, 0x7632);
                         const float2 e0 = unpack2<BF16>(raw.x), e1 = unpack2<BF16>(raw.y), e2 = unpack2<BF16>(raw.z),
                                      e3 = unpack2<BF16>(raw.w);
-                        sum += ((e0.x + e0.y) + (e1.x + e1.y)) + ((e2.x + e2.y) + (e3.x + e3.y));
+                        const float first = e0.x + e2.x, rest = ((e0.y + e2.y) + (e1.x + e3.x)) + (e1.y + e3.y);
+                        sum += first + rest;
+                        based -= base_of<BF16, 0>() * first + base_of<BF16, 1>() * rest;
                     }
                     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                     sum += __shfl_xor_sync(0xffffffffu, sum, 2);  // row g
+                    based += __shfl_xor_sync(0xffffffffu, based, 1);
+                    based += __shfl_xor_sync(0xffffffffu, based, 2);
                     qsum[n][0][grp] = __shfl_sync(0xffffffffu, sum, 8 * i);
                     qsum[n][1][grp] = __shfl_sync(0xffffffffu, sum, 8 * i + 4);
+                    qbase[n][0][grp] = __shfl_sync(0xffffffffu, based, 8 * i);
+                    qbase[n][1][grp] = __shfl_sync(0xffffffffu, based, 8 * i + 4);
                 }
             } else {
 #pragma unroll
@@ -535,15 +595,28 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
         }
 
         st.clear();
-        for (int n = 0; n < mine; ++n) {
+        for (int n = 0, at_stage = 0; n < mine; ++n) {
             copy_wait<C::kStages - 2>();
+            if (dense) {
+                ok = mbar_wait(&arrived[warp][at_stage], (phases >> at_stage) & 1, &abort_word, 1);
+                if (__any_sync(0xffffffffu, !ok)) {
+                    // gave up: a last, short wait for the copies still under way, then to the tear-down
+                    for (int m = n; m < mine && m < n + C::kStages - 1; ++m) {
+                        const int x = m % C::kStages;
+                        for (int tries = 0; tries < 4096 && !mbar_try_wait(&arrived[warp][x], (phases >> x) & 1); ++tries) {}
+                    }
+                    break;
+                }
+                phases ^= 1u << at_stage;
+            }
             __syncwarp();
-            request(n + C::kStages - 1);  // into the stage that the previous block has left
+            request(n + C::kStages - 1, at_stage == 0 ? C::kStages - 1 : at_stage - 1);  // where the previous block was
             const int key0 = blocks.block(from + warp + n * kWarps) * C::kBlock;
-            const uint8_t* stage = my_ring + (n % C::kStages) * C::kStage;
+            const uint8_t* stage = my_ring + at_stage * C::kStage;
+            at_stage = at_stage + 1 == C::kStages ? 0 : at_stage + 1;
             const bool clean = key0 + C::kBlock <= low.hi && (key0 >= high.lo || key0 + C::kBlock <= c.sinks);
-            if (clean) block_step<T, D, Q4, NT, true>(st, stage, qf, qsum, c, start, key0, row0, c2, lane);
-            else block_step<T, D, Q4, NT, false>(st, stage, qf, qsum, c, start, key0, row0, c2, lane);
+            if (clean) block_step<T, D, Q4, NT, true>(st, stage, qf, qsum, qbase, c, start, key0, row0, c2, lane);
+            else block_step<T, D, Q4, NT, false>(st, stage, qf, qsum, qbase, c, start, key0, row0, c2, lane);
             __syncwarp();
         }
         copy_wait<0>();
@@ -613,8 +686,14 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
                 if (d == 0) *reinterpret_cast<float2*>(p.part_ml + piece * 2) = make_float2(mx, sum);
             }
         }
+        fence_async_smem();  // the next piece's contiguous copies come in behind what was written here
         __syncthreads();
         at += count;
+        if (abort_word != 0) break;
+    }
+    if (threadIdx.x == 0 && abort_word != 0) {
+        *c.status = 5000 + abort_word;
+        *reinterpret_cast<volatile int*>(c.abort_flag) = 1;  // later tensor-memory and decoding launches skip their work
     }
 }
 

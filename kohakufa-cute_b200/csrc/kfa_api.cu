@@ -1422,6 +1422,10 @@ int kfa_cache_attention(const kfa_tensor* q, const kfa_tensor* k_codes, const kf
     p.start = start;
     p.scale = scale;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int err = 0;
+    p.status = status_word(&err, st);
+    if (!p.status) return err;
+    p.abort_flag = abort_flag_of_current_device();
     cudaError_t ce = timed("cache_attention", st,
                            [&] { return kfa::launch_cache_attention(p, q->dtype == KFA_BF16, workspace, st); });
     if (ce != cudaSuccess) return cuda_fail(ce, "cache attention launch");

@@ -41,6 +41,8 @@ struct CacheAttentionCall {
     int sinks;
     int B, Hq, Hkv, Sq, Sk, D, group;  // Sk = rows of the cache
     float scale;
+    int* status;      // as in AttnParams
+    int* abort_flag;
 };
 
 }  // namespace kfa

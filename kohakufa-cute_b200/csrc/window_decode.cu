@@ -25,6 +25,8 @@ CacheAttentionCall call_of(const AttnParams& p) {
     c.D = p.D;
     c.group = p.group;
     c.scale = p.scale;
+    c.status = p.status;
+    c.abort_flag = p.abort_flag;
     return c;
 }
 

@@ -493,9 +493,8 @@ def window_forward(q, k, v, starts, start, window, sinks, scale, statistics=True
     device = q.device
     with _on(device):
         out = torch.empty_like(q)
-        maximum = logsum = None
-        if statistics:
-            maximum, logsum = torch.empty((2, *q.shape[:-1]), device=device, dtype=torch.float32).unbind(0)
+        maximum = torch.empty(q.shape[:-1], device=device, dtype=torch.float32) if statistics else None
+        logsum = torch.empty_like(maximum) if statistics else None
         keep, records = _records(q, k, v, starts, out, maximum, logsum)
         need = lib.kfa_window_forward_workspace_bytes(records[0], records[1], window, sinks, statistics)
         workspace = torch.empty(need, device=device, dtype=torch.uint8) if need else None
