@@ -4,6 +4,10 @@
 
 namespace kfa {
 
+bool cache_attention_countable(const CacheAttentionCall& c) {
+    return c.D == 128 ? rows::countable<128, true>(c) : rows::countable<64, true>(c);
+}
+
 size_t cache_attention_workspace_bytes(const CacheAttentionCall& c) {
     return c.D == 128 ? rows::workspace_bytes<128, true>(c) : rows::workspace_bytes<64, true>(c);
 }

@@ -38,6 +38,7 @@ struct RowsCall {
     int64_t kvs[2][3];    // batch, head, token strides (elements)
     int rows, chunks;     // query rows per K/V head, pieces of 8 * NT of them
     int ctas;
+    uint32_t lowest, others;  // see Bases
     float* part_o;        // [ctas][2][8 NT][D]: a CTA's first and last piece of a unit
     float* part_ml;       // [ctas][2][8 NT][2]: maximum, sum
 };
@@ -49,7 +50,7 @@ constexpr int kWarps = 4;
 // CTAs per SM that registers and shared memory allow (the launch bounds hold the compiler to it).
 template <int D, bool Q4, int NT>
 constexpr int resident() {
-    return Q4 ? (D == 64 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 3 : 2)) : (D == 64 ? 3 : 2);
+    return Q4 ? (D == 64 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 4 : 2)) : (D == 64 ? 3 : 2);
 }
 
 template <int D, bool Q4>
@@ -67,7 +68,7 @@ struct Cfg {
 // ------------------------------------------------------------------ the line of blocks
 struct Blocks {
     int sinks, first, count;  // blocks [0, sinks), then `count - sinks` blocks from `first` on
-    __device__ __forceinline__ int block(int i) const { return i < sinks ? i : first + (i - sinks); }
+    __device__ __forceinline__ int block(int i) const { return i + (i < sinks ? 0 : first - sinks); }
 };
 
 __device__ __forceinline__ Blocks blocks_of(const CacheAttentionCall& c, int64_t start, int size) {
@@ -83,25 +84,23 @@ __device__ __forceinline__ int64_t start_of(const CacheAttentionCall& c, int b) 
     return c.starts ? (int64_t)c.starts[b] : c.start;
 }
 
-// Blocks of the whole call; every lane of the (converged) warp returns the sum.
-__device__ __forceinline__ int64_t total_blocks(const CacheAttentionCall& c, int64_t units, int size) {
-    int64_t sum = 0;
+// Blocks of the whole call (fewer than 2^31: the host sees to that); every lane of the (converged) warp returns the sum.
+__device__ __forceinline__ uint32_t total_blocks(const CacheAttentionCall& c, uint32_t units, int size) {
+    uint32_t sum = 0;
     for (int b = threadIdx.x & 31; b < c.B; b += 32) sum += blocks_of(c, start_of(c, b), size).count;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return sum * units;
+    return __reduce_add_sync(0xffffffffu, sum) * units;
 }
 
 // The sequence that position `at` of the line falls into and the position of its first block.
-__device__ __forceinline__ int sequence_at(const CacheAttentionCall& c, int64_t units, int size, int64_t at, int64_t& base) {
+__device__ __forceinline__ int sequence_at(const CacheAttentionCall& c, uint32_t units, int size, uint32_t at, uint32_t& base) {
     const int lane = threadIdx.x & 31;
-    int64_t before = 0;
+    uint32_t before = 0;
     for (int b0 = 0; b0 < c.B; b0 += 32) {
-        int64_t sum = b0 + lane < c.B ? blocks_of(c, start_of(c, b0 + lane), size).count * units : 0;
-        const int64_t mine = sum;
+        const uint32_t mine = b0 + lane < c.B ? blocks_of(c, start_of(c, b0 + lane), size).count * units : 0;
+        uint32_t sum = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
+            const uint32_t up = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += up;
         }
         const uint32_t hit = __ballot_sync(0xffffffffu, at < before + sum);
@@ -116,10 +115,20 @@ __device__ __forceinline__ int sequence_at(const CacheAttentionCall& c, int64_t 
     return c.B;  // behind the line
 }
 
-// CTAs that get blocks (every one of them at least one), the first block of CTA `i`, and the CTA that owns block `at`.
-__device__ __forceinline__ int used_ctas(int64_t total, int ctas) { return (int)min((int64_t)ctas, total); }
-__device__ __forceinline__ int64_t cta_begin(int64_t total, int ctas, int i) { return total * i / ctas; }
-__device__ __forceinline__ int cta_of(int64_t total, int ctas, int64_t at) { return (int)(((at + 1) * ctas - 1) / total); }
+// The line cut into equal pieces: `ctas` of them get blocks (every one at least one), the first `longer` one block more.
+struct Cut {
+    uint32_t ctas, each, longer;
+    __device__ __forceinline__ Cut(uint32_t total, uint32_t most) {
+        ctas = min(total, most);
+        each = ctas ? total / ctas : 0;
+        longer = total - each * ctas;
+    }
+    __device__ __forceinline__ uint32_t begin(uint32_t i) const { return i * each + min(i, longer); }
+    __device__ __forceinline__ uint32_t owner(uint32_t at) const {
+        const uint32_t split = longer * (each + 1);
+        return at < split ? at / (each + 1) : longer + (at - split) / each;
+    }
+};
 
 // ------------------------------------------------------------------ instructions
 // d = A B + (c0, c1, c0, c1)
@@ -185,18 +194,23 @@ __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group 
 // shifts, bounds the kernel; shifting by multiplications on the FMA pipe was slower (169 against 154 us).
 template <bool BF16, int t>
 __host__ __device__ constexpr float base_of() { return BF16 && t == 0 ? 128.f : 16.f; }
+struct Bases {
+    uint32_t lowest, others;  // the bases' bits in both halves, from the launch: values the compiler does not know stay in
+                              // registers, and mask and base go into one three-input logic instruction
+};
 template <bool BF16, int t>
-__device__ __forceinline__ uint32_t widen(uint32_t w) {
-    if constexpr (BF16 && t == 0) return (w & 0x000f000fu) | 0x43004300u;
-    constexpr int to = BF16 ? 3 : 6, shift = to - 4 * t;  // where the four bits go in the mantissa
-    constexpr uint32_t mask = BF16 ? 0x00780078u : 0x03c003c0u, sixteen = BF16 ? 0x41804180u : 0x4c004c00u;
+__device__ __forceinline__ uint32_t widen(uint32_t w, const Bases& base) {
+    constexpr int to = BF16 ? (t == 0 ? 0 : 3) : 6, shift = to - 4 * t;  // where the four bits go in the mantissa
+    constexpr uint32_t mask = 0x000f000fu << to;
     const uint32_t x = shift >= 0 ? w << (shift >= 0 ? shift : 0) : w >> (shift < 0 ? -shift : 0);
-    return (x & mask) | sixteen;
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "n"(mask), "r"(BF16 && t == 0 ? base.lowest : base.others));
+    return y;
 }
 // The same less base<t> + 8: code - 8, exactly.
 template <bool BF16, int t>
-__device__ __forceinline__ uint32_t centred(uint32_t w) {
-    const uint32_t x = widen<BF16, t>(w);
+__device__ __forceinline__ uint32_t centred(uint32_t w, const Bases& base) {
+    const uint32_t x = widen<BF16, t>(w, base);
     uint32_t y;
     if constexpr (BF16) asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(t == 0 ? 0x43084308u : 0x41c041c0u));
     else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x4e004e00u));
@@ -240,7 +254,7 @@ __device__ __forceinline__ int channel_of(int t, int g, int upper) {
 template <typename T, int D, int NT>
 __device__ __forceinline__ void scores_q4(float (&s)[2][NT][4], const uint8_t* codes, const uint8_t* params,
                                           const uint32_t (&qf)[NT][D / 16][2], const float (&qsum)[NT][2][D / 64],
-                                          const float (&qbase)[NT][2][D / 64], int g, int i) {
+                                          const float (&qbase)[NT][2][D / 64], const Bases& base, int g, int i) {
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     using C = Cfg<D, true>;
 #pragma unroll
@@ -260,8 +274,8 @@ __device__ __forceinline__ void scores_q4(float (&s)[2][NT][4], const uint8_t* c
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const uint32_t a = w[0][x], b = w[1][x];
-                const uint32_t a0 = widen<BF16, 0>(a), a1 = widen<BF16, 1>(a), a2 = widen<BF16, 2>(a), a3 = widen<BF16, 3>(a);
-                const uint32_t b0 = widen<BF16, 0>(b), b1 = widen<BF16, 1>(b), b2 = widen<BF16, 2>(b), b3 = widen<BF16, 3>(b);
+                const uint32_t a0 = widen<BF16, 0>(a, base), a1 = widen<BF16, 1>(a, base), a2 = widen<BF16, 2>(a, base), a3 = widen<BF16, 3>(a, base);
+                const uint32_t b0 = widen<BF16, 0>(b, base), b1 = widen<BF16, 1>(b, base), b2 = widen<BF16, 2>(b, base), b3 = widen<BF16, 3>(b, base);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     if (x == 0)
@@ -308,14 +322,14 @@ __device__ __forceinline__ void scores_16(float (&s)[1][NT][4], uint32_t tile, c
 template <typename T, int D, bool Q4, int NT, bool CLEAN>
 __device__ __forceinline__ void block_step(State<D, Q4, NT>& st, const uint8_t* stage, const uint32_t (&qf)[NT][D / 16][2],
                                            const float (&qsum)[NT][2][D / 64], const float (&qbase)[NT][2][D / 64],
-                                           const CacheAttentionCall& c, int64_t start,
+                                           const CacheAttentionCall& c, const Bases& base, int64_t start,
                                            int key0, int row0, float c2, int lane) {
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     using C = Cfg<D, Q4>;
     constexpr int MT = C::kBlock / 16;
     const int g = lane >> 2, i = lane & 3;
     float s[MT][NT][4];
-    if constexpr (Q4) scores_q4<T, D, NT>(s, stage, stage + C::kBlock * C::kRow, qf, qsum, qbase, g, i);
+    if constexpr (Q4) scores_q4<T, D, NT>(s, stage, stage + C::kBlock * C::kRow, qf, qsum, qbase, base, g, i);
     else scores_16<T, D, NT>(s, smem_u32(stage), qf, lane);
 
     // The reference of the probabilities is re-based only when a score beats it by more than 2^kSlack in probability
@@ -367,13 +381,14 @@ __device__ __forceinline__ void block_step(State<D, Q4, NT>& st, const uint8_t* 
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const float m = !CLEAN && st.m[n][e] == -INFINITY ? 0.f : st.m[n][e];
+            // (the rounding of m c2 is the same factor in every probability of the row, and in their sum)
+            const float mc = !CLEAN && st.m[n][e] == -INFINITY ? 0.f : -st.m[n][e] * c2;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     float& x = s[mt][n][2 * u + e];
-                    const float p = ex2((x - m) * c2);
+                    const float p = ex2(fmaf(x, c2, mc));
                     x = !CLEAN && x == -INFINITY ? 0.f : p;
                     st.l[n][e] += x;
                 }
@@ -417,8 +432,8 @@ __device__ __forceinline__ void block_step(State<D, Q4, NT>& st, const uint8_t* 
                 const uint32_t lo1 = __byte_perm(w[2], w[3], 0x5410), hi1 = __byte_perm(w[2], w[3], 0x7632);
                 auto tile = [&](auto t_) {
                     constexpr int t = decltype(t_)::value;
-                    const uint32_t a0 = centred<BF16, t>(lo0), a1 = centred<BF16, t>(hi0);
-                    const uint32_t a2 = centred<BF16, t>(lo1), a3 = centred<BF16, t>(hi1);
+                    const uint32_t a0 = centred<BF16, t>(lo0, base), a1 = centred<BF16, t>(hi0, base);
+                    const uint32_t a2 = centred<BF16, t>(lo1, base), a3 = centred<BF16, t>(hi1, base);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) mma<BF16>(st.o[grp * 4 + t][n], a0, a1, a2, a3, bf[n][0], bf[n][1]);
                 };
@@ -459,16 +474,17 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
     const CacheAttentionCall& c = p.c;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may be scheduled; it waits for this grid
-    const int64_t units = (int64_t)c.Hkv * p.chunks;
-    const int64_t total = total_blocks(c, units, C::kBlock);
-    const int ctas = used_ctas(total, p.ctas);
-    if ((int)blockIdx.x >= ctas) return;
-    const int64_t begin = cta_begin(total, ctas, blockIdx.x), end = cta_begin(total, ctas, blockIdx.x + 1);
+    const uint32_t units = c.Hkv * p.chunks;
+    const Cut cut(total_blocks(c, units, C::kBlock), p.ctas);
+    if (blockIdx.x >= cut.ctas) return;
+    const uint32_t begin = cut.begin(blockIdx.x), end = cut.begin(blockIdx.x + 1);
     uint8_t* my_ring = ring + warp * C::kStages * C::kStage;
     const float c2 = fabsf(c.scale) * kLog2e;
+    const Bases bases{p.lowest, p.others};
     State<D, Q4, NT> st;
     // Dense rows of codes come as two contiguous copies per block (32 rows of keys, 32 of values), which cost one thread
     // a few instructions instead of eight address computations per lane.
+    const bool packed = Q4 && c.half[0].ps[2] == 2 * C::kGroups && c.half[1].ps[2] == 2 * C::kGroups;
     const bool dense = Q4 && c.half[0].cs[2] == C::kRow && c.half[1].cs[2] == C::kRow;
     uint32_t phases = 0;  // parity of each stage's next arrival
     if (threadIdx.x == 0) abort_word = *reinterpret_cast<volatile int*>(c.abort_flag) != 0 ? 90 : 0;
@@ -480,13 +496,13 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
     bool ok = abort_word == 0;
     if (!ok) return;
 
-    for (int64_t at = begin; at < end;) {
-        int64_t base;
+    for (uint32_t at = begin; at < end;) {
+        uint32_t base;
         const int b = sequence_at(c, units, C::kBlock, at, base);
         const int64_t start = start_of(c, b);
         const Blocks blocks = blocks_of(c, start, C::kBlock);
-        const int unit = (int)((at - base) / blocks.count), from = (int)((at - base) - (int64_t)unit * blocks.count);
-        const int count = (int)min(end - at, (int64_t)(blocks.count - from));
+        const int unit = (int)((at - base) / (uint32_t)blocks.count), from = (int)(at - base) - unit * blocks.count;
+        const int count = min((int)(end - at), blocks.count - from);
         const int kvh = unit / p.chunks, row0 = unit % p.chunks * R;
         const WindowSpan low = window_span(start, 0, c.window, c.Sk), high = window_span(start, c.Sq - 1, c.window, c.Sk);
 
@@ -504,25 +520,37 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
                 plane[half] = static_cast<const uint8_t*>(p.kv[half]) + 2 * (b * p.kvs[half][0] + kvh * p.kvs[half][1]);
             }
         }
+        const bool bulk_params = packed && dense && ((reinterpret_cast<uintptr_t>(param_plane[0]) |
+                                                      reinterpret_cast<uintptr_t>(param_plane[1])) & 15) == 0;
         auto request = [&](int n, int into) {
             if (n < mine) {
                 const int key0 = blocks.block(from + warp + n * kWarps) * C::kBlock;
                 const uint32_t dst = smem_u32(my_ring + into * C::kStage);
                 if constexpr (Q4) {
-                    const int key = key0 + lane;
-                    const bool live = key < high.hi && (key >= low.lo || key < c.sinks);
+                    // scales and zeros come contiguously too where they can (a whole block, 16-byte aligned)
+                    const bool with_params = bulk_params && key0 + C::kBlock <= c.Sk;
+                    if (!with_params) {
+                        const int key = key0 + lane;
+                        const bool live = key < high.hi && (key >= low.lo || key < c.sinks);
 #pragma unroll
-                    for (int half = 0; half < 2; ++half)
-                        copy_async<C::kParam>(dst + half * C::kHalf + C::kBlock * C::kRow + lane * C::kParam,
-                                              param_plane[half] + (live ? key * c.half[half].ps[2] * 2 : 0), live);
+                        for (int half = 0; half < 2; ++half)
+                            copy_async<C::kParam>(dst + half * C::kHalf + C::kBlock * C::kRow + lane * C::kParam,
+                                                  param_plane[half] + (live ? key * c.half[half].ps[2] * 2 : 0), live);
+                    }
                     if (dense) {
                         // (tokens that no row sees come along; rows behind the cache's end do not, and leave what was
                         // there before: a code is a finite number whatever it is)
                         if (lane == 0) {
                             const uint32_t bytes = min(C::kBlock, c.Sk - key0) * C::kRow;
-                            mbar_expect_tx(&arrived[warp][into], 2 * bytes);
-                            copy_bulk(dst, plane[0] + (int64_t)key0 * C::kRow, bytes, &arrived[warp][into]);
-                            copy_bulk(dst + C::kHalf, plane[1] + (int64_t)key0 * C::kRow, bytes, &arrived[warp][into]);
+                            uint64_t* bar = &arrived[warp][into];
+                            mbar_expect_tx(bar, 2 * bytes + (with_params ? 2 * C::kBlock * C::kParam : 0));
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                copy_bulk(dst + half * C::kHalf, plane[half] + (int64_t)key0 * C::kRow, bytes, bar);
+                                if (with_params)
+                                    copy_bulk(dst + half * C::kHalf + C::kBlock * C::kRow,
+                                              param_plane[half] + (int64_t)key0 * C::kParam, C::kBlock * C::kParam, bar);
+                            }
                         }
                         copy_commit();
                         return;
@@ -615,8 +643,8 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
             const uint8_t* stage = my_ring + at_stage * C::kStage;
             at_stage = at_stage + 1 == C::kStages ? 0 : at_stage + 1;
             const bool clean = key0 + C::kBlock <= low.hi && (key0 >= high.lo || key0 + C::kBlock <= c.sinks);
-            if (clean) block_step<T, D, Q4, NT, true>(st, stage, qf, qsum, qbase, c, start, key0, row0, c2, lane);
-            else block_step<T, D, Q4, NT, false>(st, stage, qf, qsum, qbase, c, start, key0, row0, c2, lane);
+            if (clean) block_step<T, D, Q4, NT, true>(st, stage, qf, qsum, qbase, c, bases, start, key0, row0, c2, lane);
+            else block_step<T, D, Q4, NT, false>(st, stage, qf, qsum, qbase, c, bases, start, key0, row0, c2, lane);
             __syncwarp();
         }
         copy_wait<0>();
@@ -705,28 +733,25 @@ __global__ void __launch_bounds__(256) merge_rows(const RowsCall p) {
     using C = Cfg<D, Q4>;
     constexpr int R = 8 * NT;
     const CacheAttentionCall& c = p.c;
-    const int64_t units = (int64_t)c.Hkv * p.chunks;
+    const uint32_t units = c.Hkv * p.chunks;
     const int b = (int)(blockIdx.x / units), unit = (int)(blockIdx.x % units);
     const int kvh = unit / p.chunks, row0 = unit % p.chunks * R;
-    const int64_t total = total_blocks(c, units, C::kBlock);
+    const Cut cut(total_blocks(c, units, C::kBlock), p.ctas);
     const int count = blocks_of(c, start_of(c, b), C::kBlock).count;
-    const int ctas = used_ctas(total, p.ctas);
     int first = 0, last = -1;
-    int64_t u0 = 0;
+    uint32_t u0 = 0;
     if (count > 0) {
-        int64_t base = 0;  // blocks of the sequences before b
+        uint32_t base = 0;  // blocks of the sequences before b
         for (int x = threadIdx.x & 31; x < b; x += 32) base += blocks_of(c, start_of(c, x), C::kBlock).count;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) base += __shfl_xor_sync(0xffffffffu, base, o);
-        u0 = base * units + (int64_t)unit * count;
-        first = cta_of(total, ctas, u0);
-        last = cta_of(total, ctas, u0 + count - 1);
+        u0 = __reduce_add_sync(0xffffffffu, base) * units + (uint32_t)unit * count;
+        first = (int)cut.owner(u0);
+        last = (int)cut.owner(u0 + count - 1);
     }
     // (also where there is nothing to merge: this grid's end has to mean the end of the other one)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (count > 0 && first == last) return;
     const float c2 = fabsf(c.scale) * kLog2e;
-    const int slot0 = count > 0 && u0 == cta_begin(total, ctas, first) ? 0 : 1;
+    const int slot0 = count > 0 && u0 == cut.begin(first) ? 0 : 1;
     for (int idx = threadIdx.x; idx < R * (D / 4); idx += 256) {
         const int r = idx / (D / 4), d = idx % (D / 4) * 4, row = row0 + r;
         if (row >= p.rows) continue;
@@ -760,6 +785,13 @@ int64_t most_blocks(const CacheAttentionCall& c) {  // of one unit
     return some < all ? some : all;
 }
 
+// Whether the line of blocks can be counted in 31 bits.
+template <int D, bool Q4>
+bool countable(const CacheAttentionCall& c) {
+    const int64_t chunks = ((int64_t)c.group * c.Sq + 7) / 8;
+    return (int64_t)c.B * c.Hkv * chunks <= INT32_MAX && (int64_t)c.B * c.Hkv * chunks * most_blocks<D, Q4>(c) <= INT32_MAX;
+}
+
 inline int row_tiles(const CacheAttentionCall& c) { return (int64_t)c.group * c.Sq <= 8 ? 1 : 2; }
 
 template <int D, bool Q4, int NT>
@@ -787,6 +819,8 @@ cudaError_t launch(RowsCall& p, void* workspace, cudaStream_t st) {
     p.rows = p.c.group * p.c.Sq;
     p.chunks = (p.rows + R - 1) / R;
     p.ctas = plan_ctas<D, Q4, NT>(p.c, p.chunks);
+    p.lowest = std::is_same<T, __nv_bfloat16>::value ? 0x43004300u : 0x4c004c00u;  // 128 or 16
+    p.others = std::is_same<T, __nv_bfloat16>::value ? 0x41804180u : 0x4c004c00u;  // 16
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = p.part_o + (size_t)p.ctas * 2 * R * D;
     // the shared-memory opt-in holds per device; a decoding step is short enough for the call to show, so it is made once

@@ -1336,7 +1336,7 @@ int fill_cache_attention(kfa::CacheAttentionCall& p, const kfa_tensor* q, const 
                     "cache attention requires matching batch and channels, and query heads divisible by K/V heads");
     if (q->sizes[3] != 64 && q->sizes[3] != 128)
         return fail(KFA_INVALID_ARGUMENT, "cache attention requires head dimensions 64 or 128");
-    if (q->sizes[0] * q->sizes[1] * q->sizes[2] > INT32_MAX / 64)
+    if (q->sizes[1] * q->sizes[2] > INT32_MAX || q->sizes[0] * q->sizes[1] > INT32_MAX)
         return fail(KFA_TOO_LARGE, "cache attention: too many query rows in one call");
     if (window < 0 || sinks < 0) return fail(KFA_INVALID_ARGUMENT, "cache attention requires window >= 0 and sinks >= 0");
     p.B = (int)q->sizes[0];
@@ -1349,6 +1349,8 @@ int fill_cache_attention(kfa::CacheAttentionCall& p, const kfa_tensor* q, const 
     // no window: longer than every position a 32-bit start can reach
     p.window = window == 0 ? int64_t(1) << 40 : std::min<int64_t>(window, int64_t(1) << 40);
     p.sinks = (int)std::min<int64_t>(sinks, p.Sk);
+    if (!kfa::cache_attention_countable(p))
+        return fail(KFA_TOO_LARGE, "cache attention: too many query rows and keys in one call");
     return 0;
 }
 

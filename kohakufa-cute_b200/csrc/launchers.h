@@ -46,6 +46,7 @@ cudaError_t launch_window_decode(const AttnParams& p, bool bf16, void* workspace
 // 4-bit key/value cache: rows quantised into it, read back, attended to.
 cudaError_t launch_cache_write(const CacheCall& p, bool bf16, cudaStream_t st);
 cudaError_t launch_cache_read(const CacheCall& p, bool bf16, cudaStream_t st);
+bool cache_attention_countable(const CacheAttentionCall& p);  // else too large for one call
 size_t cache_attention_workspace_bytes(const CacheAttentionCall& p);
 cudaError_t launch_cache_attention(const CacheAttentionCall& p, bool bf16, void* workspace, cudaStream_t st);
 

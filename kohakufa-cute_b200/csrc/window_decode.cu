@@ -33,7 +33,9 @@ CacheAttentionCall call_of(const AttnParams& p) {
 }  // namespace
 
 bool window_decode_shape(const AttnParams& p) {
-    return (p.D == 64 || p.D == 128) && (int64_t)p.Sq * p.group <= 16;
+    if ((p.D != 64 && p.D != 128) || (int64_t)p.Sq * p.group > 16) return false;
+    const CacheAttentionCall c = call_of(p);
+    return p.D == 128 ? rows::countable<128, false>(c) : rows::countable<64, false>(c);
 }
 
 size_t window_decode_workspace_bytes(const AttnParams& p) {
