@@ -50,18 +50,18 @@ constexpr int kWarps = 4;
 // CTAs per SM that registers and shared memory allow (the launch bounds hold the compiler to it).
 template <int D, bool Q4, int NT>
 constexpr int resident() {
-    return Q4 ? (D == 64 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 4 : 2)) : (D == 64 ? 3 : 2);
+    return Q4 ? (D == 64 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 3 : 2)) : (D == 64 ? 3 : 2);
 }
 
-template <int D, bool Q4>
+template <int D, bool Q4, int NT>
 struct Cfg {
     static constexpr int kGroups = D / kCacheGroup;
-    static constexpr int kBlock = Q4 ? 32 : 16;                // tokens per block
+    static constexpr int kBlock = Q4 ? (NT == 1 ? 64 : 32) : 16;                // tokens per block
     static constexpr int kRow = Q4 ? D / 2 : D * 2;            // bytes of a token's codes or channels
     static constexpr int kParam = Q4 ? 4 * kGroups : 0;        // bytes of a token's scales and zeros
     static constexpr int kHalf = kBlock * (kRow + kParam);     // one block of keys or of values
     static constexpr int kStage = 2 * kHalf;
-    static constexpr int kStages = Q4 ? (D == 64 ? 4 : 3) : (D == 64 ? 4 : 3);
+    static constexpr int kStages = Q4 ? (D == 128 && NT == 1 ? 2 : 3) : (D == 64 ? 4 : 3);
     static constexpr int kRing = kWarps * kStages * kStage;
 };
 
@@ -84,36 +84,46 @@ __device__ __forceinline__ int64_t start_of(const CacheAttentionCall& c, int b) 
     return c.starts ? (int64_t)c.starts[b] : c.start;
 }
 
-// Blocks of the whole call (fewer than 2^31: the host sees to that); every lane of the (converged) warp returns the sum.
-__device__ __forceinline__ uint32_t total_blocks(const CacheAttentionCall& c, uint32_t units, int size) {
-    uint32_t sum = 0;
-    for (int b = threadIdx.x & 31; b < c.B; b += 32) sum += blocks_of(c, start_of(c, b), size).count;
-    return __reduce_add_sync(0xffffffffu, sum) * units;
-}
-
-// The sequence that position `at` of the line falls into and the position of its first block.
-__device__ __forceinline__ int sequence_at(const CacheAttentionCall& c, uint32_t units, int size, uint32_t at, uint32_t& base) {
-    const int lane = threadIdx.x & 31;
-    uint32_t before = 0;
-    for (int b0 = 0; b0 < c.B; b0 += 32) {
-        const uint32_t mine = b0 + lane < c.B ? blocks_of(c, start_of(c, b0 + lane), size).count * units : 0;
-        uint32_t sum = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t up = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += up;
-        }
-        const uint32_t hit = __ballot_sync(0xffffffffu, at < before + sum);
-        if (hit) {
-            const int src = __ffs(hit) - 1;
-            base = before + __shfl_sync(0xffffffffu, sum - mine, src);
-            return b0 + src;
-        }
-        before += __shfl_sync(0xffffffffu, sum, 31);
+// The blocks of the sequences, a lane of the (converged) warp per sequence: those of a batch of up to 32 are formed once.
+struct Line {
+    const CacheAttentionCall& c;
+    uint32_t units;
+    int size, lane;
+    uint32_t mine;  // blocks of sequence `lane` in all its units
+    __device__ __forceinline__ uint32_t of(int b) const {
+        return b < c.B ? blocks_of(c, start_of(c, b), size).count * units : 0u;
     }
-    base = before;
-    return c.B;  // behind the line
-}
+    __device__ __forceinline__ Line(const CacheAttentionCall& call, uint32_t units_, int size_)
+        : c(call), units(units_), size(size_), lane(threadIdx.x & 31), mine(of(threadIdx.x & 31)) {}
+    // Blocks of the sequences before `end` (fewer than 2^31 in all: the host sees to that).
+    __device__ __forceinline__ uint32_t before(int end) const {
+        uint32_t sum = lane < end ? mine : 0u;
+        for (int b = lane + 32; b < end; b += 32) sum += of(b);
+        return __reduce_add_sync(0xffffffffu, sum);
+    }
+    // The sequence that position `at` of the line falls into and the position of its first block.
+    __device__ __forceinline__ int sequence_at(uint32_t at, uint32_t& base) const {
+        uint32_t done = 0;
+        for (int b0 = 0; b0 < c.B; b0 += 32) {
+            const uint32_t here = b0 == 0 ? mine : of(b0 + lane);
+            uint32_t sum = here;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t up = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += up;
+            }
+            const uint32_t hit = __ballot_sync(0xffffffffu, at < done + sum);
+            if (hit) {
+                const int src = __ffs(hit) - 1;
+                base = done + __shfl_sync(0xffffffffu, sum - here, src);
+                return b0 + src;
+            }
+            done += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        base = done;
+        return c.B;  // behind the line
+    }
+};
 
 // The line cut into equal pieces: `ctas` of them get blocks (every one at least one), the first `longer` one block more.
 struct Cut {
@@ -207,7 +217,8 @@ __device__ __forceinline__ uint32_t widen(uint32_t w, const Bases& base) {
     asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "n"(mask), "r"(BF16 && t == 0 ? base.lowest : base.others));
     return y;
 }
-// The same less base<t> + 8: code - 8, exactly.
+// The same less base<t> + 8: code - 8, exactly.  (Taking the bases off by one more product, with a constant operand, was
+// slower: 122 against 112 us at 16 x 32768 tokens.)
 template <bool BF16, int t>
 __device__ __forceinline__ uint32_t centred(uint32_t w, const Bases& base) {
     const uint32_t x = widen<BF16, t>(w, base);
@@ -252,13 +263,13 @@ __device__ __forceinline__ int channel_of(int t, int g, int upper) {
 
 // Scores of a block in S[mt][n][e] (token mt * 16 + g + 8 * (e >> 1), query row 2i + (e & 1) of row tile n).
 template <typename T, int D, int NT>
-__device__ __forceinline__ void scores_q4(float (&s)[2][NT][4], const uint8_t* codes, const uint8_t* params,
+__device__ __forceinline__ void scores_q4(float (&s)[Cfg<D, true, NT>::kBlock / 16][NT][4], const uint8_t* codes, const uint8_t* params,
                                           const uint32_t (&qf)[NT][D / 16][2], const float (&qsum)[NT][2][D / 64],
                                           const float (&qbase)[NT][2][D / 64], const Bases& base, int g, int i) {
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-    using C = Cfg<D, true>;
+    using C = Cfg<D, true, NT>;
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
+    for (int mt = 0; mt < C::kBlock / 16; ++mt) {
         const int t0 = mt * 16 + g;
 #pragma unroll
         for (int grp = 0; grp < C::kGroups; ++grp) {
@@ -325,7 +336,7 @@ __device__ __forceinline__ void block_step(State<D, Q4, NT>& st, const uint8_t* 
                                            const CacheAttentionCall& c, const Bases& base, int64_t start,
                                            int key0, int row0, float c2, int lane) {
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-    using C = Cfg<D, Q4>;
+    using C = Cfg<D, Q4, NT>;
     constexpr int MT = C::kBlock / 16;
     const int g = lane >> 2, i = lane & 3;
     float s[MT][NT][4];
@@ -465,7 +476,7 @@ __device__ __forceinline__ void block_step(State<D, Q4, NT>& st, const uint8_t* 
 template <typename T, int D, bool Q4, int NT>
 __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_rows(const RowsCall p) {
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-    using C = Cfg<D, Q4>;
+    using C = Cfg<D, Q4, NT>;
     constexpr int R = 8 * NT;
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ float sm_m[kWarps][R], sm_l[kWarps][R];
@@ -475,7 +486,8 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may be scheduled; it waits for this grid
     const uint32_t units = c.Hkv * p.chunks;
-    const Cut cut(total_blocks(c, units, C::kBlock), p.ctas);
+    const Line line(c, units, C::kBlock);
+    const Cut cut(line.before(c.B), p.ctas);
     if (blockIdx.x >= cut.ctas) return;
     const uint32_t begin = cut.begin(blockIdx.x), end = cut.begin(blockIdx.x + 1);
     uint8_t* my_ring = ring + warp * C::kStages * C::kStage;
@@ -486,7 +498,8 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
     // a few instructions instead of eight address computations per lane.
     const bool packed = Q4 && c.half[0].ps[2] == 2 * C::kGroups && c.half[1].ps[2] == 2 * C::kGroups;
     const bool dense = Q4 && c.half[0].cs[2] == C::kRow && c.half[1].cs[2] == C::kRow;
-    uint32_t phases = 0;  // parity of each stage's next arrival
+    int at_stage = 0, into = 0;   // the stage that is read next, and the one that is filled next
+    uint32_t parity = 0;          // of the arrival at the stage that is read next
     if (threadIdx.x == 0) abort_word = *reinterpret_cast<volatile int*>(c.abort_flag) != 0 ? 90 : 0;
     if (lane == 0) {
         for (int n = 0; n < C::kStages; ++n) mbar_init(&arrived[warp][n], 1);
@@ -498,7 +511,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
 
     for (uint32_t at = begin; at < end;) {
         uint32_t base;
-        const int b = sequence_at(c, units, C::kBlock, at, base);
+        const int b = line.sequence_at(at, base);
         const int64_t start = start_of(c, b);
         const Blocks blocks = blocks_of(c, start, C::kBlock);
         const int unit = (int)((at - base) / (uint32_t)blocks.count), from = (int)(at - base) - unit * blocks.count;
@@ -522,7 +535,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
         }
         const bool bulk_params = packed && dense && ((reinterpret_cast<uintptr_t>(param_plane[0]) |
                                                       reinterpret_cast<uintptr_t>(param_plane[1])) & 15) == 0;
-        auto request = [&](int n, int into) {
+        auto request = [&](int n) {
             if (n < mine) {
                 const int key0 = blocks.block(from + warp + n * kWarps) * C::kBlock;
                 const uint32_t dst = smem_u32(my_ring + into * C::kStage);
@@ -530,12 +543,15 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
                     // scales and zeros come contiguously too where they can (a whole block, 16-byte aligned)
                     const bool with_params = bulk_params && key0 + C::kBlock <= c.Sk;
                     if (!with_params) {
-                        const int key = key0 + lane;
-                        const bool live = key < high.hi && (key >= low.lo || key < c.sinks);
 #pragma unroll
-                        for (int half = 0; half < 2; ++half)
-                            copy_async<C::kParam>(dst + half * C::kHalf + C::kBlock * C::kRow + lane * C::kParam,
-                                                  param_plane[half] + (live ? key * c.half[half].ps[2] * 2 : 0), live);
+                        for (int token = lane; token < C::kBlock; token += 32) {
+                            const int key = key0 + token;
+                            const bool live = key < high.hi && (key >= low.lo || key < c.sinks);
+#pragma unroll
+                            for (int half = 0; half < 2; ++half)
+                                copy_async<C::kParam>(dst + half * C::kHalf + C::kBlock * C::kRow + token * C::kParam,
+                                                      param_plane[half] + (live ? key * c.half[half].ps[2] * 2 : 0), live);
+                        }
                     }
                     if (dense) {
                         // (tokens that no row sees come along; rows behind the cache's end do not, and leave what was
@@ -553,6 +569,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
                             }
                         }
                         copy_commit();
+                        into = into + 1 == C::kStages ? 0 : into + 1;
                         return;
                     }
                 }
@@ -569,11 +586,12 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
                         copy_async<16>(dst + half * C::kHalf + token * C::kRow + to * 16, src + (live ? key * step : 0) + chunk * 16, live);
                     }
                 }
+                into = into + 1 == C::kStages ? 0 : into + 1;
             }
             copy_commit();
         };
 #pragma unroll
-        for (int n = 0; n < C::kStages - 1; ++n) request(n, n);
+        for (int n = 0; n < C::kStages - 1; ++n) request(n);
 
         // the query rows as operand B, and their sums over the groups
         uint32_t qf[NT][D / 16][2];
@@ -623,25 +641,26 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
         }
 
         st.clear();
-        for (int n = 0, at_stage = 0; n < mine; ++n) {
+        for (int n = 0; n < mine; ++n) {
             copy_wait<C::kStages - 2>();
             if (dense) {
-                ok = mbar_wait(&arrived[warp][at_stage], (phases >> at_stage) & 1, &abort_word, 1);
+                ok = mbar_wait(&arrived[warp][at_stage], parity, &abort_word, 1);
                 if (__any_sync(0xffffffffu, !ok)) {
                     // gave up: a last, short wait for the copies still under way, then to the tear-down
                     for (int m = n; m < mine && m < n + C::kStages - 1; ++m) {
-                        const int x = m % C::kStages;
-                        for (int tries = 0; tries < 4096 && !mbar_try_wait(&arrived[warp][x], (phases >> x) & 1); ++tries) {}
+                        for (int tries = 0; tries < 4096 && !mbar_try_wait(&arrived[warp][at_stage], parity); ++tries) {}
+                        at_stage = at_stage + 1 == C::kStages ? 0 : at_stage + 1;
+                        parity ^= at_stage == 0 ? 1u : 0u;
                     }
                     break;
                 }
-                phases ^= 1u << at_stage;
             }
             __syncwarp();
-            request(n + C::kStages - 1, at_stage == 0 ? C::kStages - 1 : at_stage - 1);  // where the previous block was
+            request(n + C::kStages - 1);  // into the stage that the previous block has left
             const int key0 = blocks.block(from + warp + n * kWarps) * C::kBlock;
             const uint8_t* stage = my_ring + at_stage * C::kStage;
             at_stage = at_stage + 1 == C::kStages ? 0 : at_stage + 1;
+            parity ^= at_stage == 0 ? 1u : 0u;
             const bool clean = key0 + C::kBlock <= low.hi && (key0 >= high.lo || key0 + C::kBlock <= c.sinks);
             if (clean) block_step<T, D, Q4, NT, true>(st, stage, qf, qsum, qbase, c, bases, start, key0, row0, c2, lane);
             else block_step<T, D, Q4, NT, false>(st, stage, qf, qsum, qbase, c, bases, start, key0, row0, c2, lane);
@@ -725,25 +744,25 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
     }
 }
 
-// One CTA per unit: units that one CTA served whole are done; the others' pieces are merged in order; a sequence
-// without a visible key gets its zeros here.
+// One CTA per unit: units that one CTA served whole are done; the others' pieces are merged, in an order that the cut
+// alone decides; a sequence without a visible key gets its zeros here.
 template <typename T, int D, bool Q4, int NT>
-__global__ void __launch_bounds__(256) merge_rows(const RowsCall p) {
+__global__ void __launch_bounds__(1024) merge_rows(const RowsCall p) {
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-    using C = Cfg<D, Q4>;
+    using C = Cfg<D, Q4, NT>;
     constexpr int R = 8 * NT;
+    constexpr int kLanes = D / 4, kParts = 1024 / kLanes / R;  // four channels per thread; a row's pieces kParts at a time
     const CacheAttentionCall& c = p.c;
     const uint32_t units = c.Hkv * p.chunks;
     const int b = (int)(blockIdx.x / units), unit = (int)(blockIdx.x % units);
     const int kvh = unit / p.chunks, row0 = unit % p.chunks * R;
-    const Cut cut(total_blocks(c, units, C::kBlock), p.ctas);
+    const Line line(c, units, C::kBlock);
+    const Cut cut(line.before(c.B), p.ctas);
     const int count = blocks_of(c, start_of(c, b), C::kBlock).count;
     int first = 0, last = -1;
     uint32_t u0 = 0;
     if (count > 0) {
-        uint32_t base = 0;  // blocks of the sequences before b
-        for (int x = threadIdx.x & 31; x < b; x += 32) base += blocks_of(c, start_of(c, x), C::kBlock).count;
-        u0 = __reduce_add_sync(0xffffffffu, base) * units + (uint32_t)unit * count;
+        u0 = line.before(b) + (uint32_t)unit * count;
         first = (int)cut.owner(u0);
         last = (int)cut.owner(u0 + count - 1);
     }
@@ -752,34 +771,56 @@ __global__ void __launch_bounds__(256) merge_rows(const RowsCall p) {
     if (count > 0 && first == last) return;
     const float c2 = fabsf(c.scale) * kLog2e;
     const int slot0 = count > 0 && u0 == cut.begin(first) ? 0 : 1;
-    for (int idx = threadIdx.x; idx < R * (D / 4); idx += 256) {
-        const int r = idx / (D / 4), d = idx % (D / 4) * 4, row = row0 + r;
-        if (row >= p.rows) continue;
-        float mx = -INFINITY, sum = 0.f;
-        for (int i = first; i <= last; ++i)
-            mx = fmaxf(mx, p.part_ml[(((int64_t)i * 2 + (i == first ? slot0 : 0)) * R + r) * 2]);
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int i = first; i <= last; ++i) {
-            const int64_t piece = ((int64_t)i * 2 + (i == first ? slot0 : 0)) * R + r;
-            const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + piece * 2);
-            const float4 x = *reinterpret_cast<const float4*>(p.part_o + piece * D + d);
-            const float weight = ml.x == -INFINITY ? 0.f : ex2((ml.x - mx) * c2);
-            sum += ml.y * weight;
+    const int lane = threadIdx.x % kLanes, part = threadIdx.x / kLanes % kParts, r = threadIdx.x / kLanes / kParts, d = lane * 4;
+    if (row0 + r >= p.rows) last = -1;  // (first > last: nothing to do, and nothing written below)
+    float mx = -INFINITY, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    // this thread's pieces (part, part + kParts, ...): their loads do not depend on one another
+#pragma unroll 8
+    for (int i = first + part; i <= last; i += kParts) {
+        const int64_t piece = ((int64_t)i * 2 + (i == first ? slot0 : 0)) * R + r;
+        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + piece * 2);
+        const float4 x = *reinterpret_cast<const float4*>(p.part_o + piece * D + d);
+        const float m = fmaxf(mx, ml.x);
+        const float keep = mx == -INFINITY ? 0.f : ex2((mx - m) * c2), weight = ml.x == -INFINITY ? 0.f : ex2((ml.x - m) * c2);
+        mx = m;
+        sum = sum * keep + ml.y * weight;
+        acc.x = fmaf(x.x, weight, acc.x * keep), acc.y = fmaf(x.y, weight, acc.y * keep);
+        acc.z = fmaf(x.z, weight, acc.z * keep), acc.w = fmaf(x.w, weight, acc.w * keep);
+    }
+    if constexpr (kParts > 1) {
+        __shared__ float sm_m[R][kParts], sm_l[R][kParts];
+        __shared__ float4 sm_o[R][kParts][kLanes];
+        sm_o[r][part][lane] = acc;
+        if (lane == 0) {
+            sm_m[r][part] = mx;
+            sm_l[r][part] = sum;
+        }
+        __syncthreads();
+        if (part != 0) return;
+        for (int w = 1; w < kParts; ++w) mx = fmaxf(mx, sm_m[r][w]);
+        sum = 0.f;
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kParts; ++w) {
+            const float weight = sm_m[r][w] == -INFINITY ? 0.f : ex2((sm_m[r][w] - mx) * c2);
+            const float4 x = sm_o[r][w][lane];
+            sum += sm_l[r][w] * weight;
             acc.x = fmaf(x.x, weight, acc.x), acc.y = fmaf(x.y, weight, acc.y);
             acc.z = fmaf(x.z, weight, acc.z), acc.w = fmaf(x.w, weight, acc.w);
         }
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
-        T* out = static_cast<T*>(c.out) + b * c.os[0] + (kvh * c.group + row / c.Sq) * c.os[1] + row % c.Sq * c.os[2] + d;
-        *reinterpret_cast<uint2*>(out) =
-            make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
     }
+    if (row0 + r >= p.rows) return;
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const int row = row0 + r;
+    T* out = static_cast<T*>(c.out) + b * c.os[0] + (kvh * c.group + row / c.Sq) * c.os[1] + row % c.Sq * c.os[2] + d;
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
 }
 
 // ------------------------------------------------------------------ host
-template <int D, bool Q4>
+template <int D, bool Q4, int NT>
 int64_t most_blocks(const CacheAttentionCall& c) {  // of one unit
-    constexpr int size = Cfg<D, Q4>::kBlock;
+    constexpr int size = Cfg<D, Q4, NT>::kBlock;
     const int64_t keys = c.window < c.Sk ? c.window + c.Sq - 1 : c.Sk;
     const int64_t all = (c.Sk + size - 1) / size, some = (keys + size - 1) / size + 1 + (c.sinks + size - 1) / size;
     return some < all ? some : all;
@@ -789,7 +830,7 @@ int64_t most_blocks(const CacheAttentionCall& c) {  // of one unit
 template <int D, bool Q4>
 bool countable(const CacheAttentionCall& c) {
     const int64_t chunks = ((int64_t)c.group * c.Sq + 7) / 8;
-    return (int64_t)c.B * c.Hkv * chunks <= INT32_MAX && (int64_t)c.B * c.Hkv * chunks * most_blocks<D, Q4>(c) <= INT32_MAX;
+    return (int64_t)c.B * c.Hkv * chunks * 8 <= INT32_MAX && (int64_t)c.B * c.Hkv * chunks * most_blocks<D, Q4, 2>(c) <= INT32_MAX;
 }
 
 inline int row_tiles(const CacheAttentionCall& c) { return (int64_t)c.group * c.Sq <= 8 ? 1 : 2; }
@@ -797,7 +838,7 @@ inline int row_tiles(const CacheAttentionCall& c) { return (int64_t)c.group * c.
 template <int D, bool Q4, int NT>
 int plan_ctas(const CacheAttentionCall& c, int chunks) {
     // As many CTAs as are resident at once, but no fewer blocks for a CTA than it has warps.
-    const int64_t line = (int64_t)c.B * c.Hkv * chunks * most_blocks<D, Q4>(c);
+    const int64_t line = (int64_t)c.B * c.Hkv * chunks * most_blocks<D, Q4, NT>(c);
     const int64_t most = 148 * resident<D, Q4, NT>();
     const int64_t want = (line + kWarps - 1) / kWarps;
     return (int)(want < 1 ? 1 : (want > most ? most : want));
@@ -812,7 +853,7 @@ size_t workspace_bytes(const CacheAttentionCall& c) {
 
 template <typename T, int D, bool Q4, int NT>
 cudaError_t launch(RowsCall& p, void* workspace, cudaStream_t st) {
-    using C = Cfg<D, Q4>;
+    using C = Cfg<D, Q4, NT>;
     constexpr int R = 8 * NT;
     constexpr int kMerge = kWarps * R * D * 4;
     constexpr int kSmem = C::kRing > kMerge ? C::kRing : kMerge;
@@ -839,7 +880,7 @@ cudaError_t launch(RowsCall& p, void* workspace, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned)((int64_t)p.c.B * p.c.Hkv * p.chunks));
-    config.blockDim = dim3(256);
+    config.blockDim = dim3(1024);
     config.stream = st;
     cudaLaunchAttribute dependent[1];
     dependent[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
