@@ -3,7 +3,7 @@
 // beyond the head with zeros, which add nothing to either product, and the tiled store drops them again),
 // FP16/BF16, causal and/or boolean masks, grouped-query heads.
 //
-// One CTA owns 256 query rows of one (batch, query head) as two 128-row tiles and walks
+// One CTA owns 256 query rows of one (batch, query head) as two 128-row tiles (windowed calls: 128 as one) and walks
 // the 128-key tiles they can see.  Warp roles (384 threads):
 //   warps 0-3  softmax of query tile 0   (thread i <-> TMEM lane i <-> query row i)
 //   warps 4-7  softmax of query tile 1
@@ -41,7 +41,10 @@ namespace {
 
 constexpr int kTileQ = 128;
 constexpr int kTileK = 128;
-constexpr int kThreads = 384;  // three warpgroups: softmax 0, softmax 1, (MMA, loader, 2 idle warps)
+// Query tiles per CTA: two that share their K/V tiles, in one CTA per SM; in windowed calls one, in two CTAs per SM.  A
+// window gives a CTA only a few key tiles (ten at a window of 1024), so that start-up and drain, which a CTA alone on its
+// SM leaves idle, were a third of its time.
+__host__ __device__ constexpr int threads_of(int tiles) { return 128 * tiles + 128; }  // softmax warpgroups; (MMA, loader, 2 idle warps)
 // The accumulator is re-based when the row maximum has grown by more than 2^kRebase in probability terms.  Until then
 // probabilities are formed against the stale maximum and may reach 2^kRebase: 2^14 stays inside FP16, and BF16 has
 // FP32's range (row sums stay below 2^32 * keys, far inside FP32).  Re-basing costs a round trip of the output
@@ -50,13 +53,13 @@ template <bool BF16>
 __host__ __device__ constexpr float rebase_limit() { return BF16 ? 32.0f : 14.0f; }
 constexpr int kMaxKeyTiles = 4096;  // masked calls keep one state byte per key tile in shared memory
 
-template <int D>
+template <int D, int TILES>
 struct FwdCfg {
     static constexpr int kChunks = D / 64;                 // 64-channel TMA boxes per tile
     static constexpr int kTileBytes = kTileK * D * 2;      // one Q, K or V tile
-    static constexpr int kStages = D == 128 ? 4 : 6;       // K/V ring slots
+    static constexpr int kStages = TILES == 2 ? (D == 128 ? 4 : 6) : (D == 128 ? 2 : 4);  // K/V ring slots
     static constexpr int kSmemBytes =
-        2 * kTileBytes + kStages * kTileBytes + 1024 /*align*/ + 256 /*barriers*/ + kMaxKeyTiles;
+        TILES * kTileBytes + kStages * kTileBytes + 1024 /*align*/ + 256 /*barriers*/ + kMaxKeyTiles;
 };
 
 struct FwdMaps {
@@ -102,17 +105,20 @@ __device__ __forceinline__ int key_tile_state(const AttnParams& p, int b, int h,
 // walks the key tiles of the sinks and of its window, two tiles of a CTA need not see the same ones, and positions
 // come from device memory where the call gives one per sequence.
 template <int D, bool BF16, bool MASKED, bool WINDOW>
-__global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_constant__ FwdMaps maps, AttnParams p) {
+__global__ void __launch_bounds__(threads_of(WINDOW ? 1 : 2), WINDOW ? 2 : 1)
+    pipeline_forward(const __grid_constant__ FwdMaps maps, AttnParams p) {
     if (!MASKED) p.has_mask = 0;
-    using Cfg = FwdCfg<D>;
+    constexpr int kTiles = WINDOW ? 1 : 2, kThreads = threads_of(kTiles), kRoleWarp = 4 * kTiles;
+    constexpr uint32_t kColO = 128 * kTiles, kTmemCols = 256 * kTiles;  // accumulators behind the score tiles
+    using Cfg = FwdCfg<D, kTiles>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sQ = smem;                          // two query tiles
-    uint8_t* sKV = smem + 2 * Cfg::kTileBytes;   // ring of K/V tiles
+    uint8_t* sKV = smem + kTiles * Cfg::kTileBytes;   // ring of K/V tiles
     Shared& sh = *reinterpret_cast<Shared*>(sKV + Cfg::kStages * Cfg::kTileBytes);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int nblk = (p.Sq + 2 * kTileQ - 1) / (2 * kTileQ);
+    const int nblk = (p.Sq + kTiles * kTileQ - 1) / (kTiles * kTileQ);
     // Heavy (late) causal blocks first.  Large grids go head by head (a head's CTAs share K/V in L2 and the
     // last wave is made of light blocks); grids of a few waves go block-row by block-row over all heads, so
     // that no head's heavy blocks start in the last wave.
@@ -124,7 +130,7 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
     const int64_t bh = by_row ? blockIdx.x % nbh : blockIdx.x / nblk;
     const int h = (int)(bh % p.Hq), b = (int)(bh / p.Hq);
     const int kvh = h / p.group;
-    const int q0 = qblk * 2 * kTileQ;
+    const int q0 = qblk * kTiles * kTileQ;
 
     // key tiles each query tile may see: those below n_t[t]; in a windowed call the ones its `wt` names (n_t[t] is
     // the end of them) and, for the CTA, their union `both`
@@ -135,7 +141,7 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         const int row_lo = q0 + t * kTileQ;
-        if (row_lo >= p.Sq) {
+        if (row_lo >= p.Sq || t >= kTiles) {
             n_t[t] = 0;
         } else if (WINDOW) {
             const int row_hi = min(p.Sq, row_lo + kTileQ);
@@ -174,8 +180,8 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
         }
         mbar_fence_init();
     }
-    if (warp == 8) {
-        tmem_alloc(&sh.tmem_base, 512);
+    if (warp == kRoleWarp) {
+        tmem_alloc(&sh.tmem_base, kTmemCols);
         tmem_relinquish();
     }
     if (p.has_mask)
@@ -205,9 +211,11 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
 
     const bool dead = sh.abort_word != 0;  // set before the barrier above: skip straight to the tear-down
     if (dead) {
-    } else if (warp >= 8) {
-      reg_dealloc<88>();
-      if (warp == 9) {
+    } else if (warp >= kRoleWarp) {
+      // registers move to the softmax warpgroups: (2 x 208 + 88) x 128 of 168 x 384, or (200 + 56) x 128 of 128 x 256
+      if (kTiles == 2) reg_dealloc<88>();
+      else reg_dealloc<56>();
+      if (warp == kRoleWarp + 1) {
         // ------------------------------------------------------------ loader
         if (elect_one()) {
             tma_prefetch_desc(&maps.q);
@@ -215,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
             tma_prefetch_desc(&maps.v);
             const int active = (n_t[0] > 0 ? 1 : 0) + (n_t[1] > 0 ? 1 : 0);
             mbar_expect_tx(&sh.q_full, active * Cfg::kTileBytes);
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < kTiles; ++t)
                 if (n_t[t] > 0)
                     for (int c = 0; c < Cfg::kChunks; ++c)
                         tma_load_4d(sQ + t * Cfg::kTileBytes + c * (kTileQ * 128), &maps.q, &sh.q_full, c * 64,
@@ -236,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
                 }
             }
         }
-      } else if (warp == 8) {
+      } else if (warp == kRoleWarp) {
         // ------------------------------------------------------- MMA issuer
         if (elect_one()) {
             // a negative scale takes the maximum over -S: negate the A operand of the score product
@@ -262,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
                 const uint32_t b0 = slot * Cfg::kTileBytes;
 #pragma unroll
                 for (int kk = half * (kTileK / 32); kk < (half + 1) * (kTileK / 32); ++kk)
-                    umma_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, umma_desc_advance(v_desc, b0 + kk * 2048),
+                    umma_ts(tmem + kColO + t * 128, tmem + t * 128 + kk * 8, umma_desc_advance(v_desc, b0 + kk * 2048),
                             idesc_o, accumulate || kk > 0);
             };
             // The same in a windowed call: steps of 16 keys that no row of the tile sees are left out.
@@ -273,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
                 for (int kk = half * (kTileK / 32); kk < (half + 1) * (kTileK / 32); ++kk) {
                     const int key = j * kTileK + kk * 16;
                     if (key >= hi_t[t] || (key + 16 <= lo_t[t] && key >= p.sinks)) continue;
-                    umma_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, umma_desc_advance(v_desc, b0 + kk * 2048),
+                    umma_ts(tmem + kColO + t * 128, tmem + t * 128 + kk * 8, umma_desc_advance(v_desc, b0 + kk * 2048),
                             idesc_o, begun[t]);
                     begun[t] = true;
                 }
@@ -302,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
                 ok = mbar_wait(&sh.kv_full[slot], (slot_use / Cfg::kStages) & 1, abort_word, 21);
                 if (ok) {
                     tc_fence_after();
-                    for (int t = 0; t < 2; ++t)
+                    for (int t = 0; t < kTiles; ++t)
                         if (sees(t, j)) {
                             issue_s(t, slot);
                             umma_commit(&sh.s_ready[t]);
@@ -326,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
                 PH(0);
                 bool k_waited = false;
                 if (WINDOW && ok) clear_unseen(v_slot, j);
-                for (int t = 0; t < 2 && ok; ++t) {
+                for (int t = 0; t < kTiles && ok; ++t) {
                     const bool now = sees(t, j), then = sees(t, jn);
                     if (!now && !(WINDOW && then)) continue;
                     if (now) {
@@ -371,13 +379,14 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
         }
       }
     } else {
-        reg_alloc<208>();
+        if (kTiles == 2) reg_alloc<208>();
+        else reg_alloc<200>();
         // ---------------------------------------------------------- softmax
-        const int t = warp >> 2;
+        const int t = kTiles == 1 ? 0 : warp >> 2;
         const int row_in_tile = (warp & 3) * 32 + lane;
         const int row = q0 + t * kTileQ + row_in_tile;
         const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-        const uint32_t s_addr = lane_base + t * 128, o_addr = lane_base + 256 + t * 128;
+        const uint32_t s_addr = lane_base + t * 128, o_addr = lane_base + kColO + t * 128;
         const float c2 = fabsf(p.scale) * kLog2e;
         const uint64_t c2_pair = f2_pack(c2, c2);
         // this row's line of the mask (every row shares one line when the mask is broadcast over queries)
@@ -608,19 +617,20 @@ __global__ void __launch_bounds__(kThreads, 1) pipeline_forward(const __grid_con
         *p.status = 1000 + sh.abort_word;
         *reinterpret_cast<volatile int*>(p.abort_flag) = 1;  // the remaining CTAs of this and later launches skip their work
     }
-    if (warp == 8) tmem_dealloc(tmem, 512);
+    if (warp == kRoleWarp) tmem_dealloc(tmem, kTmemCols);
 }
 
 std::atomic<int> g_configured{0};
 
 template <int D, bool BF16>
 cudaError_t launch_t(const AttnParams& p, cudaStream_t st) {
-    using Cfg = FwdCfg<D>;
+    const int tiles = p.window > 0 ? 1 : 2;
+    const int smem_bytes = tiles == 1 ? FwdCfg<D, 1>::kSmemBytes : FwdCfg<D, 2>::kSmemBytes;
     // The shared-memory opt-in is per device; it is cheap, so it is simply repeated per call.
     auto kernel = p.window > 0 ? pipeline_forward<D, BF16, false, true>
                   : p.has_mask ? pipeline_forward<D, BF16, true, false>
                                : pipeline_forward<D, BF16, false, false>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
     if (e != cudaSuccess) return e;
     constexpr int variant = (D == 128 ? 0 : 2) + (BF16 ? 0 : 1);  // D = channels the kernel runs with (p.D rounded up)
     const int bit = 1 << variant;
@@ -634,8 +644,8 @@ cudaError_t launch_t(const AttnParams& p, cudaStream_t st) {
         maps.o = maps.q;  // not used: the running state is written with plain stores
     else if (!encode_bhsd_map(&maps.o, p.out, dt, p.D, p.Sq, p.Hq, p.B, p.os, 64, kTileQ))
         return cudaErrorInvalidValue;
-    const int64_t grid = (int64_t)((p.Sq + 2 * kTileQ - 1) / (2 * kTileQ)) * p.B * p.Hq;
-    kernel<<<(unsigned)grid, kThreads, Cfg::kSmemBytes, st>>>(maps, p);
+    const int64_t grid = (int64_t)((p.Sq + tiles * kTileQ - 1) / (tiles * kTileQ)) * p.B * p.Hq;
+    kernel<<<(unsigned)grid, threads_of(tiles), smem_bytes, st>>>(maps, p);
     return cudaGetLastError();
 }
 
