@@ -128,6 +128,8 @@ def quantized_cache_write(cache, k, v, *, start=0, lengths=None):
         raise ValueError(f"{name}: K and V must have the cache's device and type.")
     if (k.shape[0], k.shape[1], k.shape[3]) != (kc.shape[0], kc.shape[1], 2 * kc.shape[3]):
         raise ValueError(f"{name}: K and V must match the cache's batch, heads and channels.")
+    if any(stride == 0 and size > 1 for t in cache for size, stride in zip(t.shape, t.stride())):
+        raise ValueError(f"{name}: the cache's rows overlap in memory (an expanded view can only be read).")
     _no_gradient(name, k, v)
     starts, at = _positions(name, "start", start, kc.shape[0], kc.device)
     if starts is None and at + k.shape[2] > kc.shape[2]:

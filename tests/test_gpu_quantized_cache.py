@@ -118,6 +118,29 @@ def test_ragged_rows_leave_the_rest_as_it_was(dtype):
     assert torch.equal(cache.k_codes[:, :, :n].cpu(), quantise(k)[0])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_written_bits_over_the_range_of_the_type(dtype):
+    """Groups of every magnitude the type has, wide and narrow, with many quotients at or next to a half: the bits equal
+    IEEE FP32 arithmetic."""
+    gen = torch.Generator().manual_seed(77)
+    n, D = 4096, 256
+    low, high = (-14, 14) if dtype == torch.float16 else (-120, 120)
+    power = torch.randint(low, high, (1, 1, n, D // 64, 1), generator=gen).double()
+    x = torch.randn(1, 1, n, D // 64, 64, generator=gen).double() * torch.exp2(power)
+    steps = torch.randint(0, 31, (1, 1, n, D // 64, 64), generator=gen).double() * 0.5 * torch.exp2(power)  # multiples of a half
+    x = torch.where(torch.arange(n).view(1, 1, n, 1, 1) % 2 == 0, x, steps)
+    x = torch.where(torch.arange(n).view(1, 1, n, 1, 1) % 5 == 0, x * torch.exp2(-8.0 * torch.rand(x.shape, generator=gen)), x)
+    x = x.clamp(-torch.finfo(dtype).max, torch.finfo(dtype).max).to(dtype).flatten(-2).cuda()
+    cache = api().quantized_cache(1, 1, n, D, dtype=dtype)
+    api().quantized_cache_write(cache, x, x.flip(-1))
+    for half, codes, params in ((x, cache.k_codes, cache.k_params), (x.flip(-1), cache.v_codes, cache.v_params)):
+        want_codes, want_params = quantise(half)
+        finite = torch.isfinite(want_params[..., 0].float())
+        assert torch.equal(params.cpu()[..., 0][finite], want_params[..., 0][finite])
+        rows_codes = codes.cpu().unflatten(-1, (-1, 32))
+        assert torch.equal(rows_codes[finite], want_codes.unflatten(-1, (-1, 32))[finite])
+
+
 def test_values_that_are_not_finite():
     for dtype in TYPES:
         k = rows(1, 1, 4, 128, dtype=dtype, seed=1)
@@ -198,6 +221,9 @@ CASES = (
     (5, 1, 7, 513, 64, 1, 1, (506, 0)),
     (64, 8, 4, 1100, 128, 4096, 4, (1096, 512)),
     (2, 1, 40, 400, 128, 64, 16, (360, 17)),                  # a longer piece
+    (8, 2, 1, 300, 128, 0, 0, tuple(range(0, 280, 4))),       # seventy sequences
+    (12, 1, 1, 5000, 64, 700, 3, (4999, 2500)),               # twelve rows per cache head
+    (4, 1, 1, 40000, 128, 0, 0, (39999,)),                    # one long sequence over many CTAs
 )
 
 
@@ -321,6 +347,37 @@ def test_decoding_steps_follow_a_prompt():
         want, bound = reference(q[:, :, t:t + 1], cache, (t, t), window, sinks)
         assert bool(((got.cpu().double() - want).abs() <= bound).all())
     assert native().device_status(reset=True) == 0
+
+
+def test_offsets_past_32_bits():
+    """A cache whose planes are longer than 4 GiB: rows near the end are written, read and attended to in place."""
+    capacity, D = (1 << 26) + 4096, 128  # 64 bytes of codes per token and plane
+    codes = [torch.empty((1, 2, capacity, D // 2), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    params = [torch.empty((1, 2, capacity, D // 64, 2), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    cache = api().QuantizedCache(codes[0], params[0], codes[1], params[1])
+    n, start = 200, capacity - 203
+    k, v = rows(1, 2, n, D, dtype=torch.bfloat16, seed=51), rows(1, 2, n, D, dtype=torch.bfloat16, seed=52)
+    q = rows(1, 4, 1, D, dtype=torch.bfloat16, seed=53)
+    api().quantized_cache_write(cache, k, v, start=start)
+    small = api().quantized_cache(1, 2, n, D)
+    api().quantized_cache_write(small, k, v)
+    far, near = (api().quantized_cache_read(c, start=s, length=n) for c, s in ((cache, start), (small, 0)))
+    assert all(torch.equal(a, b) for a, b in zip(far, near))
+    got = api().quantized_cache_attention(q, cache, query_start=start + n - 1, window=n)
+    want, bound = reference(q, small, (n - 1,), n, 0)
+    assert bool(((got.cpu().double() - want).abs() <= bound).all())
+
+
+def test_a_cache_that_overlaps_itself_is_read_but_not_written():
+    cache = filled(1, 2, 64, 64, torch.bfloat16, 61)
+    shared = api().QuantizedCache(*(t.expand(3, *t.shape[1:]) for t in cache))  # one prefix for three sequences
+    q = rows(3, 4, 1, 64, dtype=torch.bfloat16, seed=62)
+    got = api().quantized_cache_attention(q, shared, query_start=63)
+    for b in range(3):
+        assert torch.equal(got[b:b + 1], api().quantized_cache_attention(q[b:b + 1], cache, query_start=63))
+    k = rows(3, 2, 1, 64, dtype=torch.bfloat16, seed=63)
+    with pytest.raises(ValueError, match="overlap"):
+        api().quantized_cache_write(shared, k, k)
 
 
 def test_compiled_route():

@@ -174,6 +174,9 @@ def test_the_gradient_matches_differences():
     (8, 1, 3, 1000, 128, 64, 130, (2**31 - 1, 996, 129, -(2**31))),
     (6, 2, 257, 400, 80, 90, 1, (143, 20, 390, 600)),
     (4, 2, 40, 200, 256, 30, 2, (100, 160, 0, 7)),
+    (8, 1, 2, 3000, 128, 700, 20, (2998, 1500, 3, 719)),      # sixteen rows per K/V head
+    (12, 4, 4, 2000, 64, 5000, 0, (1996, 0, 1000, -2)),       # twelve
+    (4, 2, 1, 300, 128, 100, 4, tuple(range(0, 280, 4))),     # seventy sequences
 ))
 @pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
 def test_positions_per_sequence(case, dtype):
@@ -203,6 +206,23 @@ def test_positions_per_sequence(case, dtype):
     if starts[0] >= 0 and starts[0] < 2**31 - 1:  # the int form is the same call
         one = api().sliding_window_attention(q[:1], k[:1], v[:1], window=window, sinks=sinks, query_start=starts[0])
         torch.testing.assert_close(one, got[:1], atol=TOL[dtype]["elem"], rtol=TOL[dtype]["elem"])
+    assert native().device_status(reset=True) == 0
+
+
+def test_one_new_token_against_a_long_cache():
+    """Many CTAs per sequence; the cache is a view of a larger one, [B, S, H, D] in memory."""
+    B, Hq, Hkv, Sk, D = 2, 8, 2, 30000, 128
+    q, k, v, dout = make_inputs(B, Hq, Hkv, 1, Sk, D, torch.bfloat16, seed=15)
+    held = [torch.full((B, Sk + 100, Hkv, D), float("nan"), device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+    for t, x in zip(held, (k, v)):
+        t[:, :Sk] = x.transpose(1, 2)
+    views = [t[:, 7:Sk].transpose(1, 2) for t in held]
+    for window, sinks in ((20000, 4), (1 << 20, 0), (5, 17)):
+        with torch.no_grad():
+            got = api().sliding_window_attention(q, *views, window=window, sinks=sinks, query_start=Sk - 8)
+        mask = window_mask([Sk - 8] * B, 1, Sk - 7, window, sinks)
+        want = ao.math_reference([t.cpu() for t in (q, *views)], dout.cpu(), mask, False, None)[0]
+        assert ao.per_head_relative_error(got.cpu(), want) < TOL[torch.bfloat16]["norm"]
     assert native().device_status(reset=True) == 0
 
 
