@@ -8,7 +8,8 @@
 //   P      = ex2(s~ * c)          c = |scale| * log2(e)
 //   P_low  = round(P)             one rounding to the input type
 //   dS_low = round(P_low * dP~)
-// (windowed calls form dS_low from the unrounded P, one rounding less).  Hidden entries get P = 0.  The work of a unit runs in two phases so that the tensor core never waits
+// (windowed calls form dS from the unrounded P and hand it over as two 16-bit pieces, the rounded value and what the
+// rounding left, so that dK carries no rounding but its own).  Hidden entries get P = 0.  The work of a unit runs in two phases so that the tensor core never waits
 // for all of it: P_low needs only the score tile and goes back at once (dV and the next score tile run
 // under the second phase), dS_low needs the dP tile and the P_low values kept in registers.
 #pragma once
@@ -139,7 +140,7 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
         if (!ok) break;
         PH(6);
         tc_fence_after();
-        uint32_t dw[kCols / 2];
+        uint32_t dw[kCols / 2], rest_w[kCols / 2];  // windowed calls: what the rounding of dS left
         {
             uint32_t dp[kCols];
             tmem_ld32(dp_addr, *reinterpret_cast<uint32_t(*)[32]>(&dp[0]));
@@ -154,10 +155,17 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
                 f2_unpack(f2_mul(f2_pack(pl.x, pl.y), f2_pack(__uint_as_float(dp[c]), __uint_as_float(dp[c + 1]))),
                           da, db);
                 dw[c / 2] = pack2<BF16>(da, db);
+                if (W::kWindow) {
+                    const float2 low = unpack2<BF16>(dw[c / 2]);
+                    float ra, rb;
+                    f2_unpack(f2_sub(f2_pack(da, db), f2_pack(low.x, low.y)), ra, rb);
+                    rest_w[c / 2] = pack2<BF16>(ra, rb);
+                }
             }
         }
         PH(7);
         tmem_st(dp_addr, dw);
+        if (W::kWindow) tmem_st(dp_addr + kCols / 2, rest_w);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&sh.ds_done);

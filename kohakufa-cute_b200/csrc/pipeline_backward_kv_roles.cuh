@@ -165,6 +165,13 @@ __device__ __forceinline__ void mma_role(const AttnParams& p, const W& w, Shared
             umma_ts(d_col, a_col + a_off, umma_desc_advance(ring_mn_desc, st + kk * 2048), idesc_g,
                     accumulate || kk > 0);
         }
+        if (W::kWindow && which == 1) {  // the second pieces of dS
+#pragma unroll
+            for (int kk = 0; kk < kTile / 16; ++kk) {
+                const uint32_t a_off = (kk / 4) * kCols + kCols / 2 + (kk % 4) * 8;
+                umma_ts(d_col, a_col + a_off, umma_desc_advance(ring_mn_desc, st + kk * 2048), idesc_g, 1);
+            }
+        }
     };
 
     bool ok = mbar_wait(&sh.owner_full, 0, abort_word, 120);

@@ -9,8 +9,9 @@
 // P_low of a unit is formed as soon as its score tile is there (the tensor core is still busy with
 // the previous unit's dQ and this unit's dP); the dP values are then pulled into registers, the dP
 // buffer is handed back, and dS_low is packed over the thread's own (dead) score columns.
-// Windowed calls have no reference to round like: they form dS_low = round(P * (dP - delta)) from the unrounded P (one
-// rounding less) and take the row sum of dS_low times a mean key off dQ (see mean_role).
+// Windowed calls have no reference to round like: they form dS from the unrounded P, hand it over as two 16-bit pieces
+// (the rounded value and what the rounding left, 32 packed columns each), so that dQ carries no rounding but its own,
+// and take the row sum of dS times a mean key off dQ (see mean_role).
 #pragma once
 #include "pipeline_backward_q_roles.cuh"
 
@@ -51,7 +52,7 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
     w.begin(p, g, i);
     int unit = 0;
     bool ok = true;
-    uint64_t row_sum = f2_pack(0.f, 0.f);  // windowed calls: sum of this thread's dS_low (see mean_role)
+    uint64_t row_sum = f2_pack(0.f, 0.f);  // windowed calls: sum of this thread's dS (see mean_role)
     PH_DECL;
     while (w.valid(g) && ok) {
         PH(5);
@@ -144,7 +145,7 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
         if (!ok) break;
         PH(6);
         tc_fence_after();
-        uint32_t dw[kCols / 2];
+        uint32_t dw[kCols / 2], rest_w[kCols / 2];  // windowed calls: what the rounding of dS left
         {
             uint32_t dp[kCols];
             tmem_ld32(dp_addr, *reinterpret_cast<uint32_t(*)[32]>(&dp[0]));
@@ -165,12 +166,17 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
                 dw[c / 2] = pack2<BF16>(da, db);
                 if (W::kWindow) {
                     const float2 low = unpack2<BF16>(dw[c / 2]);
-                    row_sum = f2_add(row_sum, f2_pack(low.x, low.y));
+                    const uint64_t pair = f2_pack(da, db);
+                    row_sum = f2_add(row_sum, pair);
+                    float ra, rb;
+                    f2_unpack(f2_sub(pair, f2_pack(low.x, low.y)), ra, rb);
+                    rest_w[c / 2] = pack2<BF16>(ra, rb);
                 }
             }
         }
         PH(7);
         tmem_st(s_addr, dw);
+        if (W::kWindow) tmem_st(s_addr + kCols / 2, rest_w);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&sh.ds_done);
@@ -228,7 +234,7 @@ __device__ __forceinline__ void consumer_role(const Maps& maps, const AttnParams
     // end are not written by the store.
     const uint32_t acc = lane_base + kColGrad + ch0;
     const float mul = p.scale;
-    float rest = 0.f;  // windowed calls: minus the row sum of dS_low
+    float rest = 0.f;  // windowed calls: minus the row sum of dS
     if (W::kWindow) {
         float* sums = reinterpret_cast<float*>(s_owner + Cfg<D>::kTileBytes);  // the dO tile is dead
         float x0, x1;

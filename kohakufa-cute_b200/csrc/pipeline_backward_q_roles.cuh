@@ -52,10 +52,10 @@ struct Shared {
 constexpr uint32_t kColS = 0, kColDp = 256, kColGrad = 384;
 
 // Windowed calls: the mean of 32 keys spread evenly over those the tile's rows see, by an otherwise idle warp while the
-// pipeline fills.  The exact dS of a row sums to zero, so dQ = sum dS K = sum dS (K - c) for any c; the rounded dS sums
-// to some R instead, and the epilogue takes R c off again.  Without that a per-channel offset of the keys multiplies
-// every rounding of dS (and the rounding of O inside delta): with offsets of 1.2 standard deviations the BF16 dQ was
-// 5.8e-3 from 64 bits.
+// pipeline fills.  The exact dS of a row sums to zero, so dQ = sum dS K = sum dS (K - c) for any c; with the stored O's
+// rounding in delta it sums to some R instead, and the epilogue takes R c off again.  Without that a per-channel offset
+// of the keys multiplies that error: with offsets of 1.2 standard deviations (and a rounded dS) the BF16 dQ was 5.8e-3
+// from 64 bits, with it 2.6e-3, and with dS in two pieces 1.9e-3, of which the rounding of dQ itself is 1.7e-3.
 template <int D, class T, class W>
 __device__ __forceinline__ void mean_role(const AttnParams& p, const W& w, Shared& sh, int lane) {
     int g, i;
@@ -167,6 +167,13 @@ __device__ __forceinline__ void mma_role(const AttnParams& p, const W& w, Shared
             const uint32_t a_off = (kk / 4) * kCols + (kk % 4) * 8;
             umma_ts(tmem + kColGrad, a_col + a_off, umma_desc_advance(grad_desc, st + kk * 2048), idesc_g,
                     accumulate || kk > 0);
+        }
+        if (W::kWindow) {  // the second pieces of dS
+#pragma unroll
+            for (int kk = 0; kk < kTile / 16; ++kk) {
+                const uint32_t a_off = (kk / 4) * kCols + kCols / 2 + (kk % 4) * 8;
+                umma_ts(tmem + kColGrad, a_col + a_off, umma_desc_advance(grad_desc, st + kk * 2048), idesc_g, 1);
+            }
         }
     };
 
