@@ -12,6 +12,7 @@ import hashlib
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -78,7 +79,31 @@ def build(force=False, verbose=True, phases=False):
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.check_call(cmd)
+    if not phases:
+        build_records(force, verbose)
     return lib
+
+
+def build_records(force=False, verbose=True):
+    """The optional CPython module that packs tensor records (``csrc/fast_records.c``), or ``None`` without Python's
+    headers: the binding then packs them itself, with the same results."""
+    include = sysconfig.get_paths()["include"]
+    source = os.path.join(CSRC, "fast_records.c")
+    header = os.path.join(os.path.dirname(HERE), "include", "kfa.h")
+    target = os.path.join(OUT_DIR, "_fast_records" + sysconfig.get_config_var("EXT_SUFFIX"))
+    if not os.path.exists(os.path.join(include, "Python.h")):
+        return None
+    cmd = [os.environ.get("CC", "gcc"), "-O2", "-std=c11", "-Wall", "-Wextra", "-shared", "-fPIC", "-I", include, source]
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    stamp = os.path.join(OBJ_DIR, "fast_records.sha")
+    digest = _digest([source, header], cmd)
+    if force or not os.path.exists(target) or not os.path.exists(stamp) or open(stamp).read() != digest:
+        if verbose:
+            print(" ".join(cmd + ["-o", target]), flush=True)
+        subprocess.check_call(cmd + ["-o", target])
+        with open(stamp, "w") as f:
+            f.write(digest)
+    return target
 
 
 if __name__ == "__main__":

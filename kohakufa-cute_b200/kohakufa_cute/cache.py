@@ -41,18 +41,19 @@ def quantized_cache(batch, heads, capacity, head_dim, *, dtype=torch.bfloat16, d
 
 def _check_cache(name, cache):
     """Raises ``ValueError`` unless ``cache`` is a quantised cache this library can address."""
-    if not isinstance(cache, tuple) or len(cache) != 4 or not all(isinstance(t, torch.Tensor) for t in cache):
+    if not isinstance(cache, tuple) or len(cache) != 4 or any(not isinstance(t, torch.Tensor) for t in cache):
         raise ValueError(f"{name}: cache must be a QuantizedCache.")
     kc, kp, vc, vp = cache
-    if kc.dtype != torch.uint8 or kc.ndim != 4 or 0 in kc.shape or kc.shape[3] % 32 or kc.shape[3] > 256:
+    shape, pair, device = kc.shape, kp.shape, kc.device
+    if kc.dtype != torch.uint8 or len(shape) != 4 or 0 in shape or shape[3] % 32 or shape[3] > 256:
         raise ValueError(f"{name}: cache codes must be uint8 [B, H, capacity, D / 2], D a multiple of 64 up to 512.")
-    if kp.dtype not in _HALF_TYPES or kp.shape != (*kc.shape[:3], kc.shape[3] // 32, 2):
+    if kp.dtype not in _HALF_TYPES or pair != (*shape[:3], shape[3] // 32, 2):
         raise ValueError(f"{name}: cache params must be FP16/BF16 [B, H, capacity, D / 64, 2].")
-    if vc.dtype != kc.dtype or vc.shape != kc.shape or vp.dtype != kp.dtype or vp.shape != kp.shape:
+    if vc.dtype != kc.dtype or vc.shape != shape or vp.dtype != kp.dtype or vp.shape != pair:
         raise ValueError(f"{name}: the cache's key and value tensors must match.")
-    if kc.device.type != "cuda" or any(t.device != kc.device for t in (kp, vc, vp)):
+    if device.type != "cuda" or kp.device != device or vc.device != device or vp.device != device:
         raise ValueError(f"{name}: the cache must live on one CUDA device.")
-    if not _device_supported(kc.device):
+    if not _device_supported(device):
         raise ValueError("This build of CuTe attention requires an sm_100 (B200) device.")
 
 
@@ -128,7 +129,7 @@ def quantized_cache_write(cache, k, v, *, start=0, lengths=None):
         raise ValueError(f"{name}: K and V must have the cache's device and type.")
     if (k.shape[0], k.shape[1], k.shape[3]) != (kc.shape[0], kc.shape[1], 2 * kc.shape[3]):
         raise ValueError(f"{name}: K and V must match the cache's batch, heads and channels.")
-    if any(stride == 0 and size > 1 for t in cache for size, stride in zip(t.shape, t.stride())):
+    if any(0 in t.stride() and not t.is_contiguous() for t in cache):
         raise ValueError(f"{name}: the cache's rows overlap in memory (an expanded view can only be read).")
     _no_gradient(name, k, v)
     starts, at = _positions(name, "start", start, kc.shape[0], kc.device)

@@ -17,6 +17,11 @@ import threading
 
 import torch
 
+try:  # optional: packs tensor records in C (build.py leaves it out where Python's headers are missing)
+    from . import _fast_records
+except ImportError:
+    _fast_records = None
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIBRARY_PATH = os.path.join(_HERE, "libkfa.so")
 
@@ -147,7 +152,7 @@ _RECORDS = [struct.Struct(f"<Qii{n}q{8 * (6 - n)}x{n}q{8 * (6 - n)}x") for n in 
 _RECORD_BYTES = ctypes.sizeof(KfaTensor)
 
 
-def _records(*tensors):
+def _packed_records(*tensors):
     """``(buffer, addresses)``: the records of ``describe`` side by side in one buffer, for the entry points whose host
     time matters (a decoding step launches for a few microseconds); the buffer has to outlive the call."""
     buffer = bytearray(_RECORD_BYTES * len(tensors))
@@ -158,10 +163,17 @@ def _records(*tensors):
             addresses.append(None)
         else:
             n = t.dim()
-            _RECORDS[n].pack_into(buffer, offset, t.data_ptr(), _DTYPES[t.dtype], n, *t.shape, *t.stride())
+            _RECORDS[n].pack_into(buffer, offset, t.data_ptr(), _DTYPES.get(t.dtype, -1), n, *t.shape, *t.stride())
             addresses.append(base + offset)
         offset += _RECORD_BYTES
     return buffer, addresses
+
+
+if _fast_records is not None:
+    _fast_records.set_dtypes(tuple(_DTYPES))  # in the order of their codes
+    _records = _fast_records.records
+else:
+    _records = _packed_records
 
 
 _NO_CONTEXT = contextlib.nullcontext()
@@ -214,6 +226,14 @@ def _rows_16_byte_addressable(t):
     return True
 
 
+def _all_rows_16_byte_addressable(*tensors):
+    return all(_rows_16_byte_addressable(t) for t in tensors)
+
+
+if _fast_records is not None:
+    _all_rows_16_byte_addressable = _fast_records.addressable
+
+
 def _blocks_shape(q, k, mask):
     return (
         1 if mask.stride(0) == 0 else q.shape[0],
@@ -239,7 +259,7 @@ def _for_tensor_cores(tensors):
     whose rows are not 16-byte addressable.  Returns the tensors unchanged when nothing has to be done."""
     D = tensors[0].shape[-1]
     target = tensor_core_head_dim(D)
-    if target == D and all(_rows_16_byte_addressable(t) for t in tensors):
+    if target == D and _all_rows_16_byte_addressable(*tensors):
         return tensors, D
     if target != D:
         return [torch.nn.functional.pad(t, (0, target - D)) for t in tensors], D
@@ -526,7 +546,9 @@ def window_backward(q, k, v, out, maximum, logsum, dout, start, window, sinks, s
 def cache_write(k, v, k_codes, k_params, v_codes, v_params, starts, lengths, start):
     """Quantises the rows of ``k`` and ``v`` into a 4-bit cache in place (``kfa_cache_write``)."""
     lib = library()
-    k, v = (t if _rows_16_byte_addressable(t) else t.contiguous() for t in (_plain(k), _plain(v)))
+    k, v = _plain(k), _plain(v)
+    if not _all_rows_16_byte_addressable(k, v):
+        k, v = (t if _rows_16_byte_addressable(t) else t.contiguous() for t in (k, v))
     device = k.device
     with _on(device):
         keep, records = _records(k, v, k_codes, k_params, v_codes, v_params, starts, lengths)
@@ -550,7 +572,7 @@ def cache_attention(q, k_codes, k_params, v_codes, v_params, starts, start, wind
     """Attention of a few query rows to a 4-bit cache (``kfa_cache_attention``); ``window`` 0 means none."""
     lib = library()
     q = _plain(q)
-    if not _rows_16_byte_addressable(q):
+    if not _all_rows_16_byte_addressable(q):
         q = q.contiguous()
     device = q.device
     with _on(device):
