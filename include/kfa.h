@@ -241,7 +241,7 @@ KFA_API int kfa_merge_splits(kfa_tensor* out, kfa_tensor* maximum, kfa_tensor* l
  *
  * kfa_window_backward takes the forward's out/maximum/logsum and one `start` >= 0 for all batches; `workspace` holds
  * kfa_window_backward_workspace_bytes() bytes, 256-byte aligned.  Every gradient has one owner and a fixed order of
- * additions.
+ * additions.  All of k and v must hold finite numbers here (pass views that end with the last row's position).
  */
 KFA_API size_t kfa_window_forward_workspace_bytes(const kfa_tensor* q, const kfa_tensor* k, int64_t window,
                        int64_t sinks, int statistics);

@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kWarps * 32) general_forward(AttnParams p) {
     const int kend = windowed ? window_span(start, last_row, p.window, p.Sk).hi
                               : (p.causal ? min(p.Sk, last_row + 1) : p.Sk);
     for (int k0 = 0; k0 < kend; k0 += 32) {
-        if (windowed && k0 >= p.sinks && k0 + 32 <= first_lo) continue;  // between the sinks and the window
+        if (windowed && k0 >= p.sinks && k0 + 32 <= first_lo) k0 = first_lo & ~31;  // from the sinks to the window
         if (p.has_mask && (k0 & 63) == 0) {
             // skip a 64-key block that the tile table marks hidden for every row of this warp
             int tq0 = row0 >> 6, tq1 = last_row >> 6;
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kWarps * 32) general_backward_q(AttnParams p) 
     const int kend = windowed ? window_span(start, last_row, p.window, p.Sk).hi
                               : (p.causal ? min(p.Sk, last_row + 1) : p.Sk);
     for (int k0 = 0; k0 < kend; k0 += 32) {
-        if (windowed && k0 >= p.sinks && k0 + 32 <= first_lo) continue;  // between the sinks and the window
+        if (windowed && k0 >= p.sinks && k0 + 32 <= first_lo) k0 = first_lo & ~31;  // from the sinks to the window
         if (p.has_mask && (k0 & 63) == 0) {
             int tq0 = row0 >> 6, tq1 = last_row >> 6;
             bool any = tile_state(p, b, h, tq0, k0 >> 6) != 0 || tile_state(p, b, h, tq1, k0 >> 6) != 0;

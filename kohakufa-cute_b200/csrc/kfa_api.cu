@@ -1075,6 +1075,8 @@ int fill_window(kfa::AttnParams& p, const kfa_tensor* starts, int64_t start, int
     if (starts && (!starts->data || starts->dtype != KFA_I32 || starts->ndim != 1 || starts->sizes[0] != p.B ||
                    (p.B > 1 && starts->strides[0] != 1)))
         return fail(KFA_INVALID_ARGUMENT, "window attention requires contiguous int32 [batch] query positions");
+    if (p.Sk > INT32_MAX - 256 || p.Sq > INT32_MAX - 256)
+        return fail(KFA_TOO_LARGE, "window attention: sequences are limited to 2^31 - 257 tokens");
     if (!starts && (start > INT32_MAX || start < INT32_MIN))
         return fail(KFA_INVALID_ARGUMENT, "window attention: the query position exceeds 32 bits");
     // positions stay below 2^32 + 2^31: a longer window is the same as none
@@ -1119,7 +1121,7 @@ size_t kfa_window_forward_workspace_bytes(const kfa_tensor* q, const kfa_tensor*
                                           int statistics) {
     if (!q || !k || statistics || q->ndim != 4 || k->ndim != 4 || window < 1 || sinks < 0) return 0;
     for (int i = 0; i < 4; ++i)
-        if (q->sizes[i] <= 0 || k->sizes[i] <= 0 || q->sizes[i] > INT32_MAX || k->sizes[i] > INT32_MAX) return 0;
+        if (q->sizes[i] <= 0 || k->sizes[i] <= 0 || q->sizes[i] > INT32_MAX - 256 || k->sizes[i] > INT32_MAX - 256) return 0;
     if (q->sizes[1] % k->sizes[1] != 0) return 0;
     kfa::AttnParams p;
     std::memset(&p, 0, sizeof(p));
@@ -1253,7 +1255,7 @@ int fill_cache_half(kfa::CacheView& view, const kfa_tensor* codes, const kfa_ten
                     "FP16/BF16 model type");
     const int64_t bytes = codes->sizes[3], groups = bytes / 32;
     for (int i = 0; i < 4; ++i)
-        if (codes->sizes[i] <= 0 || codes->sizes[i] > INT32_MAX || codes->sizes[i] != like->sizes[i])
+        if (codes->sizes[i] <= 0 || codes->sizes[i] > INT32_MAX - 256 || codes->sizes[i] != like->sizes[i])
             return fail(KFA_INVALID_ARGUMENT, "quantized cache: K and V codes must be nonempty and of one shape");
     if (bytes % 32 != 0 || groups > 8)
         return fail(KFA_INVALID_ARGUMENT, "quantized cache requires head dimensions that are multiples of 64 up to 512");
@@ -1329,8 +1331,8 @@ int fill_cache_attention(kfa::CacheAttentionCall& p, const kfa_tensor* q, const 
     if (!q || !codes || q->ndim != 4 || codes->ndim != 4 || !is_half_type(q))
         return fail(KFA_INVALID_ARGUMENT, "cache attention requires 4D FP16/BF16 queries and a quantized cache");
     for (int i = 0; i < 4; ++i)
-        if (q->sizes[i] <= 0 || q->sizes[i] > INT32_MAX || codes->sizes[i] <= 0 || codes->sizes[i] > INT32_MAX)
-            return fail(KFA_INVALID_ARGUMENT, "cache attention requires nonempty operands");
+        if (q->sizes[i] <= 0 || q->sizes[i] > INT32_MAX - 256 || codes->sizes[i] <= 0 || codes->sizes[i] > INT32_MAX - 256)
+            return fail(KFA_INVALID_ARGUMENT, "cache attention requires nonempty operands of at most 2^31 - 257 tokens");
     if (q->sizes[0] != codes->sizes[0] || q->sizes[1] % codes->sizes[1] != 0 || q->sizes[3] != 2 * codes->sizes[3])
         return fail(KFA_INVALID_ARGUMENT,
                     "cache attention requires matching batch and channels, and query heads divisible by K/V heads");
