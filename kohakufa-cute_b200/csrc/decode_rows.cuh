@@ -21,7 +21,8 @@
 // Work is cut evenly however ragged the batch is: the blocks of tokens that the units (sequence, K/V head, chunk of
 // query rows) have to read are numbered through, and each CTA takes an equal piece of that line; where a unit spans
 // several CTAs their partial (maximum, sum, accumulator) are merged by a second, dependent launch.  The lengths come
-// from device memory, so a captured call follows new positions.  Within a CTA the warps take blocks in turn, each with
+// from device memory, so a captured call follows new positions.  Short calls (few units of few blocks) skip the second
+// launch: a cluster of eight CTAs owns a unit and merges over distributed shared memory.  Within a CTA the warps take blocks in turn, each with
 // its own ring of asynchronous copies.  (A piece per warp, without the merge within the CTA, was no faster: 114 against
 // 113 us at 16 x 32768 tokens, 44 against 42 at 16 x 8192, and slower for one sequence.)
 //
@@ -47,6 +48,7 @@ struct RowsCall {
     int64_t kvs[2][3];    // batch, head, token strides (elements)
     int rows, chunks;     // query rows per K/V head, pieces of 8 * NT of them
     int ctas;
+    int cluster;          // != 0: short calls, a thread-block cluster of kCluster CTAs per unit and no second launch
     uint32_t lowest, others;  // see Bases
     float* part_o;        // [ctas][2][8 NT][D]: a CTA's first and last piece of a unit
     float* part_ml;       // [ctas][2][8 NT][2]: maximum, sum
@@ -55,6 +57,7 @@ struct RowsCall {
 namespace rows {
 
 constexpr int kWarps = 4;
+constexpr int kCluster = 8;
 
 // CTAs per SM that registers and shared memory allow (the launch bounds hold the compiler to it).
 template <int D, bool Q4, int NT>
@@ -203,6 +206,30 @@ __device__ __forceinline__ void copy_bulk(uint32_t dst, const void* src, uint32_
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                  "l"(src), "r"(bytes), "r"(smem_u32(bar))
                  : "memory");
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// Address of the same shared-memory location in CTA `rank` of the cluster, and loads from there.
+__device__ __forceinline__ uint32_t cluster_address(const void* p, uint32_t rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float4 cluster_load4(uint32_t a) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 cluster_load2(uint32_t a) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+    return v;
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -495,15 +522,25 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may be scheduled; it waits for this grid
     const uint32_t units = c.Hkv * p.chunks;
+    // This CTA's piece of the line; in a cluster its share of one unit, counted from that unit's first block.
     const Line line(c, units, C::kBlock);
-    const Cut cut(line.before(c.B), p.ctas);
-    if (blockIdx.x >= cut.ctas) return;
-    const uint32_t begin = cut.begin(blockIdx.x), end = cut.begin(blockIdx.x + 1);
+    const uint32_t my_unit = blockIdx.x / kCluster, my_rank = p.cluster ? cluster_rank() : 0;
+    uint32_t begin, end;
+    if (p.cluster) {
+        const uint32_t n = blocks_of(c, start_of(c, (int)(my_unit / units)), C::kBlock).count;
+        begin = n * my_rank / kCluster;
+        end = n * (my_rank + 1) / kCluster;
+    } else {
+        const Cut cut(line.before(c.B), p.ctas);
+        if (blockIdx.x >= cut.ctas) return;
+        begin = cut.begin(blockIdx.x);
+        end = cut.begin(blockIdx.x + 1);
+    }
     uint8_t* my_ring = ring + warp * C::kStages * C::kStage;
     const float c2 = fabsf(c.scale) * kLog2e;
     const Bases bases{p.lowest, p.others};
     State<D, Q4, NT> st;
-    // Dense rows of codes come as two contiguous copies per block (32 rows of keys, 32 of values), which cost one thread
+    // Dense rows of codes come as two contiguous copies per block (one of keys, one of values), which cost one thread
     // a few instructions instead of eight address computations per lane.
     const bool packed = Q4 && c.half[0].ps[2] == 2 * C::kGroups && c.half[1].ps[2] == 2 * C::kGroups;
     const bool dense = Q4 && c.half[0].cs[2] == C::kRow && c.half[1].cs[2] == C::kRow;
@@ -516,14 +553,21 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
     }
     __syncthreads();
     bool ok = abort_word == 0;
-    if (!ok) return;
+    if (!ok) {
+        if (!p.cluster) return;
+        end = begin;  // (a cluster's CTAs stay to its barriers: the others read this one's part)
+    }
+    float* sm_o = reinterpret_cast<float*>(ring);              // [warp][R][D], where the ring is idle
+    float* cta_o = sm_o + kWarps * R * D;                       // a cluster's CTA: its part, [R][D]
+    float2* cta_ml = reinterpret_cast<float2*>(cta_o + R * D);  // and its (maximum, sum), [R]
 
     for (uint32_t at = begin; at < end;) {
-        uint32_t base;
-        const int b = line.sequence_at(at, base);
+        uint32_t base = 0;
+        const int b = p.cluster ? (int)(my_unit / units) : line.sequence_at(at, base);
         const int64_t start = start_of(c, b);
         const Blocks blocks = blocks_of(c, start, C::kBlock);
-        const int unit = (int)((at - base) / (uint32_t)blocks.count), from = (int)(at - base) - unit * blocks.count;
+        const int unit = p.cluster ? (int)(my_unit % units) : (int)((at - base) / (uint32_t)blocks.count);
+        const int from = p.cluster ? (int)at : (int)(at - base) - unit * blocks.count;
         const int count = min((int)(end - at), blocks.count - from);
         const int kvh = unit / p.chunks, row0 = unit % p.chunks * R;
         const WindowSpan low = window_span(start, 0, c.window, c.Sk), high = window_span(start, c.Sq - 1, c.window, c.Sk);
@@ -679,7 +723,6 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
 
         // the warps of the CTA, merged in a fixed order through the (now idle) ring
         __syncthreads();
-        float* sm_o = reinterpret_cast<float*>(ring);  // [warp][R][D]
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -728,7 +771,10 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
                 acc.x = fmaf(x.x, weight, acc.x), acc.y = fmaf(x.y, weight, acc.y);
                 acc.z = fmaf(x.z, weight, acc.z), acc.w = fmaf(x.w, weight, acc.w);
             }
-            if (whole) {
+            if (p.cluster) {
+                *reinterpret_cast<float4*>(cta_o + r * D + d) = acc;
+                if (d == 0) cta_ml[r] = make_float2(mx, sum);
+            } else if (whole) {
                 const int row = row0 + r;
                 if (row < p.rows) {
                     const float inv = sum > 0.f ? 1.f / sum : 0.f;
@@ -746,6 +792,39 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
         __syncthreads();
         at += count;
         if (abort_word != 0) break;
+    }
+    if (p.cluster) {
+        if (begin == end) {  // no block for this CTA
+            for (int r = threadIdx.x; r < R; r += kWarps * 32) cta_ml[r] = make_float2(-INFINITY, 0.f);
+            for (int x = threadIdx.x; x < R * D / 4; x += kWarps * 32) reinterpret_cast<float4*>(cta_o)[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        cluster_barrier();
+        const int b = (int)(my_unit / units), unit = (int)(my_unit % units), kvh = unit / p.chunks, row0 = unit % p.chunks * R;
+        for (int idx = threadIdx.x * kCluster + my_rank; idx < R * (D / 4); idx += kWarps * 32 * kCluster) {
+            const int r = idx / (D / 4), d = idx % (D / 4) * 4, row = row0 + r;
+            if (row >= p.rows) break;
+            float2 ml[kCluster];
+            float4 x[kCluster];
+            float mx = -INFINITY, sum = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kCluster; ++w) {
+                ml[w] = cluster_load2(cluster_address(cta_ml + r, w));
+                x[w] = cluster_load4(cluster_address(cta_o + r * D + d, w));
+                mx = fmaxf(mx, ml[w].x);
+            }
+#pragma unroll
+            for (int w = 0; w < kCluster; ++w) {
+                const float weight = ml[w].x == -INFINITY ? 0.f : ex2((ml[w].x - mx) * c2);
+                sum += ml[w].y * weight;
+                acc.x = fmaf(x[w].x, weight, acc.x), acc.y = fmaf(x[w].y, weight, acc.y);
+                acc.z = fmaf(x[w].z, weight, acc.z), acc.w = fmaf(x[w].w, weight, acc.w);
+            }
+            const float inv = sum > 0.f ? 1.f / sum : 0.f;
+            T* out = static_cast<T*>(c.out) + b * c.os[0] + (kvh * c.group + row / c.Sq) * c.os[1] + row % c.Sq * c.os[2] + d;
+            *reinterpret_cast<uint2*>(out) = make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
+        }
+        cluster_barrier();  // nobody leaves while its part is read
     }
     if (threadIdx.x == 0 && abort_word != 0) {
         *c.status = 5000 + abort_word;
@@ -853,9 +932,21 @@ int plan_ctas(const CacheAttentionCall& c, int chunks) {
     return (int)(want < 1 ? 1 : (want > most ? most : want));
 }
 
+// Whether clusters serve the call: no more of their CTAs than are resident at once, and at most three blocks per warp.
+// B1 Hq32 Hkv8 D128, GPU time of a step in a graph, two launches -> one cluster launch: window of 1024 10.9 -> 7.6 us,
+// 256 9.3 -> 5.9; 4-bit cache of 1024 tokens 8.5 -> 7.7, 4096 9.9 -> 9.7, 8192 (four blocks per warp) 12.3 -> 13.0; B6
+// at 4096 tokens 19.1 -> 14.6; B6 with a window of 512 11.2 -> 11.7.  Outside graphs a call saves 2.5 us of host time.
+template <int D, bool Q4, int NT>
+bool clustered(const CacheAttentionCall& c, int chunks) {
+    return (int64_t)c.B * c.Hkv * chunks * kCluster <= 148 * resident<D, Q4, NT>() &&
+           most_blocks<D, Q4, NT>(c) <= 3 * kWarps * kCluster;
+}
+
 template <int D, bool Q4>
 size_t workspace_bytes(const CacheAttentionCall& c) {
     const int NT = row_tiles(c), R = 8 * NT, chunks = (c.group * c.Sq + R - 1) / R;
+    // (a call that clusters serve keeps nothing; 16 bytes keep the size positive)
+    if (NT == 1 ? clustered<D, Q4, 1>(c, chunks) : clustered<D, Q4, 2>(c, chunks)) return 16;
     const int ctas = NT == 1 ? plan_ctas<D, Q4, 1>(c, chunks) : plan_ctas<D, Q4, 2>(c, chunks);
     return (size_t)ctas * 2 * R * (D + 2) * sizeof(float);
 }
@@ -868,7 +959,8 @@ cudaError_t launch(RowsCall& p, void* workspace, cudaStream_t st) {
     constexpr int kSmem = C::kRing > kMerge ? C::kRing : kMerge;
     p.rows = p.c.group * p.c.Sq;
     p.chunks = (p.rows + R - 1) / R;
-    p.ctas = plan_ctas<D, Q4, NT>(p.c, p.chunks);
+    p.cluster = clustered<D, Q4, NT>(p.c, p.chunks) ? 1 : 0;
+    p.ctas = p.cluster ? p.c.B * p.c.Hkv * p.chunks * kCluster : plan_ctas<D, Q4, NT>(p.c, p.chunks);
     p.lowest = std::is_same<T, __nv_bfloat16>::value ? 0x43004300u : 0x4c004c00u;  // 128 or 16
     p.others = std::is_same<T, __nv_bfloat16>::value ? 0x41804180u : 0x4c004c00u;  // 16
     p.part_o = static_cast<float*>(workspace);
@@ -884,10 +976,24 @@ cudaError_t launch(RowsCall& p, void* workspace, cudaStream_t st) {
         if (e != cudaSuccess) return e;
         opted.fetch_or(bit, std::memory_order_relaxed);
     }
+    cudaLaunchConfig_t config = {};
+    if (p.cluster) {
+        static_assert(C::kRing >= (kWarps + 1) * R * D * 4 + R * 8, "the warps' and the CTA's rows go through the ring");
+        config.gridDim = dim3((unsigned)p.ctas);
+        config.blockDim = dim3(kWarps * 32);
+        config.dynamicSmemBytes = kSmem;
+        config.stream = st;
+        cudaLaunchAttribute together[1];
+        together[0].id = cudaLaunchAttributeClusterDimension;
+        together[0].val.clusterDim.x = kCluster;
+        together[0].val.clusterDim.y = together[0].val.clusterDim.z = 1;
+        config.attrs = together;
+        config.numAttrs = 1;
+        return cudaLaunchKernelEx(&config, decode_rows<T, D, Q4, NT>, (const RowsCall)p);
+    }
     decode_rows<T, D, Q4, NT><<<p.ctas, kWarps * 32, kSmem, st>>>(p);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned)((int64_t)p.c.B * p.c.Hkv * p.chunks));
     config.blockDim = dim3(1024);
     config.stream = st;

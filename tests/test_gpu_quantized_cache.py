@@ -256,6 +256,29 @@ def test_attention_matches_fp64(case, dtype):
     assert native().device_status(reset=True) == 0
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", (
+    # both sides of the rule that chooses between one cluster per unit and a line of blocks cut over all CTAs:
+    # Hq, Hkv, Sq, capacity, D, window, sinks, starts
+    (4, 4, 1, 96 * 64, 128, 0, 0, (96 * 64 - 1, -1, 500)),         # the longest that clusters take, and the next
+    (4, 4, 1, 96 * 64 + 1, 128, 0, 0, (96 * 64, -1, 500)),
+    (16, 8, 1, 333, 128, 0, 0, tuple(range(-2, 333, 61))),         # 48 units fit ...
+    (16, 8, 1, 333, 128, 0, 0, tuple(range(-2, 333, 49))),         # ... 56 do not
+    (32, 2, 4, 700, 64, 150, 9, tuple(range(-6, 720, 53))),        # 32 rows, two units per cache head: 56 units do not
+    (12, 1, 1, 900, 128, 0, 0, tuple(range(-1, 900, 26))),         # 35 units of 16 rows fit ...
+    (12, 1, 1, 900, 128, 0, 0, tuple(range(-1, 900, 23))),         # ... 40 do not
+))
+def test_short_and_full_batches(case, dtype):
+    Hq, Hkv, Sq, capacity, D, window, sinks, starts = case
+    cache = filled(len(starts), Hkv, capacity, D, dtype, seed=capacity + 3)
+    q = rows(len(starts), Hq, Sq, D, dtype=dtype, seed=capacity + 11, offset=False) * 1.5
+    at = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    want, bound = reference(q, cache, starts, window, sinks)
+    got = api().quantized_cache_attention(q, cache, query_start=at, window=window or None, sinks=sinks)
+    assert bool(((got.cpu().double() - want).abs() <= bound).all())
+    assert native().device_status(reset=True) == 0
+
+
 def test_a_zero_scale_averages_the_visible_values():
     cache = filled(1, 2, 300, 128, torch.bfloat16, seed=5)
     q = rows(1, 4, 1, 128, dtype=torch.bfloat16, seed=6)

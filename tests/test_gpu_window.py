@@ -209,6 +209,33 @@ def test_positions_per_sequence(case, dtype):
     assert native().device_status(reset=True) == 0
 
 
+@pytest.mark.parametrize("case", (
+    # both sides of the rule that chooses between one cluster per unit and a line of blocks cut over all CTAs:
+    # Hq, Hkv, Sq, Sk, D, window, sinks, starts
+    (4, 2, 1, 96 * 16, 128, 4000, 0, (96 * 16 - 1, -1, 200)),       # the longest that clusters take, and the next
+    (4, 2, 1, 96 * 16 + 1, 128, 4000, 0, (96 * 16, -1, 200)),
+    (8, 4, 1, 400, 128, 150, 4, tuple(range(-2, 400, 46))),         # 36 units fit ...
+    (8, 4, 1, 400, 128, 150, 4, tuple(range(-2, 400, 41))),         # ... 40 do not
+    (16, 1, 3, 300, 64, 120, 20, tuple(range(-4, 320, 19))),        # three units of 16 rows: 54 fit ...
+    (16, 1, 3, 300, 64, 120, 20, tuple(range(-4, 320, 17))),        # ... 60 do not
+))
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+def test_decoding_of_short_and_full_batches(case, dtype):
+    Hq, Hkv, Sq, Sk, D, window, sinks, starts = case
+    q, k, v, dout = make_inputs(len(starts), Hq, Hkv, Sq, Sk, D, dtype, seed=Sk + len(starts))
+    mask = window_mask(starts, Sq, Sk, window, sinks)
+    want = ao.math_reference([t.cpu() for t in (q, k, v)], dout.cpu(), mask, False, None)[0]
+    at = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        got = api().sliding_window_attention(q, k, v, window=window, sinks=sinks, query_start=at)
+    for b in range(len(starts)):
+        if mask[b].any():
+            assert ao.per_head_relative_error(got[b:b + 1].cpu(), want[b:b + 1]) < TOL[dtype]["norm"]
+    blind = ~mask.any(-1).expand(len(starts), Hq, Sq)
+    assert float(got.cpu()[blind].abs().sum()) == 0
+    assert native().device_status(reset=True) == 0
+
+
 def test_one_new_token_against_a_long_cache():
     """Many CTAs per sequence; the cache is a view of a larger one, [B, S, H, D] in memory."""
     B, Hq, Hkv, Sk, D = 2, 8, 2, 30000, 128
