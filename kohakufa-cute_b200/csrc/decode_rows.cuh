@@ -22,7 +22,7 @@
 // query rows) have to read are numbered through, and each CTA takes an equal piece of that line; where a unit spans
 // several CTAs their partial (maximum, sum, accumulator) are merged by a second, dependent launch.  The lengths come
 // from device memory, so a captured call follows new positions.  Short calls (few units of few blocks) skip the second
-// launch: a cluster of eight CTAs owns a unit and merges over distributed shared memory.  Within a CTA the warps take blocks in turn, each with
+// launch: a cluster of up to eight CTAs owns a unit and merges over distributed shared memory.  Within a CTA the warps take blocks in turn, each with
 // its own ring of asynchronous copies.  (A piece per warp, without the merge within the CTA, was no faster: 114 against
 // 113 us at 16 x 32768 tokens, 44 against 42 at 16 x 8192, and slower for one sequence.)
 //
@@ -48,7 +48,7 @@ struct RowsCall {
     int64_t kvs[2][3];    // batch, head, token strides (elements)
     int rows, chunks;     // query rows per K/V head, pieces of 8 * NT of them
     int ctas;
-    int cluster;          // != 0: short calls, a thread-block cluster of kCluster CTAs per unit and no second launch
+    int cluster;          // != 0: a thread-block cluster of that many CTAs serves a unit, and there is no second launch
     uint32_t lowest, others;  // see Bases
     float* part_o;        // [ctas][2][8 NT][D]: a CTA's first and last piece of a unit
     float* part_ml;       // [ctas][2][8 NT][2]: maximum, sum
@@ -57,7 +57,7 @@ struct RowsCall {
 namespace rows {
 
 constexpr int kWarps = 4;
-constexpr int kCluster = 8;
+constexpr int kCluster = 8;  // CTAs of a cluster at most
 
 // CTAs per SM that registers and shared memory allow (the launch bounds hold the compiler to it).
 template <int D, bool Q4, int NT>
@@ -209,11 +209,6 @@ __device__ __forceinline__ void copy_bulk(uint32_t dst, const void* src, uint32_
 }
 __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
 }
 // Address of the same shared-memory location in CTA `rank` of the cluster, and loads from there.
 __device__ __forceinline__ uint32_t cluster_address(const void* p, uint32_t rank) {
@@ -524,12 +519,12 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
     const uint32_t units = c.Hkv * p.chunks;
     // This CTA's piece of the line; in a cluster its share of one unit, counted from that unit's first block.
     const Line line(c, units, C::kBlock);
-    const uint32_t my_unit = blockIdx.x / kCluster, my_rank = p.cluster ? cluster_rank() : 0;
+    const uint32_t my_unit = p.cluster ? blockIdx.x / p.cluster : 0, my_rank = p.cluster ? blockIdx.x % p.cluster : 0;
     uint32_t begin, end;
     if (p.cluster) {
         const uint32_t n = blocks_of(c, start_of(c, (int)(my_unit / units)), C::kBlock).count;
-        begin = n * my_rank / kCluster;
-        end = n * (my_rank + 1) / kCluster;
+        begin = n * my_rank / p.cluster;
+        end = n * (my_rank + 1) / p.cluster;
     } else {
         const Cut cut(line.before(c.B), p.ctas);
         if (blockIdx.x >= cut.ctas) return;
@@ -800,7 +795,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
         }
         cluster_barrier();
         const int b = (int)(my_unit / units), unit = (int)(my_unit % units), kvh = unit / p.chunks, row0 = unit % p.chunks * R;
-        for (int idx = threadIdx.x * kCluster + my_rank; idx < R * (D / 4); idx += kWarps * 32 * kCluster) {
+        for (int idx = threadIdx.x * p.cluster + my_rank; idx < R * (D / 4); idx += kWarps * 32 * p.cluster) {
             const int r = idx / (D / 4), d = idx % (D / 4) * 4, row = row0 + r;
             if (row >= p.rows) break;
             float2 ml[kCluster];
@@ -809,8 +804,13 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < kCluster; ++w) {
-                ml[w] = cluster_load2(cluster_address(cta_ml + r, w));
-                x[w] = cluster_load4(cluster_address(cta_o + r * D + d, w));
+                if (w < p.cluster) {
+                    ml[w] = cluster_load2(cluster_address(cta_ml + r, w));
+                    x[w] = cluster_load4(cluster_address(cta_o + r * D + d, w));
+                } else {
+                    ml[w] = make_float2(-INFINITY, 0.f);
+                    x[w] = make_float4(0.f, 0.f, 0.f, 0.f);
+                }
                 mx = fmaxf(mx, ml[w].x);
             }
 #pragma unroll
@@ -932,21 +932,32 @@ int plan_ctas(const CacheAttentionCall& c, int chunks) {
     return (int)(want < 1 ? 1 : (want > most ? most : want));
 }
 
-// Whether clusters serve the call: no more of their CTAs than are resident at once, and at most three blocks per warp.
-// B1 Hq32 Hkv8 D128, GPU time of a step in a graph, two launches -> one cluster launch: window of 1024 10.9 -> 7.6 us,
-// 256 9.3 -> 5.9; 4-bit cache of 1024 tokens 8.5 -> 7.7, 4096 9.9 -> 9.7, 8192 (four blocks per warp) 12.3 -> 13.0; B6
-// at 4096 tokens 19.1 -> 14.6; B6 with a window of 512 11.2 -> 11.7.  Outside graphs a call saves 2.5 us of host time.
+// The CTAs of a cluster per unit, or 0 for the line of blocks cut over all CTAs and a second launch that merges.
+// Clusters of at most eight, nine tenths of what is resident (at 48 units of six, 97 % of the places, some did not find
+// theirs in a first wave: 14.1 us, five each 8.5, the line 11.0), where a warp gets at most two rounds of blocks more
+// than in the line, which costs a second launch and a second start at every cut; four for 16-bit rows, whose blocks
+// are a quarter as long.  D128, 32 query heads on 8, GPU time of a step in a graph, line -> clusters:
+//   4-bit: B1 1024 tokens 7.9 -> 8.0 us, 4096 10.0 -> 10.0, 8192 (3 rounds more, kept in the line) 12.4 -> 13.4;
+//     B6 4096 19.1 -> 15.0; B12 8192 38.5 -> 35.3; B16 8192 46.4 -> 45.0, 16384 (3 more) 76.8 -> 80.9;
+//     64 heads, 4 rows, B8 4096 41.0 -> 38.0.
+//   16-bit: B1 window 256 9.4 -> 6.3, 1024 10.7 -> 8.0, 2048 13.0 -> 9.9, 4000 (7 more) 12.3 -> 12.5;
+//     B8 window 1024 13.9 -> 11.3; B12 window 1000 15.5 -> 14.6; B32 window 1024 29.0 -> 25.5.
+// Outside graphs a call saves 2.5 us of host time besides.
 template <int D, bool Q4, int NT>
-bool clustered(const CacheAttentionCall& c, int chunks) {
-    return (int64_t)c.B * c.Hkv * chunks * kCluster <= 148 * resident<D, Q4, NT>() &&
-           most_blocks<D, Q4, NT>(c) <= 3 * kWarps * kCluster;
+int cluster_size(const CacheAttentionCall& c, int chunks) {
+    const int64_t units = (int64_t)c.B * c.Hkv * chunks, blocks = most_blocks<D, Q4, NT>(c);
+    const int64_t fit = 133 * resident<D, Q4, NT>() / units, size = fit < kCluster ? fit : kCluster;
+    if (size == 0) return 0;
+    const int64_t line = (int64_t)plan_ctas<D, Q4, NT>(c, chunks) * kWarps;
+    const int64_t rounds = (blocks + size * kWarps - 1) / (size * kWarps), spread = (units * blocks + line - 1) / line;
+    return rounds <= spread + (Q4 ? 2 : 4) ? (int)size : 0;
 }
 
 template <int D, bool Q4>
 size_t workspace_bytes(const CacheAttentionCall& c) {
     const int NT = row_tiles(c), R = 8 * NT, chunks = (c.group * c.Sq + R - 1) / R;
     // (a call that clusters serve keeps nothing; 16 bytes keep the size positive)
-    if (NT == 1 ? clustered<D, Q4, 1>(c, chunks) : clustered<D, Q4, 2>(c, chunks)) return 16;
+    if (NT == 1 ? cluster_size<D, Q4, 1>(c, chunks) : cluster_size<D, Q4, 2>(c, chunks)) return 16;
     const int ctas = NT == 1 ? plan_ctas<D, Q4, 1>(c, chunks) : plan_ctas<D, Q4, 2>(c, chunks);
     return (size_t)ctas * 2 * R * (D + 2) * sizeof(float);
 }
@@ -959,8 +970,8 @@ cudaError_t launch(RowsCall& p, void* workspace, cudaStream_t st) {
     constexpr int kSmem = C::kRing > kMerge ? C::kRing : kMerge;
     p.rows = p.c.group * p.c.Sq;
     p.chunks = (p.rows + R - 1) / R;
-    p.cluster = clustered<D, Q4, NT>(p.c, p.chunks) ? 1 : 0;
-    p.ctas = p.cluster ? p.c.B * p.c.Hkv * p.chunks * kCluster : plan_ctas<D, Q4, NT>(p.c, p.chunks);
+    p.cluster = cluster_size<D, Q4, NT>(p.c, p.chunks);
+    p.ctas = p.cluster ? p.c.B * p.c.Hkv * p.chunks * p.cluster : plan_ctas<D, Q4, NT>(p.c, p.chunks);
     p.lowest = std::is_same<T, __nv_bfloat16>::value ? 0x43004300u : 0x4c004c00u;  // 128 or 16
     p.others = std::is_same<T, __nv_bfloat16>::value ? 0x41804180u : 0x4c004c00u;  // 16
     p.part_o = static_cast<float*>(workspace);
@@ -985,7 +996,7 @@ cudaError_t launch(RowsCall& p, void* workspace, cudaStream_t st) {
         config.stream = st;
         cudaLaunchAttribute together[1];
         together[0].id = cudaLaunchAttributeClusterDimension;
-        together[0].val.clusterDim.x = kCluster;
+        together[0].val.clusterDim.x = (unsigned)p.cluster;
         together[0].val.clusterDim.y = together[0].val.clusterDim.z = 1;
         config.attrs = together;
         config.numAttrs = 1;

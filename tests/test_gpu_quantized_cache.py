@@ -258,15 +258,21 @@ def test_attention_matches_fp64(case, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("case", (
-    # both sides of the rule that chooses between one cluster per unit and a line of blocks cut over all CTAs:
-    # Hq, Hkv, Sq, capacity, D, window, sinks, starts
+    # both sides of the rule that chooses between one cluster per unit and a line of blocks cut over all CTAs, and
+    # clusters of every size:  Hq, Hkv, Sq, capacity, D, window, sinks, starts
     (4, 4, 1, 96 * 64, 128, 0, 0, (96 * 64 - 1, -1, 500)),         # the longest that clusters take, and the next
     (4, 4, 1, 96 * 64 + 1, 128, 0, 0, (96 * 64, -1, 500)),
-    (16, 8, 1, 333, 128, 0, 0, tuple(range(-2, 333, 61))),         # 48 units fit ...
-    (16, 8, 1, 333, 128, 0, 0, tuple(range(-2, 333, 49))),         # ... 56 do not
-    (32, 2, 4, 700, 64, 150, 9, tuple(range(-6, 720, 53))),        # 32 rows, two units per cache head: 56 units do not
-    (12, 1, 1, 900, 128, 0, 0, tuple(range(-1, 900, 26))),         # 35 units of 16 rows fit ...
-    (12, 1, 1, 900, 128, 0, 0, tuple(range(-1, 900, 23))),         # ... 40 do not
+    (16, 8, 1, 333, 128, 0, 0, tuple(range(-2, 333, 61))),         # 48 units: eight CTAs each
+    (16, 8, 1, 333, 128, 0, 0, tuple(range(-2, 333, 49))),         # 56: seven
+    (16, 8, 1, 333, 128, 0, 0, tuple(range(-2, 333, 43))),         # 64: six
+    (16, 8, 1, 700, 128, 0, 0, tuple(range(-2, 700, 79))),         # 72: five
+    (16, 8, 1, 700, 128, 200, 3, tuple(range(-2, 700, 54))),       # 104: three
+    (16, 8, 1, 600, 128, 0, 0, tuple(range(-2, 600, 33))),         # 152: two
+    (16, 8, 1, 400, 128, 0, 0, tuple(range(-2, 400, 11))),         # 296: one
+    (16, 8, 1, 200, 128, 0, 0, tuple(range(-2, 200, 4))),          # 408: the line
+    (32, 2, 4, 700, 64, 150, 9, tuple(range(-6, 720, 53))),        # 32 rows, two units per cache head
+    (12, 1, 1, 900, 128, 0, 0, tuple(range(-1, 900, 23))),         # 40 units of 16 rows
+    (12, 1, 1, 300, 128, 0, 0, tuple(range(-1, 300, 1))),          # 301: the line
 ))
 def test_short_and_full_batches(case, dtype):
     Hq, Hkv, Sq, capacity, D, window, sinks, starts = case

@@ -210,14 +210,15 @@ def test_positions_per_sequence(case, dtype):
 
 
 @pytest.mark.parametrize("case", (
-    # both sides of the rule that chooses between one cluster per unit and a line of blocks cut over all CTAs:
-    # Hq, Hkv, Sq, Sk, D, window, sinks, starts
-    (4, 2, 1, 96 * 16, 128, 4000, 0, (96 * 16 - 1, -1, 200)),       # the longest that clusters take, and the next
-    (4, 2, 1, 96 * 16 + 1, 128, 4000, 0, (96 * 16, -1, 200)),
-    (8, 4, 1, 400, 128, 150, 4, tuple(range(-2, 400, 46))),         # 36 units fit ...
-    (8, 4, 1, 400, 128, 150, 4, tuple(range(-2, 400, 41))),         # ... 40 do not
-    (16, 1, 3, 300, 64, 120, 20, tuple(range(-4, 320, 19))),        # three units of 16 rows: 54 fit ...
-    (16, 1, 3, 300, 64, 120, 20, tuple(range(-4, 320, 17))),        # ... 60 do not
+    # both sides of the rule that chooses between one cluster per unit and a line of blocks cut over all CTAs, and
+    # clusters of several sizes:  Hq, Hkv, Sq, Sk, D, window, sinks, starts
+    (4, 2, 1, 160 * 16, 128, 4000, 0, (160 * 16 - 1, -1, 200)),     # the longest that clusters take, and the next
+    (4, 2, 1, 160 * 16 + 1, 128, 4000, 0, (160 * 16, -1, 200)),
+    (8, 4, 1, 400, 128, 150, 4, tuple(range(-2, 400, 51))),         # 32 units: eight CTAs each
+    (8, 4, 1, 400, 128, 150, 4, tuple(range(-2, 400, 41))),         # 40: six
+    (8, 8, 1, 300, 128, 150, 4, tuple(range(-2, 300, 28))),         # 88: three
+    (8, 8, 1, 300, 128, 150, 4, tuple(range(-2, 300, 9))),          # 272: the line
+    (16, 1, 3, 300, 64, 120, 20, tuple(range(-4, 320, 17))),        # three units of 16 rows: 60
 ))
 @pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
 def test_decoding_of_short_and_full_batches(case, dtype):
