@@ -1167,9 +1167,11 @@ int kfa_window_forward(const kfa_tensor* q, const kfa_tensor* k, const kfa_tenso
             return fail(KFA_INVALID_ARGUMENT, "window forward workspace too small or not 16-byte aligned");
         if (rows_ok(p.q, p.qs, q->sizes) && rows_ok(p.k, p.ks, k->sizes) && rows_ok(p.v, p.vs, v->sizes) &&
             rows_ok(p.out, p.os, out->sizes)) {
-            cudaError_t ce = timed("window_decode", st, [&] { return kfa::launch_window_decode(p, bf16, workspace, st); });
+            int launches = 0;
+            cudaError_t ce = timed("window_decode", st,
+                                   [&] { return kfa::launch_window_decode(p, bf16, workspace, &launches, st); });
             if (ce != cudaSuccess) return cuda_fail(ce, "window decode launch");
-            count_kernel("window_decode", 1);  // two launches
+            if (launches > 1) count_kernel("window_decode", (uint64_t)(launches - 1));
             return 0;
         }
     }
@@ -1278,7 +1280,9 @@ int fill_cache_half(kfa::CacheView& view, const kfa_tensor* codes, const kfa_ten
     return 0;
 }
 
-int check_positions(const kfa_tensor* t, int64_t batch, const char* name) {
+int check_positions(const kfa_tensor* t, int64_t batch, const char* name, int64_t start = 0) {
+    if (!t && (start > INT32_MAX || start < INT32_MIN))
+        return fail(KFA_INVALID_ARGUMENT, "quantized cache: the position exceeds 32 bits");
     if (t && (!t->data || t->dtype != KFA_I32 || t->ndim != 1 || t->sizes[0] != batch || (batch > 1 && t->strides[0] != 1)))
         return fail(KFA_INVALID_ARGUMENT, "quantized cache: %s must be contiguous int32 [batch]", name);
     return 0;
@@ -1313,7 +1317,7 @@ int fill_cache_call(kfa::CacheCall& p, const kfa_tensor* k, const kfa_tensor* v,
     p.n = (int)k->sizes[2];
     p.D = (int)k->sizes[3];
     p.capacity = (int)k_codes->sizes[2];
-    if (int e = check_positions(starts, p.B, "starts")) return e;
+    if (int e = check_positions(starts, p.B, "starts", start)) return e;
     if (k->sizes[0] * k->sizes[1] > INT32_MAX / 2 || 2 * k->sizes[0] * k->sizes[1] * (k->sizes[2] / 16 + 1) > INT32_MAX)
         return fail(KFA_TOO_LARGE, "quantized cache: too many rows in one call");
     p.starts = starts ? static_cast<const int32_t*>(starts->data) : nullptr;
@@ -1406,7 +1410,7 @@ int kfa_cache_attention(const kfa_tensor* q, const kfa_tensor* k_codes, const kf
     if (int e = fill_cache_attention(p, q, k_codes, window, sinks)) return e;
     if (int e = fill_cache_half(p.half[0], k_codes, k_params, k_codes, q->dtype)) return e;
     if (int e = fill_cache_half(p.half[1], v_codes, v_params, k_codes, q->dtype)) return e;
-    if (int e = check_positions(starts, p.B, "starts")) return e;
+    if (int e = check_positions(starts, p.B, "starts", start)) return e;
     if (int e = check_like(out, q, "out")) return e;
     for (const kfa_tensor* t : {q, static_cast<const kfa_tensor*>(out)}) {
         bool ok = t->data && t->strides[3] == 1 && reinterpret_cast<uintptr_t>(t->data) % 16 == 0;
@@ -1430,10 +1434,11 @@ int kfa_cache_attention(const kfa_tensor* q, const kfa_tensor* k_codes, const kf
     p.status = status_word(&err, st);
     if (!p.status) return err;
     p.abort_flag = abort_flag_of_current_device();
+    int launches = 0;
     cudaError_t ce = timed("cache_attention", st,
-                           [&] { return kfa::launch_cache_attention(p, q->dtype == KFA_BF16, workspace, st); });
+                           [&] { return kfa::launch_cache_attention(p, q->dtype == KFA_BF16, workspace, &launches, st); });
     if (ce != cudaSuccess) return cuda_fail(ce, "cache attention launch");
-    count_kernel("cache_attention", 1);  // two launches
+    if (launches > 1) count_kernel("cache_attention", (uint64_t)(launches - 1));
     return 0;
 }
 

@@ -41,14 +41,14 @@ cudaError_t launch_decode_forward(const AttnParams& p, bool bf16, void* workspac
 // Windowed forward for at most 16 query rows per K/V head (64 or 128 channels, 16-byte addressable rows): no statistics.
 bool window_decode_shape(const AttnParams& p);
 size_t window_decode_workspace_bytes(const AttnParams& p);
-cudaError_t launch_window_decode(const AttnParams& p, bool bf16, void* workspace, cudaStream_t st);
+cudaError_t launch_window_decode(const AttnParams& p, bool bf16, void* workspace, int* launches, cudaStream_t st);
 
 // 4-bit key/value cache: rows quantised into it, read back, attended to.
 cudaError_t launch_cache_write(const CacheCall& p, bool bf16, cudaStream_t st);
 cudaError_t launch_cache_read(const CacheCall& p, bool bf16, cudaStream_t st);
 bool cache_attention_countable(const CacheAttentionCall& p);  // else too large for one call
 size_t cache_attention_workspace_bytes(const CacheAttentionCall& p);
-cudaError_t launch_cache_attention(const CacheAttentionCall& p, bool bf16, void* workspace, cudaStream_t st);
+cudaError_t launch_cache_attention(const CacheAttentionCall& p, bool bf16, void* workspace, int* launches, cudaStream_t st);
 
 cudaError_t launch_neighborhood_forward(const AttnParams& p, bool bf16, cudaStream_t st);
 cudaError_t launch_neighborhood_backward(const AttnParams& p, bool bf16, int which, cudaStream_t st);

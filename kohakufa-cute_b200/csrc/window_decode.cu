@@ -43,7 +43,7 @@ size_t window_decode_workspace_bytes(const AttnParams& p) {
     return p.D == 128 ? rows::workspace_bytes<128, false>(c) : rows::workspace_bytes<64, false>(c);
 }
 
-cudaError_t launch_window_decode(const AttnParams& p, bool bf16, void* workspace, cudaStream_t st) {
+cudaError_t launch_window_decode(const AttnParams& p, bool bf16, void* workspace, int* launches, cudaStream_t st) {
     RowsCall r = {};
     r.c = call_of(p);
     r.kv[0] = p.k;
@@ -52,7 +52,10 @@ cudaError_t launch_window_decode(const AttnParams& p, bool bf16, void* workspace
         r.kvs[0][i] = p.ks[i];
         r.kvs[1][i] = p.vs[i];
     }
-    return bf16 ? rows::dispatch<__nv_bfloat16, false>(r, workspace, st) : rows::dispatch<__half, false>(r, workspace, st);
+    const cudaError_t e =
+        bf16 ? rows::dispatch<__nv_bfloat16, false>(r, workspace, st) : rows::dispatch<__half, false>(r, workspace, st);
+    *launches = r.cluster ? 1 : 2;
+    return e;
 }
 
 }  // namespace kfa

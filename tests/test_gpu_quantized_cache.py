@@ -293,6 +293,15 @@ def test_a_zero_scale_averages_the_visible_values():
     assert bool(((got.cpu().double() - want).abs() <= bound).all())
 
 
+def test_launches_are_counted():
+    cache = filled(1, 2, 9000, 128, torch.bfloat16, seed=3)
+    q = rows(1, 8, 1, 128, dtype=torch.bfloat16, seed=4)
+    for window, launches in ((100, 1), (None, 2)):  # one cluster per K/V head; a line of blocks and its merge
+        before = native().launch_count()
+        api().quantized_cache_attention(q, cache, query_start=8999, window=window)
+        assert native().launch_count() - before == launches
+
+
 def test_large_logits_pick_one_key():
     """Scores that differ by hundreds: the softmax is a copy of one value row."""
     for dtype in TYPES:
@@ -441,6 +450,10 @@ def test_refusals():
                  lambda: attend(q, cache, query_start=0, scale=float("inf")),
                  lambda: attend(q, cache, query_start=torch.zeros(2, dtype=torch.int64, device="cuda"))):
         with pytest.raises(ValueError):
+            call()
+    for call in (lambda: native().cache_write(k, k, *cache, None, None, 2**31), lambda: native().cache_read(*cache, None, -2**40, 1),
+                 lambda: native().cache_attention(q, *cache, None, 2**62, 0, 0, 0.1)):
+        with pytest.raises(ValueError, match="32 bits"):  # (the public calls refuse these before the library does)
             call()
     wide = api().quantized_cache(1, 1, 4, 256)
     with pytest.raises(ValueError, match="64 and 128"):
