@@ -22,9 +22,11 @@
 // query rows) have to read are numbered through, and each CTA takes an equal piece of that line; where a unit spans
 // several CTAs their partial (maximum, sum, accumulator) are merged by a second, dependent launch.  The lengths come
 // from device memory, so a captured call follows new positions.  Short calls (few units of few blocks) skip the second
-// launch: a cluster of up to eight CTAs owns a unit and merges over distributed shared memory.  Within a CTA the warps take blocks in turn, each with
-// its own ring of asynchronous copies.  (A piece per warp, without the merge within the CTA, was no faster: 114 against
-// 113 us at 16 x 32768 tokens, 44 against 42 at 16 x 8192, and slower for one sequence.)
+// launch: a cluster of up to eight CTAs owns a unit and merges over distributed shared memory.  Within a CTA the warps
+// take blocks in turn, each with its own ring of asynchronous copies.  (A piece per warp, without the merge within the
+// CTA, was no faster: 114 against 113 us at 16 x 32768 tokens, 44 against 42 at 16 x 8192, and slower for one sequence.)
+// More than 16 rows per K/V head widen the codes once per 16.  (Once per 32, into shared memory for four warps of eight
+// rows each, was slower, 58 against 44 us at 32 rows: every warp then reads the whole tile from there.)
 //
 // Measured: 16-bit cache, 48 sequences with windows of 4096 tokens, 8 K/V heads of 128: 126 us, 6.4 TB/s, the HBM copy
 // rate.  4-bit cache, 16 x 24 600 tokens on average: 113 us, 4.1 TB/s (64 %): issue slots 58 % and the integer pipe 57 %

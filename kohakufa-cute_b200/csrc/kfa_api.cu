@@ -1293,8 +1293,9 @@ int check_cache_rows(const kfa_tensor* t, const kfa_tensor* codes) {
     if (!t || !t->data || t->ndim != 4 || !is_half_type(t))
         return fail(KFA_INVALID_ARGUMENT, "quantized cache requires 4D FP16/BF16 K/V rows");
     if (t->sizes[0] != codes->sizes[0] || t->sizes[1] != codes->sizes[1] || t->sizes[3] != 2 * codes->sizes[3] ||
-        t->sizes[2] <= 0 || t->sizes[2] > INT32_MAX)
+        t->sizes[2] <= 0)
         return fail(KFA_INVALID_ARGUMENT, "quantized cache: K/V rows do not match the cache's batch, heads and channels");
+    if (t->sizes[2] > INT32_MAX - 256) return fail(KFA_TOO_LARGE, "quantized cache: at most 2^31 - 257 rows in one call");
     bool ok = t->strides[3] == 1 && reinterpret_cast<uintptr_t>(t->data) % 16 == 0;
     for (int i = 0; i < 3; ++i) ok = ok && (t->sizes[i] == 1 || t->strides[i] % 8 == 0);
     if (!ok) return fail(KFA_INVALID_ARGUMENT, "quantized cache requires 16-byte addressable K/V rows");
