@@ -9,7 +9,9 @@ how many cycles each role of one CTA spends in each phase of its loop (see ``csr
 """
 
 import hashlib
+import importlib.util
 import os
+import shutil
 import subprocess
 import sys
 import sysconfig
@@ -81,6 +83,7 @@ def build(force=False, verbose=True, phases=False):
         subprocess.check_call(cmd)
     if not phases:
         build_records(force, verbose)
+        build_calls(force, verbose)
     return lib
 
 
@@ -97,6 +100,37 @@ def build_records(force=False, verbose=True):
     os.makedirs(OBJ_DIR, exist_ok=True)
     stamp = os.path.join(OBJ_DIR, "fast_records.sha")
     digest = _digest([source, header], cmd)
+    if force or not os.path.exists(target) or not os.path.exists(stamp) or open(stamp).read() != digest:
+        if verbose:
+            print(" ".join(cmd + ["-o", target]), flush=True)
+        subprocess.check_call(cmd + ["-o", target])
+        with open(stamp, "w") as f:
+            f.write(digest)
+    return target
+
+
+def build_calls(force=False, verbose=True):
+    """The optional torch module that serves plain window and cache calls in one step (``csrc/fast_calls.cpp``), or
+    ``None`` without the headers it needs: the Python layer then serves them, with the same results."""
+    include = sysconfig.get_paths()["include"]
+    spec = importlib.util.find_spec("torch")
+    home = os.path.dirname(spec.origin) if spec and spec.origin else ""
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(shutil.which(_nvcc()) or _nvcc()))), "include")
+    needed = (os.path.join(include, "Python.h"), os.path.join(home, "include", "c10", "cuda", "CUDAStream.h"),
+              os.path.join(cuda, "cuda_runtime_api.h"))
+    if not all(os.path.exists(path) for path in needed):
+        return None
+    source = os.path.join(CSRC, "fast_calls.cpp")
+    header = os.path.join(os.path.dirname(HERE), "include", "kfa.h")
+    target = os.path.join(OUT_DIR, "_fast_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-Wall", "-shared", "-fPIC", "-fvisibility=hidden", "-I", include]
+    for path in (os.path.join(home, "include"), os.path.join(home, "include", "torch", "csrc", "api", "include"), cuda):
+        cmd += ["-isystem", path]
+    cmd += [source, "-L", os.path.join(home, "lib"), "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda"]
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    stamp = os.path.join(OBJ_DIR, "fast_calls.sha")
+    # (the module belongs to one torch: its version is part of the stamp)
+    digest = _digest([source, header, os.path.join(home, "version.py")], cmd)
     if force or not os.path.exists(target) or not os.path.exists(stamp) or open(stamp).read() != digest:
         if verbose:
             print(" ".join(cmd + ["-o", target]), flush=True)

@@ -21,6 +21,8 @@ from math import isfinite, prod
 
 import torch
 
+from . import native
+
 _native_sdpa = torch.nn.functional.scaled_dot_product_attention
 _HALF_TYPES = (torch.float16, torch.bfloat16)
 _SUPPORTED_CAPABILITY = (10, 0)
@@ -34,7 +36,10 @@ def _device_supported(device):
 
 @lru_cache(maxsize=None)
 def _device_supported_once(device):
-    return torch.cuda.get_device_capability(device) == _SUPPORTED_CAPABILITY
+    supported = torch.cuda.get_device_capability(device) == _SUPPORTED_CAPABILITY
+    if supported and native.fast is not None and device.index is not None:
+        native.fast.allow(device.index)
+    return supported
 
 
 def _check_arguments(q, k, v, mask, dropout, causal, gqa, *, combined_mask=False):
@@ -166,6 +171,10 @@ def sliding_window_attention(q, k, v, *, window, sinks=0, query_start=0, scale=N
     graph can be replayed with new positions; any value is allowed, keys behind a sequence's last position may hold
     anything).  Differentiable with respect to Q, K and V when ``query_start`` is an int.
     """
+    if native.fast is not None and not torch.compiler.is_compiling():
+        out = native.fast.window_attention(q, k, v, window, sinks, query_start, scale)
+        if out is not None:
+            return out
     _check_arguments(q, k, v, None, 0.0, False, True)
     starts, start = _window_arguments("sliding_window_attention", q.shape[0], q.device, window, sinks, query_start)
     scale = _resolved_scale("sliding_window_attention", scale, q.shape[-1])

@@ -120,6 +120,9 @@ def quantized_cache_write(cache, k, v, *, start=0, lengths=None):
     (an int ``start`` that would write past the end is refused).  A group of channels with a value that is not finite
     reads back as NaN.
     """
+    if native.fast is not None and not torch.compiler.is_compiling():
+        if native.fast.cache_write(cache, k, v, start, lengths):
+            return
     name = "quantized_cache_write"
     _check_cache(name, cache)
     kc, kp = cache[0], cache[1]
@@ -149,6 +152,10 @@ def quantized_cache_read(cache, *, start=0, length=None):
     """``(k, v)``: the values of ``length`` rows of every sequence from position ``start`` (an int or an int32 ``[B]``
     tensor) on, ``[B, H, length, D]`` in the cache's type, rounded once.  ``length`` defaults to the rest of the cache
     behind an int ``start``; rows outside the cache (possible with a tensor) read as zeros."""
+    if native.fast is not None and not torch.compiler.is_compiling():
+        rows = native.fast.cache_read(cache, start, length)
+        if rows is not None:
+            return rows
     name = "quantized_cache_read"
     _check_cache(name, cache)
     kc = cache[0]
@@ -175,6 +182,10 @@ def quantized_cache_attention(q, cache, *, query_start, window=None, sinks=0, sc
     ``sliding_window_attention``.  A row that sees no key is zero; what lies behind a sequence's last position may hold
     anything.  Inference only.
     """
+    if native.fast is not None and not torch.compiler.is_compiling():
+        out = native.fast.cache_attention(q, cache, query_start, window, sinks, scale)
+        if out is not None:
+            return out
     name = "quantized_cache_attention"
     _check_cache(name, cache)
     kc, kp = cache[0], cache[1]

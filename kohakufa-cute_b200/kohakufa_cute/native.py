@@ -21,6 +21,10 @@ try:  # optional: packs tensor records in C (build.py leaves it out where Python
     from . import _fast_records
 except ImportError:
     _fast_records = None
+try:  # optional: plain window and cache calls in one step (build.py leaves it out where torch's headers are missing)
+    from . import _fast_calls as fast
+except ImportError:
+    fast = None
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIBRARY_PATH = os.path.join(_HERE, "libkfa.so")
@@ -126,6 +130,9 @@ def library():
                     fn.restype = restype
                     fn.argtypes = argtypes
                 _library = lib
+                if fast is not None:
+                    fast.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
+                               for name in SIGNATURES if name.startswith(("kfa_window_", "kfa_cache_"))}, _check)
     return _library
 
 
