@@ -111,7 +111,8 @@ def build_records(force=False, verbose=True):
 
 def build_calls(force=False, verbose=True):
     """The optional torch module that serves plain window and cache calls in one step (``csrc/fast_calls.cpp``), or
-    ``None`` without the headers it needs: the Python layer then serves them, with the same results."""
+    ``None`` without the headers it needs, or where this torch's do not compile here: the Python layer then serves
+    them, with the same results."""
     include = sysconfig.get_paths()["include"]
     spec = importlib.util.find_spec("torch")
     home = os.path.dirname(spec.origin) if spec and spec.origin else ""
@@ -134,7 +135,13 @@ def build_calls(force=False, verbose=True):
     if force or not os.path.exists(target) or not os.path.exists(stamp) or open(stamp).read() != digest:
         if verbose:
             print(" ".join(cmd + ["-o", target]), flush=True)
-        subprocess.check_call(cmd + ["-o", target])
+        try:
+            subprocess.check_call(cmd + ["-o", target])
+        except (OSError, subprocess.CalledProcessError) as error:
+            print(f"left out: {target} ({error})", flush=True)
+            if os.path.exists(target):  # (of other sources or another torch)
+                os.remove(target)
+            return None
         with open(stamp, "w") as f:
             f.write(digest)
     return target
