@@ -10,7 +10,7 @@
 // bytes, and its rows are tokens only in one of the two products.)
 //
 // 4-bit caches are never widened to values.  Codes become 16-bit floats in two instructions per pair (shift, and one
-// logic operation that masks the code into the mantissa of a base, 16 or 128), and scale and zero of a token's group of
+// logic operation that masks the code into the mantissa of a base, 16 to 1024), and scale and zero of a token's group of
 // 64 channels are applied to sums, in FP32:
 //   s    = sum_g  scale_g * (sum_d q_d (base_d + code_d) - sum_d q_d base_d)  +  zero_g * (sum_d q_d)
 //   o_d  = sum_t  round16(p_t scale_g) * (code_d - 8)  +  sum_t p_t (zero_g + 8 scale_g)
@@ -233,31 +233,41 @@ template <int N>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // Code t (0..3) of both halves of a word as a pair of 16-bit floats base<t> + code: the four bits land in the mantissa of
-// the base (in BF16 the lowest code is in place already: 128 + code).  The integer pipe, which has the masks and the
-// shifts, bounds the kernel; shifting by multiplications on the FMA pipe was slower (169 against 154 us).
+// the base (in BF16 the lowest code is in place already: 128 + code; in FP16 the second: 64 + code).  The integer pipe,
+// which has the masks and the shifts, bounds the kernel; shifting by multiplications on the FMA pipe was slower (169
+// against 154 us).
 template <bool BF16, int t>
-__host__ __device__ constexpr float base_of() { return BF16 && t == 0 ? 128.f : 16.f; }
+__host__ __device__ constexpr float base_of() { return BF16 ? (t == 0 ? 128.f : 16.f) : 64.f; }
 struct Bases {
     uint32_t lowest, others;  // the bases' bits in both halves, from the launch: values the compiler does not know stay in
                               // registers, and mask and base go into one three-input logic instruction
 };
-template <bool BF16, int t>
-__device__ __forceinline__ uint32_t widen(uint32_t w, const Bases& base) {
-    constexpr int to = BF16 ? (t == 0 ? 0 : 3) : 6, shift = to - 4 * t;  // where the four bits go in the mantissa
-    constexpr uint32_t mask = 0x000f000fu << to;
-    const uint32_t x = shift >= 0 ? w << (shift >= 0 ? shift : 0) : w >> (shift < 0 ? -shift : 0);
+template <uint32_t mask>
+__device__ __forceinline__ uint32_t masked_or(uint32_t x, uint32_t base) {
     uint32_t y;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "n"(mask), "r"(BF16 && t == 0 ? base.lowest : base.others));
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "n"(mask), "r"(base));
     return y;
 }
-// The same less base<t> + 8: code - 8, exactly.  (Taking the bases off by one more product, with a constant operand, was
-// slower: 122 against 112 us at 16 x 32768 tokens.)
+template <bool BF16, int t>
+__device__ __forceinline__ uint32_t widen(uint32_t w, const Bases& base) {
+    constexpr int to = BF16 ? (t == 0 ? 0 : 3) : 4, shift = to - 4 * t;  // where the four bits go in the mantissa
+    const uint32_t x = shift >= 0 ? w << (shift >= 0 ? shift : 0) : w >> (shift < 0 ? -shift : 0);
+    return masked_or<(0x000f000fu << to)>(x, BF16 && t == 0 ? base.lowest : base.others);
+}
+// The same less the base and 8: code - 8, exactly.  In FP16, where the base goes at once, the codes of a byte stay where
+// they are (1024 + code, 64 + code), and one shift serves both of the upper byte.  (Taking the bases off by one more
+// product, with a constant operand, was slower: 122 against 112 us at 16 x 32768 tokens.)
 template <bool BF16, int t>
 __device__ __forceinline__ uint32_t centred(uint32_t w, const Bases& base) {
-    const uint32_t x = widen<BF16, t>(w, base);
     uint32_t y;
-    if constexpr (BF16) asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(t == 0 ? 0x43084308u : 0x41c041c0u));
-    else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x4e004e00u));
+    if constexpr (BF16) {
+        const uint32_t x = widen<BF16, t>(w, base);
+        asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(t == 0 ? 0x43084308u : 0x41c041c0u));
+    } else {
+        const uint32_t at = t < 2 ? w : w >> 8;
+        const uint32_t x = t % 2 == 0 ? masked_or<0x000f000fu>(at, base.lowest) : masked_or<0x00f000f0u>(at, base.others);
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(t % 2 == 0 ? 0x64086408u : 0x54805480u));
+    }
     return y;
 }
 
@@ -974,8 +984,8 @@ cudaError_t launch(RowsCall& p, void* workspace, cudaStream_t st) {
     p.chunks = (p.rows + R - 1) / R;
     p.cluster = cluster_size<D, Q4, NT>(p.c, p.chunks);
     p.ctas = p.cluster ? p.c.B * p.c.Hkv * p.chunks * p.cluster : plan_ctas<D, Q4, NT>(p.c, p.chunks);
-    p.lowest = std::is_same<T, __nv_bfloat16>::value ? 0x43004300u : 0x4c004c00u;  // 128 or 16
-    p.others = std::is_same<T, __nv_bfloat16>::value ? 0x41804180u : 0x4c004c00u;  // 16
+    p.lowest = std::is_same<T, __nv_bfloat16>::value ? 0x43004300u : 0x64006400u;  // 128 or 1024
+    p.others = std::is_same<T, __nv_bfloat16>::value ? 0x41804180u : 0x54005400u;  // 16 or 64
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = p.part_o + (size_t)p.ctas * 2 * R * D;
     // the shared-memory opt-in holds per device; a decoding step is short enough for the call to show, so it is made once
