@@ -21,6 +21,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -29,7 +30,9 @@
 #include <cmath>
 #include <cstring>
 #include <initializer_list>
+#include <memory>
 #include <optional>
+#include <vector>
 
 #include "../../include/kfa.h"
 
@@ -212,6 +215,15 @@ struct WindowAttention : public torch::autograd::Function<WindowAttention> {
             python_error error;
             error.persist();
             throw python_error(std::move(error));
+        }
+        if (at::GradMode::is_enabled()) {
+            // create_graph: gradients that raise when they are differentiated, not constants
+            const auto twice = std::make_shared<torch::autograd::DelayedError>(
+                "sliding_window_attention cannot be differentiated twice", 3);
+            torch::autograd::variable_list results{dq, dk, dv};
+            for (Tensor& t : results) t = t.detach().set_requires_grad(true);
+            results = (*twice)(std::move(results));
+            dq = results[0], dk = results[1], dv = results[2];
         }
         return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()};
     }

@@ -169,7 +169,7 @@ def sliding_window_attention(q, k, v, *, window, sinks=0, query_start=0, scale=N
     ``c < sinks``); a row that sees no key is zero.  ``query_start`` is an int (0: queries and keys start together, as
     in training), or an int32 ``[B]`` CUDA tensor with one position per sequence, read by the kernels (a captured
     graph can be replayed with new positions; any value is allowed, keys behind a sequence's last position may hold
-    anything).  Differentiable with respect to Q, K and V when ``query_start`` is an int.
+    anything).  Differentiable (once) with respect to Q, K and V when ``query_start`` is an int.
     """
     if native.fast is not None and not torch.compiler.is_compiling():
         out = native.fast.window_attention(q, k, v, window, sinks, query_start, scale)

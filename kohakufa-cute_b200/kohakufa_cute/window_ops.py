@@ -2,7 +2,7 @@
 
 Like the attention operator (``_ops.py``): eager calls use a ``torch.autograd.Function`` (least host overhead), calls
 under ``torch.compile`` the ``kohakufa_cute::window_forward`` / ``window_backward`` custom operators.  Only O is
-differentiable; the two row statistics are saved outputs.
+differentiable, and only once; the two row statistics are saved outputs.
 """
 
 from typing import Optional
@@ -64,7 +64,11 @@ class _EagerWindow(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         q, k, v, out, maximum, logsum = ctx.saved_tensors
-        return *native.window_backward(q, k, v, out, maximum, logsum, dout, *ctx.parameters), None, None, None, None
+        grads = native.window_backward(q, k, v, out, maximum, logsum, dout, *ctx.parameters)
+        if torch.is_grad_enabled():  # create_graph: gradients that raise when they are differentiated, not constants
+            twice = torch._C._functions.DelayedError("sliding_window_attention cannot be differentiated twice", 3)
+            grads = twice(*(grad.detach().requires_grad_() for grad in grads))
+        return *grads, None, None, None, None
 
 
 def attention(q, k, v, starts, start, window, sinks, scale):

@@ -162,6 +162,21 @@ def test_graph_node_behaves(counted):
         assert torch.equal(api().sliding_window_attention(q, k, v, **call), out)
 
 
+def test_second_derivatives_are_refused_both_ways(counted, monkeypatch):
+    q, k, v = (rows(1, 2, 100, 64, seed=s).requires_grad_() for s in (1, 2, 3))
+
+    def twice():
+        out = api().sliding_window_attention(q, k, v, window=9)
+        grad, = torch.autograd.grad(out.sum(), q, create_graph=True)
+        with pytest.raises(RuntimeError, match="twice"):
+            (grad.float().square().sum() + q.float().sum()).backward()
+        return grad.detach()
+
+    out = api().sliding_window_attention(q, k, v, window=9)
+    want, = torch.autograd.grad(out.sum(), q)
+    assert torch.equal(twice(), want) and torch.equal(without(monkeypatch, twice), want)
+
+
 def test_a_report_of_a_wait_that_ran_out_reaches_both_directions(counted):
     q = rows(1, 2, 200, 64).requires_grad_()
     out = api().sliding_window_attention(q, q, q, window=20)
