@@ -236,8 +236,8 @@ KFA_API int kfa_merge_splits(kfa_tensor* out, kfa_tensor* maximum, kfa_tensor* l
  * call can be captured in a graph and replayed with new positions).  Any position is allowed: a row that sees no key
  * yields out = 0, maximum = -inf, logsum = 0.  window >= 1, sinks >= 0, any other operand as for kfa_forward; the
  * statistics may both be NULL.  `workspace` holds kfa_window_forward_workspace_bytes() bytes, 16-byte aligned (0: may be
- * NULL): without statistics, calls of at most 16 query rows per K/V head (positions x grouped heads, 64 or 128
- * channels) run on the decoding kernels, which need it.
+ * NULL): without statistics, calls of few query rows per K/V head (positions x grouped heads: up to 16, and more where
+ * the tensor-memory forward would have few long CTAs; 64 or 128 channels) run on the decoding kernels, which need it.
  *
  * kfa_window_backward takes the forward's out/maximum/logsum and one `start` >= 0 for all batches; `workspace` holds
  * kfa_window_backward_workspace_bytes() bytes, 256-byte aligned.  Every gradient has one owner and a fixed order of

@@ -219,6 +219,12 @@ def test_positions_per_sequence(case, dtype):
     (8, 8, 1, 300, 128, 150, 4, tuple(range(-2, 300, 28))),         # 88: three
     (8, 8, 1, 300, 128, 150, 4, tuple(range(-2, 300, 9))),          # 272: the line
     (16, 1, 3, 300, 64, 120, 20, tuple(range(-4, 320, 17))),        # three units of 16 rows: 60
+    # more rows than a unit has, on both sides of the rule that leaves them to the tensor-memory forward
+    (32, 4, 4, 900, 128, 500, 4, (896, 2, -3, 500, 901)),           # 32 rows
+    (4, 2, 33, 700, 128, 300, 0, (667, 0, -20, 690)),               # 66: the last unit holds two
+    (8, 1, 100, 600, 64, 77, 3, (500, 30, 590)),
+    (6, 2, 256, 900, 128, 800, 130, (644, -100)),
+    (2, 2, 64, 300, 128, 50, 1, tuple(range(-60, 300, 3))),         # 120 sequences: too many
 ))
 @pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
 def test_decoding_of_short_and_full_batches(case, dtype):
