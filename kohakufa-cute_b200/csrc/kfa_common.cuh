@@ -74,6 +74,7 @@ struct AttnParams {
     // afterwards.  0 = not split.
     int sink_tiles, sink_chunks;
     float* sink_partial;
+    int key_splits;  // windowed forward: CTAs of a cluster that share a query tile's key tiles (0 or 1: one CTA)
     int* status;      // device-visible status word (mapped host memory)
     int* abort_flag;  // device memory: set by the first CTA whose bounded wait gives up; later CTAs skip their work
 };

@@ -118,16 +118,20 @@ __global__ void __launch_bounds__(threads_of(WINDOW ? 1 : 2), WINDOW ? 2 : 1)
     Shared& sh = *reinterpret_cast<Shared*>(sKV + Cfg::kStages * Cfg::kTileBytes);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // A windowed call of few query tiles: a cluster of CTAs per tile, each with a piece of its key tiles.
+    const int splits = WINDOW && p.key_splits > 1 ? p.key_splits : 1;
+    const unsigned block = blockIdx.x / splits;
+    const int piece = blockIdx.x % splits;
     const int nblk = (p.Sq + kTiles * kTileQ - 1) / (kTiles * kTileQ);
     // Heavy (late) causal blocks first.  Large grids go head by head (a head's CTAs share K/V in L2 and the
     // last wave is made of light blocks); grids of a few waves go block-row by block-row over all heads, so
     // that no head's heavy blocks start in the last wave.
     const int64_t nbh = (int64_t)p.B * p.Hq;
     // (row by row also when all K/V of the call fit in half of L2: measured 4.6 % faster on 2048 CTAs)
-    const bool by_row = (int64_t)gridDim.x < KFA_ROW_MAJOR_LIMIT ||
+    const bool by_row = (int64_t)(gridDim.x / splits) < KFA_ROW_MAJOR_LIMIT ||
                         (int64_t)p.B * p.Hkv * p.Sk * D * 4 <= (int64_t(64) << 20);
-    const int qblk = nblk - 1 - (int)(by_row ? blockIdx.x / nbh : blockIdx.x % nblk);
-    const int64_t bh = by_row ? blockIdx.x % nbh : blockIdx.x / nblk;
+    const int qblk = nblk - 1 - (int)(by_row ? block / nbh : block % nblk);
+    const int64_t bh = by_row ? block % nbh : block / nblk;
     const int h = (int)(bh % p.Hq), b = (int)(bh / p.Hq);
     const int kvh = h / p.group;
     const int q0 = qblk * kTiles * kTileQ;
@@ -146,6 +150,7 @@ __global__ void __launch_bounds__(threads_of(WINDOW ? 1 : 2), WINDOW ? 2 : 1)
         } else if (WINDOW) {
             const int row_hi = min(p.Sq, row_lo + kTileQ);
             wt[t] = window_key_tiles(start, row_lo, row_hi, p.window, p.sinks, p.Sk);
+            if (splits > 1) wt[t] = window_piece(wt[t], piece, splits);
             lo_t[t] = window_span(start, row_lo, p.window, p.Sk).lo;
             hi_t[t] = window_span(start, row_hi - 1, p.window, p.Sk).hi;
             n_t[t] = wt[t].end;
@@ -211,6 +216,10 @@ __global__ void __launch_bounds__(threads_of(WINDOW ? 1 : 2), WINDOW ? 2 : 1)
 
     const bool dead = sh.abort_word != 0;  // set before the barrier above: skip straight to the tear-down
     if (dead) {
+        if (WINDOW && splits > 1) {  // (a cluster's CTAs stay to its barriers: the others read this one's part)
+            cluster_barrier();
+            cluster_barrier();
+        }
     } else if (warp >= kRoleWarp) {
       // registers move to the softmax warpgroups: (2 x 208 + 88) x 128 of 168 x 384, or (200 + 56) x 128 of 128 x 256
       if (kTiles == 2) reg_dealloc<88>();
@@ -378,6 +387,11 @@ __global__ void __launch_bounds__(threads_of(WINDOW ? 1 : 2), WINDOW ? 2 : 1)
             PH_FLUSH(2);
         }
       }
+      if (WINDOW && splits > 1) {
+          __syncwarp();
+          cluster_barrier();
+          cluster_barrier();
+      }
     } else {
         if (kTiles == 2) reg_alloc<208>();
         else reg_alloc<200>();
@@ -520,6 +534,87 @@ __global__ void __launch_bounds__(threads_of(WINDOW ? 1 : 2), WINDOW ? 2 : 1)
         }
         if ((threadIdx.x & 127) == 0) PH_FLUSH(t);
         // epilogue: wait for the last product, normalise, store
+        if (WINDOW && splits > 1) {
+            // The pieces' accumulators and (reference, sum, maximum), in place of the ring and the query tile, are merged
+            // in their order over distributed shared memory; each CTA writes its share of the rows.
+            float4* part_o = reinterpret_cast<float4*>(sKV);  // [128 rows][D / 4], chunks exchanged by the row
+            float4* part_ml = reinterpret_cast<float4*>(sQ);
+            static_assert(!WINDOW || kTileQ * D * 4 <= Cfg::kStages * Cfg::kTileBytes, "a tile's accumulator fits the ring");
+            constexpr int kChunks4 = D / 4;
+            if (iter > 0 && ok) ok = mbar_wait(&sh.s_ready[t], iter & 1, abort_word, 32 + t);
+            if (!ok) iter = 0;
+            if (__any_sync(0xffffffffu, iter > 0)) {  // (a piece's tiles are the same for all rows)
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t r[32];
+                    tmem_ld32(o_addr + c, r);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        part_o[row_in_tile * kChunks4 + (((c + i) / 4) ^ (row_in_tile & (kChunks4 - 1)))] =
+                            make_float4(__uint_as_float(r[i]), __uint_as_float(r[i + 1]), __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
+                }
+            }
+            part_ml[row_in_tile] = make_float4(iter > 0 ? m_used : -INFINITY, iter > 0 ? l : 0.f, iter > 0 ? m_true : -INFINITY, 0.f);
+            cluster_barrier();
+            auto merge = [&](auto pieces_) {
+                constexpr int S = decltype(pieces_)::value, kRows = kTileQ / S, kWarpRows = kRows / 4, kAtOnce = 32 / kChunks4;
+                using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+                for (int r4 = 0; r4 < kWarpRows; r4 += 4) {
+                    const int r0 = piece * kRows + (warp & 3) * kWarpRows + r4;
+                    // the weights of four rows' pieces: lane 8 row + piece
+                    const int from = lane & 7, r = r0 + (lane >> 3);
+                    float4 ml = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+                    if (from < S) ml = cluster_load4(cluster_address(part_ml + r, from));
+                    float m = ml.x, top = ml.z;
+#pragma unroll
+                    for (int o = 1; o < 8; o <<= 1) {
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    }
+                    // (a piece without a visible key has no accumulator either: weight zero, and nothing is loaded)
+                    float weight = ml.x == -INFINITY ? 0.f : ex2((ml.x - m) * c2), sum = ml.y * weight;
+#pragma unroll
+                    for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    weight *= sum > 0.f ? 1.f / sum : 0.f;
+                    if (from == 0 && q0 + r < p.Sq && p.maximum) {
+                        const int64_t si = ((int64_t)b * p.Hq + h) * p.Sq + q0 + r;
+                        p.maximum[si] = top;
+                        p.logsum[si] = sum > 0.f ? log2f(sum) + (m - top) * c2 : 0.f;
+                    }
+                    const int c = lane & (kChunks4 - 1);
+#pragma unroll(8 / S > 4 / kAtOnce ? 4 / kAtOnce : 8 / S)
+                    for (int i = 0; i < 4; i += kAtOnce) {
+                        const int mine = i + lane / kChunks4, row_at = r0 + mine;
+                        float4 x[S], acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                        float w[S];
+#pragma unroll
+                        for (int n = 0; n < S; ++n) {
+                            w[n] = __shfl_sync(0xffffffffu, weight, 8 * mine + n);
+                            x[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (w[n] != 0.f)
+                                x[n] = cluster_load4(cluster_address(part_o + row_at * kChunks4 + (c ^ (row_at & (kChunks4 - 1))), n));
+                        }
+#pragma unroll
+                        for (int n = 0; n < S; ++n) {
+                            acc.x = fmaf(x[n].x, w[n], acc.x), acc.y = fmaf(x[n].y, w[n], acc.y);
+                            acc.z = fmaf(x[n].z, w[n], acc.z), acc.w = fmaf(x[n].w, w[n], acc.w);
+                        }
+                        if (q0 + row_at < p.Sq && c * 4 < p.D) {
+                            T* to = reinterpret_cast<T*>(p.out) + (int64_t)b * p.os[0] + (int64_t)h * p.os[1] +
+                                    (int64_t)(q0 + row_at) * p.os[2] + c * 4;
+                            *reinterpret_cast<uint2*>(to) = make_uint2(pack2<BF16>(acc.x, acc.y), pack2<BF16>(acc.z, acc.w));
+                        }
+                    }
+                }
+            };
+            if (splits == 2) merge(std::integral_constant<int, 2>{});
+            else if (splits == 4) merge(std::integral_constant<int, 4>{});
+            else merge(std::integral_constant<int, 8>{});
+            cluster_barrier();  // nobody leaves while its part is read
+            iter = -1;          // (nothing is left to write)
+        }
         if (ok && iter == 0 && row < p.Sq && (WINDOW || n_t[t] > 0) && !p.running) {
             // every key tile of this row is hidden: zero output, empty statistics
             using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
@@ -645,6 +740,23 @@ cudaError_t launch_t(const AttnParams& p, cudaStream_t st) {
     else if (!encode_bhsd_map(&maps.o, p.out, dt, p.D, p.Sq, p.Hq, p.B, p.os, 64, kTileQ))
         return cudaErrorInvalidValue;
     const int64_t grid = (int64_t)((p.Sq + tiles * kTileQ - 1) / (tiles * kTileQ)) * p.B * p.Hq;
+    const int splits = p.window > 0 ? window_key_splits(p) : 1;
+    if (splits > 1) {
+        AttnParams split = p;
+        split.key_splits = splits;
+        cudaLaunchConfig_t config = {};
+        config.gridDim = dim3((unsigned)(grid * splits));
+        config.blockDim = dim3(threads_of(tiles));
+        config.dynamicSmemBytes = smem_bytes;
+        config.stream = st;
+        cudaLaunchAttribute together[1];
+        together[0].id = cudaLaunchAttributeClusterDimension;
+        together[0].val.clusterDim.x = (unsigned)splits;
+        together[0].val.clusterDim.y = together[0].val.clusterDim.z = 1;
+        config.attrs = together;
+        config.numAttrs = 1;
+        return cudaLaunchKernelEx(&config, kernel, maps, split);
+    }
     kernel<<<(unsigned)grid, threads_of(tiles), smem_bytes, st>>>(maps, p);
     return cudaGetLastError();
 }

@@ -57,6 +57,21 @@ __host__ __device__ __forceinline__ WindowTiles window_key_tiles(int64_t start, 
     return t;
 }
 
+// Piece `piece` of `pieces` of these tiles, in equal parts; the sinks' tiles all belong to the first.
+__host__ __device__ __forceinline__ WindowTiles window_piece(const WindowTiles& all, int piece, int pieces) {
+    const int window = all.end - all.first, total = all.sink_end + window;
+    auto before = [&](int i) {  // window tiles of the pieces before i
+        const int n = (int)((int64_t)total * i / pieces) - all.sink_end;
+        return i == 0 || n < 0 ? 0 : n;
+    };
+    WindowTiles t;
+    t.sink_end = piece == 0 ? all.sink_end : 0;
+    t.first = all.first + before(piece);
+    t.end = all.first + before(piece + 1);
+    if (t.first == t.end) t.first = t.end = t.sink_end;
+    return t;
+}
+
 // The 128-row query tiles [first, end) that hold a row which sees one of the keys [key0, key1), key1 <= Sk.  A tile in
 // between may hold no such row when the range of keys has sinks at its head; its scores are hidden one by one then.
 struct WindowRange {
@@ -70,6 +85,20 @@ __host__ __device__ __forceinline__ WindowRange window_query_tiles(int64_t start
     r1 = r1 > Sq ? Sq : r1;
     if (r0 >= r1) return WindowRange{0, 0};
     return WindowRange{(int)(r0 >> 7), (int)((r1 + 127) >> 7)};
+}
+
+// CTAs per query tile of the tensor-memory forward (1: no cluster).  Where the tiles leave most SMs empty, a cluster of
+// two, four or eight shares a tile's keys: at most one CTA per SM, or two (nine tenths of the places, which clusters
+// have to find) where that makes four and more.  Times in a graph, D 128, by batch, heads, rows, window, one CTA -> a
+// cluster: 1 8 512 1024: 22.9 -> 14.6 us (four); 8 8 40 2048: 36.4 -> 23.4 (four); 1 64 64 4096: 62.7 -> 31.6 (four);
+// left alone: 16 8 33 1000: 24.2 -> 25.7 (two, two per SM); 2 8 1000 300, four key tiles: 17.7 -> 21.1 (two).
+inline int window_key_splits(const AttnParams& p) {
+    const int64_t tiles = (int64_t)p.B * p.Hq * ((p.Sq + 127) / 128);
+    const int64_t keys = (p.window < p.Sk ? p.window : p.Sk) / 128 + 1 + (p.sinks + 127) / 128;
+    int splits = 1;
+    for (int more = 2; more <= 8; more *= 2)
+        if (keys >= (more == 8 ? 20 : more + 6) && (tiles * more <= 148 || (more >= 4 && tiles * more <= 266))) splits = more;
+    return splits;
 }
 
 }  // namespace kfa

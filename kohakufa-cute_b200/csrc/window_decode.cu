@@ -34,12 +34,11 @@ CacheAttentionCall call_of(const AttnParams& p) {
 
 // Up to 16 query rows per K/V head, a unit reads its keys once and nothing beats that.  More rows come in pieces of 16,
 // each of which reads the window of all rows; the tensor-memory forward has a CTA per head and 128 rows, which reads that
-// of its own.  About 155 (D 128; 220 at D 64) units cost what a wave of 296 such CTAs does for the same keys, also where
-// the wave is not full, since units spread over idle SMs and a CTA does not.  Times in a graph, tensor-memory forward ->
-// this, D 128, by batch, query / K/V heads, rows, window: 1 64/8 4 4096: 62 -> 21 us; 16 64/8 4 4096: 299 -> 83;
-// 48 64/8 8 1024: 282 -> 165; 1 8/1 33 1024: 22 -> 12; 1 8/2 256 4096 (0.85 of the rule's bound): 62 -> 52; 4 8/8 64
-// 2048 (0.83): 36 -> 29; kept there: 4 16/8 33 2048 (1.03): 36 -> 36; 8 8/8 40 2048 (1.2): 36 -> 40; 16 32/8 16 1000
-// (1.6): 52 -> 59.  D 64: 16 64/8 4 1024: 88 -> 23; 4 16/8 33 2048 (0.73): 33 -> 24.
+// of its own.  About 155 units (D 128; 220 at D 64) cost what a wave of 296 such CTAs does for the same keys, also where
+// the wave is not full, since units spread over idle SMs and a CTA does not; about 65 (95) where clusters share a tile's
+// keys there.  Times in a graph, tensor-memory forward -> this, D 128, by batch, query / K/V heads, rows, window:
+// 16 64/8 4 4096: 299 -> 83 us; 48 64/8 8 1024: 282 -> 165; 8 16/8 16 2048: 36 -> 29; 1 8/1 33 1024: 15 -> 12; kept
+// there: 1 64/8 33 4096: 32 -> 50; 16 32/8 16 1000: 52 -> 59.  D 64: 16 64/8 4 1024: 88 -> 23.
 bool window_decode_shape(const AttnParams& p) {
     if (p.D != 64 && p.D != 128) return false;
     const int64_t rows = (int64_t)p.Sq * p.group;
@@ -47,7 +46,8 @@ bool window_decode_shape(const AttnParams& p) {
         const int64_t seen = p.window < p.Sk ? p.window : p.Sk;
         const double units = (double)p.B * p.Hkv * (double)((rows + 15) / 16);
         const double waves = (double)(((int64_t)p.B * p.Hq * ((p.Sq + 127) / 128) + 295) / 296);
-        if (units * (double)(seen + p.Sq) > (p.D == 128 ? 155. : 220.) * waves * (double)(seen + (p.Sq < 128 ? p.Sq : 128))) return false;
+        const double wave = window_key_splits(p) > 1 ? (p.D == 128 ? 65. : 95.) : (p.D == 128 ? 155. : 220.);
+        if (units * (double)(seen + p.Sq) > wave * waves * (double)(seen + (p.Sq < 128 ? p.Sq : 128))) return false;
     }
     const CacheAttentionCall c = call_of(p);
     return p.D == 128 ? rows::countable<128, false>(c) : rows::countable<64, false>(c);

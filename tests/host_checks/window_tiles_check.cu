@@ -53,6 +53,17 @@ int main() {
                                 walked[j] = 1;
                                 last = j;
                             }
+                            for (int pieces : {2, 4, 8}) {  // one after the other, they walk the same tiles
+                                int j = keys[tq].begin();
+                                for (int piece = 0; piece < pieces; ++piece) {
+                                    const kfa::WindowTiles part = kfa::window_piece(keys[tq], piece, pieces);
+                                    for (int i = part.begin(); i < part.end; i = part.next(i)) {
+                                        if (i != j || !part.has(i)) return 7;
+                                        j = keys[tq].next(j);
+                                    }
+                                }
+                                if (j < keys[tq].end) return 8;
+                            }
                             for (int tk = 0; tk < nk; ++tk) {
                                 if (walked[tk] != keys[tq].has(tk) || walked[tk] < needed[tq * nk + tk]) {
                                     std::printf("key tiles: Sq %d Sk %d start %lld window %lld sinks %d tile %d %d\n", Sq, Sk,

@@ -260,6 +260,37 @@ def test_one_new_token_against_a_long_cache():
     assert native().device_status(reset=True) == 0
 
 
+@pytest.mark.parametrize("case", (
+    # few query tiles, so that a cluster shares a tile's keys:  B, Hq, Hkv, Sq, Sk, D, window, sinks
+    (1, 2, 1, 128, 5000, 128, 3000, 4),      # eight CTAs a tile
+    (1, 2, 2, 200, 3001, 64, 10000, 300),    # sinks over three key tiles, a query tile that is not full
+    (2, 4, 2, 300, 1500, 96, 900, 0),        # channels that the tile pads
+    (1, 4, 4, 1000, 1000, 128, 1000, 1),     # tiles at the start see fewer keys than there are CTAs
+    (3, 6, 1, 640, 2000, 80, 700, 130),      # two CTAs a tile
+))
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+def test_few_query_tiles_share_their_keys(case, dtype):
+    B, Hq, Hkv, Sq, Sk, D, window, sinks = case
+    q, k, v, dout = make_inputs(B, Hq, Hkv, Sq, Sk, D, dtype, seed=Sk)
+    for start in (Sk - Sq, 0, Sk - Sq // 2):
+        call = dict(window=window, sinks=sinks, query_start=start)
+        got = run_attention(api().sliding_window_attention, q, k, v, dout, **call)
+        check(got, q, k, v, dout, window_mask([start], Sq, Sk, window, sinks), None)
+        again = run_attention(api().sliding_window_attention, q, k, v, dout, **call)
+        assert all(torch.equal(a, b) for a, b in zip(got, again))
+    at = torch.tensor([-Sq - 5, Sk // 2, Sk - 3][:B], dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        got = api().sliding_window_attention(q, k, v, window=window, sinks=sinks, query_start=at)
+    mask = window_mask(at.tolist(), Sq, Sk, window, sinks)
+    want = ao.math_reference([t.cpu() for t in (q, k, v)], dout.cpu(), mask, False, None)[0]
+    for b in range(B):
+        if mask[b].any():
+            assert ao.per_head_relative_error(got[b:b + 1].cpu(), want[b:b + 1]) < TOL[dtype]["norm"]
+    blind = ~mask.any(-1).expand(B, Hq, Sq)
+    assert float(got.cpu()[blind].abs().sum()) == 0
+    assert native().device_status(reset=True) == 0
+
+
 def test_layouts_give_the_same_result():
     B, Hq, Hkv, S, D, window, sinks = 2, 4, 2, 333, 64, 77, 4
     q, k, v, dout = make_inputs(B, Hq, Hkv, S, S, D, torch.bfloat16, seed=2)
