@@ -103,7 +103,7 @@ __device__ __forceinline__ int key_tile_state(const AttnParams& p, int b, int h,
 // MASKED = false is the instantiation for calls without a mask (the flag is cleared at compile time).
 // WINDOW is the instantiation for sliding-window calls (window.cuh; neither a mask nor `causal` then): a query tile
 // walks the key tiles of the sinks and of its window, two tiles of a CTA need not see the same ones, and positions
-// come from device memory where the call gives one per sequence.
+// come from device memory where the call gives one per sequence.  With `key_splits` a cluster of CTAs shares a tile's keys.
 template <int D, bool BF16, bool MASKED, bool WINDOW>
 __global__ void __launch_bounds__(threads_of(WINDOW ? 1 : 2), WINDOW ? 2 : 1)
     pipeline_forward(const __grid_constant__ FwdMaps maps, AttnParams p) {

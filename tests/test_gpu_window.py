@@ -305,6 +305,29 @@ def test_layouts_give_the_same_result():
         assert torch.equal(a, b) and torch.equal(a, c)
 
 
+def test_captured_clusters_follow_new_positions():
+    B, Hq, Hkv, Sq, Sk, D, window, sinks = 2, 4, 2, 200, 3000, 128, 2000, 4  # sixteen query tiles of eight CTAs
+    q, k, v, _ = make_inputs(B, Hq, Hkv, Sq, Sk, D, torch.bfloat16, seed=8)
+    at = torch.tensor([2500, 20], dtype=torch.int32, device="cuda")
+    q.requires_grad_()
+    with torch.no_grad():
+        api().sliding_window_attention(q, k, v, window=window, sinks=sinks, query_start=at)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = api().sliding_window_attention(q, k, v, window=window, sinks=sinks, query_start=at)
+        for positions in ([2500, 20], [0, 2800], [-500, 1400]):
+            at.copy_(torch.tensor(positions, dtype=torch.int32))
+            graph.replay()
+            want = api().sliding_window_attention(q, k, v, window=window, sinks=sinks, query_start=at)
+            assert torch.equal(out, want)
+            mask = window_mask(positions, Sq, Sk, window, sinks)
+            exact = ao.math_reference([t.detach().cpu() for t in (q, k, v)], q.detach().cpu(), mask, False, None)[0]
+            for b in range(B):
+                if mask[b].any():
+                    assert ao.per_head_relative_error(out[b:b + 1].cpu(), exact[b:b + 1]) < TOL[torch.bfloat16]["norm"]
+    assert native().device_status(reset=True) == 0
+
+
 @pytest.mark.parametrize("Sq", (1, 300))
 def test_captured_calls_follow_new_positions(Sq):
     B, Hq, Hkv, Sk, D, window, sinks = 3, 8, 2, 800, 128, 200, 4
