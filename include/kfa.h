@@ -261,7 +261,7 @@ KFA_API int kfa_window_backward(const kfa_tensor* q, const kfa_tensor* k, const 
  *   codes  uint8 [B,H,capacity,D/2]     byte i of a row: channels 2i (low half) and 2i+1 (high half)
  *   params 16-bit type [B,H,capacity,D/64,2]   per group of 64 channels: (scale, zero); value = zero + scale * code
  * D is a multiple of 64 up to 512.  Strides are free except that the last axis of codes and the last two of params are
- * dense and every row starts on a 16-byte (codes) / 4*(D/64)-byte (params) boundary.
+ * dense and every row starts on a 16-byte (codes) / 4-byte (params) boundary; attention at D = 128 wants params on 8 bytes.
  *
  * kfa_cache_write quantises k, v [B,H,n,D] (16-byte addressable rows) into the rows start_b + r, r < lengths[b]
  * (lengths NULL: all n): scale = round16((max - min) / 15), zero = min, code = round_half_even((x - zero) / scale).  A

@@ -1247,9 +1247,11 @@ int kfa_window_backward(const kfa_tensor* q, const kfa_tensor* k, const kfa_tens
 
 namespace {
 
-// One half of a 4-bit cache (format: quantized_cache.cuh) against the first half's shape.
+// One half of a 4-bit cache (format: quantized_cache.cuh) against the first half's shape.  `at_once`: how many of a
+// token's (scale, zero) pairs the kernels address in one access (4 bytes each), which the params' rows have to be
+// aligned to: one where rows are written or read back, all of a token's for attention.
 int fill_cache_half(kfa::CacheView& view, const kfa_tensor* codes, const kfa_tensor* params, const kfa_tensor* like,
-                    int dtype) {
+                    int dtype, int64_t at_once) {
     if (!codes || !params || !codes->data || !params->data || codes->dtype != KFA_U8 || codes->ndim != 4 ||
         params->ndim != 5 || params->dtype != dtype)
         return fail(KFA_INVALID_ARGUMENT,
@@ -1267,14 +1269,15 @@ int fill_cache_half(kfa::CacheView& view, const kfa_tensor* codes, const kfa_ten
     if (params->sizes[3] != groups || params->sizes[4] != 2)
         return fail(KFA_INVALID_ARGUMENT, "quantized cache: params do not match the codes");
     bool ok = codes->strides[3] == 1 && reinterpret_cast<uintptr_t>(codes->data) % 16 == 0 && params->strides[4] == 1 &&
-              (groups == 1 || params->strides[3] == 2) && reinterpret_cast<uintptr_t>(params->data) % (4 * groups) == 0;
+              (groups == 1 || params->strides[3] == 2) && reinterpret_cast<uintptr_t>(params->data) % (4 * at_once) == 0;
     for (int i = 0; i < 3; ++i) {
         view.cs[i] = codes->strides[i];
         view.ps[i] = params->strides[i];
-        if (codes->sizes[i] > 1) ok = ok && view.cs[i] % 16 == 0 && view.ps[i] % (2 * groups) == 0;
+        if (codes->sizes[i] > 1) ok = ok && view.cs[i] % 16 == 0 && view.ps[i] % (2 * at_once) == 0;
     }
     if (!ok)
-        return fail(KFA_INVALID_ARGUMENT, "quantized cache: rows must be dense and aligned (codes 16 bytes, params one token)");
+        return fail(KFA_INVALID_ARGUMENT,
+                    "quantized cache: rows must be dense and aligned (codes to 16 bytes, params to %d bytes)", (int)(4 * at_once));
     view.codes = static_cast<uint8_t*>(codes->data);
     view.params = static_cast<uint16_t*>(params->data);
     return 0;
@@ -1311,8 +1314,8 @@ int fill_cache_call(kfa::CacheCall& p, const kfa_tensor* k, const kfa_tensor* v,
     if (int e = check_cache_rows(v, k_codes)) return e;
     if (!same_shape(k, v) || k->dtype != v->dtype)
         return fail(KFA_INVALID_ARGUMENT, "quantized cache requires K and V rows of one shape and type");
-    if (int e = fill_cache_half(p.half[0], k_codes, k_params, k_codes, k->dtype)) return e;
-    if (int e = fill_cache_half(p.half[1], v_codes, v_params, k_codes, k->dtype)) return e;
+    if (int e = fill_cache_half(p.half[0], k_codes, k_params, k_codes, k->dtype, 1)) return e;
+    if (int e = fill_cache_half(p.half[1], v_codes, v_params, k_codes, k->dtype, 1)) return e;
     p.B = (int)k->sizes[0];
     p.H = (int)k->sizes[1];
     p.n = (int)k->sizes[2];
@@ -1409,8 +1412,8 @@ int kfa_cache_attention(const kfa_tensor* q, const kfa_tensor* k_codes, const kf
     if (int e = check_device_ok()) return e;
     kfa::CacheAttentionCall p;
     if (int e = fill_cache_attention(p, q, k_codes, window, sinks)) return e;
-    if (int e = fill_cache_half(p.half[0], k_codes, k_params, k_codes, q->dtype)) return e;
-    if (int e = fill_cache_half(p.half[1], v_codes, v_params, k_codes, q->dtype)) return e;
+    if (int e = fill_cache_half(p.half[0], k_codes, k_params, k_codes, q->dtype, p.D / 64)) return e;
+    if (int e = fill_cache_half(p.half[1], v_codes, v_params, k_codes, q->dtype, p.D / 64)) return e;
     if (int e = check_positions(starts, p.B, "starts", start)) return e;
     if (int e = check_like(out, q, "out")) return e;
     for (const kfa_tensor* t : {q, static_cast<const kfa_tensor*>(out)}) {

@@ -463,3 +463,50 @@ def test_refusals():
         write(cache._replace(k_codes=shifted), k, k)
     assert all(not t.any() for t in cache)
     assert native().device_status(reset=True) == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", (192, 320, 384, 448, 128))
+def test_params_may_start_at_any_pair(D, dtype):
+    """Rows of any number of groups, wherever the allocator puts the params: their bases at successive multiples of 512
+    bytes, as torch allocates, and in between.  Written bits and what is read back equal the definition."""
+    B, H, n, capacity = 2, 2, 21, 30
+    k, v = rows(B, H, n, D, dtype=dtype, seed=D), rows(B, H, n, D, dtype=dtype, seed=D + 1, offset=False)
+    shape, size = (B, H, capacity, D // 64, 2), B * H * capacity * (D // 64) * 2
+    want = [quantise(x) for x in (k, v)]
+    wide = [torch.zeros(B, H, capacity, D // 2, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    for at in (0, 256, 512, 768, 1024, 1280, 1536, 2, 6, 1030):  # 16-bit elements
+        store = [torch.zeros(size + 2048, dtype=dtype, device="cuda") for _ in range(2)]
+        assert all(t.data_ptr() % 512 == 0 for t in store)
+        params = [t[at + 2 * i:at + 2 * i + size].view(shape) for i, t in enumerate(store)]
+        cache = api().QuantizedCache(wide[0], params[0], wide[1], params[1])
+        api().quantized_cache_write(cache, k, v, start=4)
+        got = api().quantized_cache_read(cache, start=4, length=n)
+        for (want_codes, want_params), codes, held, half in zip(want, wide, params, got):
+            assert torch.equal(codes[:, :, 4:n + 4].cpu(), want_codes) and torch.equal(held[:, :, 4:n + 4].cpu(), want_params)
+            u, exact = torch.finfo(dtype).eps / 2, values(want_codes, want_params)
+            assert bool(((half.cpu().double() - exact).abs() <= (u + 2**-22) * exact.abs() + torch.finfo(dtype).tiny).all())
+        for i, t in enumerate(store):  # nothing around them was written
+            assert not t[:at + 2 * i].any() and not t[at + 2 * i + size:].any()
+    assert native().device_status(reset=True) == 0
+
+
+def test_attention_wants_a_tokens_params_in_one_piece():
+    """Attention copies a token's scales and zeros at once: 8 bytes at 128 channels, 4 at 64."""
+    for D, at, served in ((64, 2, True), (128, 4, True), (128, 2, False)):
+        B, H, capacity = 1, 2, 40
+        shape, size = (B, H, capacity, D // 64, 2), B * H * capacity * (D // 64) * 2
+        plain = filled(B, H, capacity, D, torch.bfloat16, seed=D)
+        moved = []
+        for held in (plain.k_params, plain.v_params):
+            store = torch.zeros(size + 64, dtype=torch.bfloat16, device="cuda")[at:at + size].view(shape)
+            moved.append(store.copy_(held))
+        cache = plain._replace(k_params=moved[0], v_params=moved[1])
+        assert all(torch.equal(a, b) for a, b in zip(api().quantized_cache_read(plain), api().quantized_cache_read(cache)))
+        q = rows(B, 4, 1, D, dtype=torch.bfloat16, seed=3)
+        if served:
+            want = api().quantized_cache_attention(q, plain, query_start=39)
+            assert torch.equal(want, api().quantized_cache_attention(q, cache, query_start=39))
+        else:
+            with pytest.raises(ValueError, match="aligned"):
+                api().quantized_cache_attention(q, cache, query_start=39)
