@@ -577,7 +577,9 @@ __global__ void __launch_bounds__(threads_of(WINDOW ? 1 : 2), WINDOW ? 2 : 1)
                     float weight = ml.x == -INFINITY ? 0.f : ex2((ml.x - m) * c2), sum = ml.y * weight;
 #pragma unroll
                     for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                    weight *= sum > 0.f ? 1.f / sum : 0.f;
+                    // (a sum that is not a number stays one: every weight of the row becomes NaN, and so does its output, as
+                    // where one CTA has all the keys)
+                    weight *= sum == 0.f ? 0.f : 1.f / sum;
                     if (from == 0 && q0 + r < p.Sq && p.maximum) {
                         const int64_t si = ((int64_t)b * p.Hq + h) * p.Sq + q0 + r;
                         p.maximum[si] = top;

@@ -419,3 +419,26 @@ def test_refusals():
     with pytest.raises(ValueError, match="int32"):
         native().window_forward(q, k, v, at[:1], 0, 4, 0, 0.1)
     assert native().device_status(reset=True) == 0
+
+
+def test_nan_stays_where_a_cluster_shares_the_keys():
+    """One CTA per query tile or a cluster of them: what is not a number stays visible in every row that sees it."""
+    q, k, v, _ = make_inputs(1, 2, 1, 128, 5000, 128, torch.bfloat16, seed=5)
+    q[0, 1, 7, 30] = float("nan")     # a whole row of one head
+    k[0, 0, 3000, 5] = float("nan")   # seen by the rows from position 3000 to 4999
+    v[0, 0, 4000, 9] = float("inf")   # a channel of the rows that see it
+    start, window = 4800, 1900        # rows at 4800 .. 4927, windows from 2901 .. 3028 on
+    k_seen = (4800 + torch.arange(128)) - window < 3000
+    with torch.no_grad():
+        got = api().sliding_window_attention(q, k, v, window=window, sinks=4, query_start=start).cpu()
+    leaf = q.clone().requires_grad_(True)
+    kept = api().sliding_window_attention(leaf, k, v, window=window, sinks=4, query_start=start).detach().cpu()
+    for out in (got, kept):
+        assert bool(torch.isnan(out[0, 1, 7]).all())
+        assert bool(torch.isnan(out[0, :, k_seen]).all())
+        rest = ~k_seen
+        rest[7] = False
+        assert bool((~torch.isfinite(out[0, :, rest][..., 9])).all())
+        others = [c for c in range(128) if c != 9]
+        assert bool(torch.isfinite(out[0, :, rest][..., others]).all())
+    assert native().device_status(reset=True) == 0
