@@ -2,7 +2,8 @@
 
 Like the attention operator (``_ops.py``): eager calls use a ``torch.autograd.Function`` (least host overhead), calls
 under ``torch.compile`` the ``kohakufa_cute::window_forward`` / ``window_backward`` custom operators.  Only O is
-differentiable, and only once; the two row statistics are saved outputs.
+differentiable, and only once; the two row statistics are saved outputs.  Calls that nobody differentiates keep none
+(``kohakufa_cute::window_inference`` under ``torch.compile``): only these reach the decoding kernels, which form none.
 """
 
 from typing import Optional
@@ -24,6 +25,19 @@ def forward(
 def _forward_fake(q, k, v, starts, start, window, sinks, scale):
     stats = torch.empty(q.shape[:-1], device=q.device, dtype=torch.float32)
     return torch.empty_like(q), stats, torch.empty_like(stats)
+
+
+@torch.library.custom_op("kohakufa_cute::window_inference", mutates_args=())
+def inference(
+    q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: Optional[torch.Tensor], start: int, window: int,
+    sinks: int, scale: float
+) -> torch.Tensor:
+    return native.window_forward(q, k, v, starts, start, window, sinks, scale, statistics=False)[0]
+
+
+@inference.register_fake
+def _inference_fake(q, k, v, starts, start, window, sinks, scale):
+    return torch.empty_like(q)
 
 
 @torch.library.custom_op("kohakufa_cute::window_backward", mutates_args=())
@@ -81,6 +95,8 @@ def attention(q, k, v, starts, start, window, sinks, scale):
     elif differentiated:
         raise ValueError("sliding_window_attention: gradients need one query_start (an int) for the whole batch.")
     if torch.compiler.is_compiling():
+        if not differentiated:
+            return inference(q, k, v, starts, start, window, sinks, scale)
         return forward(q, k, v, starts, start, window, sinks, scale)[0]
     if not differentiated:
         return native.window_forward(q, k, v, starts, start, window, sinks, scale, statistics=False)[0]

@@ -442,3 +442,31 @@ def test_nan_stays_where_a_cluster_shares_the_keys():
         others = [c for c in range(128) if c != 9]
         assert bool(torch.isfinite(out[0, :, rest][..., others]).all())
     assert native().device_status(reset=True) == 0
+
+
+def test_compiled_decoding_keeps_no_statistics():
+    """A compiled call that nobody differentiates is the eager one: the decoding kernels serve it."""
+    q, k, v, _ = make_inputs(3, 8, 2, 1, 600, 128, torch.bfloat16, seed=12)
+    at = torch.tensor([599, 3, 250], dtype=torch.int32, device="cuda")
+
+    def f(q, k, v, at):
+        return api().sliding_window_attention(q, k, v, window=200, sinks=4, query_start=at)
+
+    def decoded():
+        return native().launch_stats().get("window_decode", 0)
+
+    compiled = torch.compile(f, fullgraph=True, backend="aot_eager")
+    want = f(q, k, v, at)
+    for grad in (True, False):  # nothing requires a gradient; nothing is recorded
+        with torch.set_grad_enabled(grad):
+            before = decoded()
+            got = compiled(q if grad else q.clone().requires_grad_(True), k, v, at)
+            assert decoded() > before
+            assert torch.equal(got, want) and got.stride() == want.stride()
+    narrow = [t[..., :80] for t in make_inputs(2, 4, 2, 70, 300, 96, torch.float16, seed=13)[:3]]  # the tensor-memory forward
+
+    def g(q, k, v):
+        return api().sliding_window_attention(q, k, v, window=100, query_start=20, scale=0.2)
+
+    a, b = g(*narrow), torch.compile(g, fullgraph=True, backend="aot_eager")(*narrow)
+    assert torch.equal(a, b) and a.stride() == b.stride()
