@@ -252,6 +252,14 @@ __device__ __forceinline__ uint32_t centred(uint32_t w, const Bases& base) {
     return y;
 }
 
+// What probabilities relative to the maximum m weigh relative to the maximum `top`.  They are formed as 2^(s c2 - round(m
+// c2)), so that the weight takes the same rounded products: the references then cancel exactly, however large an offset all
+// scores share (with (m - top) c2 the parts of warps, CTAs and re-basings were off by up to ln 2 half steps of m c2 against
+// one another: 2 % at scores of 2^19).
+__device__ __forceinline__ float reference_weight(float m, float top, float c2) {
+    return m == -INFINITY ? 0.f : ex2(__fsub_rn(__fmul_rn(m, c2), __fmul_rn(top, c2)));
+}
+
 // ------------------------------------------------------------------ one unit's piece, one warp
 // Running state of a warp over its blocks: thread (g, i) = (lane / 4, lane % 4) holds the maximum of query rows 2i and
 // 2i + 1, its own part of their sums, and the accumulator of those rows at its channels (channel_of).
@@ -397,7 +405,7 @@ __device__ __forceinline__ void block_step(State<D, Q4, NT>& st, const uint8_t* 
             for (int e = 0; e < 2; ++e) {
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) mn[n][e] = fmaxf(mn[n][e], __shfl_xor_sync(0xffffffffu, mn[n][e], o));
-                const float alpha = st.m[n][e] == -INFINITY ? 0.f : ex2((st.m[n][e] - mn[n][e]) * c2);
+                const float alpha = reference_weight(st.m[n][e], mn[n][e], c2);
                 st.m[n][e] = mn[n][e];
                 st.l[n][e] *= alpha;
                 if (Q4) {
@@ -416,8 +424,8 @@ __device__ __forceinline__ void block_step(State<D, Q4, NT>& st, const uint8_t* 
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            // (the rounding of m c2 is the same factor in every probability of the row, and in their sum)
-            const float mc = !CLEAN && st.m[n][e] == -INFINITY ? 0.f : -st.m[n][e] * c2;
+            // (the rounding of m c2 is a factor that alpha and the merges' weights share: reference_weight)
+            const float mc = !CLEAN && st.m[n][e] == -INFINITY ? 0.f : -__fmul_rn(st.m[n][e], c2);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -753,7 +761,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                const float weight = sm_m[w][r] == -INFINITY ? 0.f : ex2((sm_m[w][r] - mx) * c2);
+                const float weight = reference_weight(sm_m[w][r], mx, c2);
                 const float4 x = *reinterpret_cast<const float4*>(sm_o + (w * R + r) * D + d);
                 sum += sm_l[w][r] * weight;
                 acc.x = fmaf(x.x, weight, acc.x), acc.y = fmaf(x.y, weight, acc.y);
@@ -808,7 +816,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, Q4, NT>()) decode_row
             }
 #pragma unroll
             for (int w = 0; w < kCluster; ++w) {
-                const float weight = ml[w].x == -INFINITY ? 0.f : ex2((ml[w].x - mx) * c2);
+                const float weight = reference_weight(ml[w].x, mx, c2);
                 sum += ml[w].y * weight;
                 acc.x = fmaf(x[w].x, weight, acc.x), acc.y = fmaf(x[w].y, weight, acc.y);
                 acc.z = fmaf(x[w].z, weight, acc.z), acc.w = fmaf(x[w].w, weight, acc.w);
@@ -863,7 +871,7 @@ __global__ void __launch_bounds__(1024) merge_rows(const RowsCall p) {
         const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + piece * 2);
         const float4 x = *reinterpret_cast<const float4*>(p.part_o + piece * D + d);
         const float m = fmaxf(mx, ml.x);
-        const float keep = mx == -INFINITY ? 0.f : ex2((mx - m) * c2), weight = ml.x == -INFINITY ? 0.f : ex2((ml.x - m) * c2);
+        const float keep = reference_weight(mx, m, c2), weight = reference_weight(ml.x, m, c2);
         mx = m;
         sum = sum * keep + ml.y * weight;
         acc.x = fmaf(x.x, weight, acc.x * keep), acc.y = fmaf(x.y, weight, acc.y * keep);
@@ -884,7 +892,7 @@ __global__ void __launch_bounds__(1024) merge_rows(const RowsCall p) {
         acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kParts; ++w) {
-            const float weight = sm_m[r][w] == -INFINITY ? 0.f : ex2((sm_m[r][w] - mx) * c2);
+            const float weight = reference_weight(sm_m[r][w], mx, c2);
             const float4 x = sm_o[r][w][lane];
             sum += sm_l[r][w] * weight;
             acc.x = fmaf(x.x, weight, acc.x), acc.y = fmaf(x.y, weight, acc.y);

@@ -510,3 +510,27 @@ def test_attention_wants_a_tokens_params_in_one_piece():
         else:
             with pytest.raises(ValueError, match="aligned"):
                 api().quantized_cache_attention(q, cache, query_start=39)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("capacity", (1000, 40000))  # one cluster; a line of blocks cut over all CTAs
+def test_a_large_common_score(capacity, dtype):
+    """Scores of about 2^20 that differ by a few units, integers throughout, so that every score is exact: warps and CTAs
+    have references of their own, and their parts are weighted alike.  Blocks of 64 tokens hold values that tell them
+    apart."""
+    gen = torch.Generator().manual_seed(capacity)
+    codes = [torch.randint(0, 256, (1, 1, capacity, 64), generator=gen).to(torch.uint8) for _ in range(2)]
+    params = [torch.ones(1, 1, capacity, 2, 2) for _ in range(2)]
+    codes[0][..., :32] = 0                      # keys: the first group is 256 throughout, the second 0 .. 15
+    params[0][..., 0, 1], params[0][..., 1, 1] = 256, 0
+    params[1][..., 0] = 2.0**-8                 # values: about 1, 2, 3, 4 by block
+    params[1][..., 1] = (torch.arange(capacity) // 64 % 4 + 1).view(1, 1, capacity, 1)
+    q = torch.zeros(1, 4, 1, 128)
+    q[..., :64] = 64
+    q[..., 64:70] = torch.randint(-1, 2, (1, 4, 1, 6), generator=gen)
+    cache = api().QuantizedCache(codes[0].cuda(), params[0].to(dtype).cuda(), codes[1].cuda(), params[1].to(dtype).cuda())
+    q = q.to(dtype).cuda()
+    want, bound = reference(q, cache, (capacity - 1,), 0, 0, 0.5)
+    got = api().quantized_cache_attention(q, cache, query_start=capacity - 1, scale=0.5)
+    assert bool(((got.cpu().double() - want).abs() <= bound).all())
+    assert native().device_status(reset=True) == 0

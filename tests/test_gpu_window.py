@@ -470,3 +470,27 @@ def test_compiled_decoding_keeps_no_statistics():
 
     a, b = g(*narrow), torch.compile(g, fullgraph=True, backend="aot_eager")(*narrow)
     assert torch.equal(a, b) and a.stride() == b.stride()
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("Sk", (400, 30000))  # one cluster; a line of blocks cut over all CTAs
+def test_decoding_with_a_large_common_score(Sk, dtype):
+    """Scores of about 2^20 that differ by a few units, small integers throughout, so that every score is exact: warps and
+    CTAs have references of their own, and their parts are weighted alike.  Blocks of 16 keys, which the warps take in
+    turn, hold values that tell them apart."""
+    D, Hq = 64, 4
+    gen = torch.Generator().manual_seed(Sk)
+    k = torch.randint(-2, 3, (1, 1, Sk, D), generator=gen).double()
+    q = torch.randint(-1, 2, (1, Hq, 1, D), generator=gen).double()
+    q[..., 8:] = 0
+    q[..., 0], k[..., 0] = 512, 2048
+    v = torch.randint(-1, 2, (1, 1, Sk, D), generator=gen).double() / 64 + (torch.arange(Sk) // 16 % 4 + 1).view(1, 1, Sk, 1)
+    q, k, v = (t.to(dtype).cuda() for t in (q, k, v))
+    with torch.no_grad():
+        got = api().sliding_window_attention(q, k, v, window=Sk, query_start=Sk - 1, scale=0.5)
+    s = q.cpu().double() @ k.cpu().double().transpose(-1, -2) * 0.5
+    prob, vd = torch.softmax(s, -1), v.cpu().double()
+    out, u = prob @ vd, 1.1 * torch.finfo(dtype).eps / 2
+    # the output's rounding and that of the probabilities; FP32 steps, on differences of scores, in the tenth
+    assert bool(((got.cpu().double() - out).abs() <= u * out.abs() + u * (prob @ vd.abs())).all())
+    assert native().device_status(reset=True) == 0
