@@ -580,7 +580,8 @@ def cache_attention(q, k_codes, k_params, v_codes, v_params, starts, start, wind
     lib = library()
     q = _plain(q)
     if not _all_rows_16_byte_addressable(q):
-        q = q.contiguous()
+        dense = q.clone(memory_format=torch.contiguous_format)
+        return _like(q, cache_attention(dense, k_codes, k_params, v_codes, v_params, starts, start, window, sinks, scale))
     device = q.device
     with _on(device):
         out = torch.empty_like(q)

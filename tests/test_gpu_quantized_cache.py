@@ -534,3 +534,21 @@ def test_a_large_common_score(capacity, dtype):
     got = api().quantized_cache_attention(q, cache, query_start=capacity - 1, scale=0.5)
     assert bool(((got.cpu().double() - want).abs() <= bound).all())
     assert native().device_status(reset=True) == 0
+
+
+def test_the_output_is_laid_out_like_the_queries():
+    """Also where the rows cannot be addressed as they are; the compiled route declares the same layout."""
+    B, Hq, Sq, D = 2, 4, 3, 64
+    cache = filled(B, 2, 200, D, torch.float16, seed=71)
+    odd = torch.zeros(B * Sq * Hq * D + 1, dtype=torch.float16, device="cuda")[1:].view(B, Sq, Hq, D).transpose(1, 2)
+    odd.copy_(rows(B, Hq, Sq, D, dtype=torch.float16, seed=72))
+
+    def f(q, cache):
+        out = api().quantized_cache_attention(q, cache, query_start=100, window=50, sinks=2)
+        return out, out.transpose(1, 2).view(B, Sq, Hq * D)
+
+    want = api().quantized_cache_attention(odd.contiguous(), cache, query_start=100, window=50, sinks=2)
+    for call in (f, torch.compile(f, fullgraph=True, backend="aot_eager")):
+        out, flat = call(odd, cache)
+        assert out.stride() == torch.empty_like(odd).stride() and torch.equal(out, want)
+        assert torch.equal(flat, want.transpose(1, 2).reshape(B, Sq, Hq * D))
