@@ -241,6 +241,11 @@ if _fast_records is not None:
     _all_rows_16_byte_addressable = _fast_records.addressable
 
 
+def _addressable_copy(t):
+    """A dense copy that starts on a boundary (``contiguous`` returns a dense tensor itself, wherever it starts)."""
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def _blocks_shape(q, k, mask):
     return (
         1 if mask.stride(0) == 0 else q.shape[0],
@@ -555,7 +560,7 @@ def cache_write(k, v, k_codes, k_params, v_codes, v_params, starts, lengths, sta
     lib = library()
     k, v = _plain(k), _plain(v)
     if not _all_rows_16_byte_addressable(k, v):
-        k, v = (t if _rows_16_byte_addressable(t) else t.contiguous() for t in (k, v))
+        k, v = (t if _rows_16_byte_addressable(t) else _addressable_copy(t) for t in (k, v))
     device = k.device
     with _on(device):
         keep, records = _records(k, v, k_codes, k_params, v_codes, v_params, starts, lengths)
@@ -580,8 +585,8 @@ def cache_attention(q, k_codes, k_params, v_codes, v_params, starts, start, wind
     lib = library()
     q = _plain(q)
     if not _all_rows_16_byte_addressable(q):
-        dense = q.clone(memory_format=torch.contiguous_format)
-        return _like(q, cache_attention(dense, k_codes, k_params, v_codes, v_params, starts, start, window, sinks, scale))
+        return _like(q, cache_attention(_addressable_copy(q), k_codes, k_params, v_codes, v_params, starts, start, window,
+                                        sinks, scale))
     device = q.device
     with _on(device):
         out = torch.empty_like(q)

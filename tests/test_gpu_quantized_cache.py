@@ -552,3 +552,18 @@ def test_the_output_is_laid_out_like_the_queries():
         out, flat = call(odd, cache)
         assert out.stride() == torch.empty_like(odd).stride() and torch.equal(out, want)
         assert torch.equal(flat, want.transpose(1, 2).reshape(B, Sq, Hq * D))
+
+
+def test_dense_rows_off_a_16_byte_boundary_are_taken():
+    """A contiguous view that starts at an odd element: nothing but its address differs."""
+    def shifted(x):
+        return torch.zeros(x.numel() + 1, dtype=x.dtype, device="cuda")[1:].view(x.shape).copy_(x)
+
+    k, v, q = (rows(2, H, 20, 64, dtype=torch.bfloat16, seed=s) for s, H in ((81, 2), (82, 2), (83, 4)))
+    cache, other = (api().quantized_cache(2, 2, 30, 64) for _ in range(2))
+    api().quantized_cache_write(cache, k, v, start=3)
+    api().quantized_cache_write(other, shifted(k), shifted(v), start=3)
+    assert all(torch.equal(a, b) for a, b in zip(cache, other))
+    few = q[:, :, :2].contiguous()
+    want = api().quantized_cache_attention(few, cache, query_start=20)
+    assert torch.equal(want, api().quantized_cache_attention(shifted(few), cache, query_start=20))
