@@ -198,7 +198,7 @@ struct WindowAttention : public torch::autograd::Function<WindowAttention> {
         std::memcpy(&scale, &call[3], sizeof(scale));
         const c10::cuda::CUDAGuard guard(q.device());
         Tensor dout = grads[0].resolve_conj().resolve_neg();
-        if (!addressable(dout)) dout = dout.contiguous();
+        if (!addressable(dout)) dout = dout.clone(at::MemoryFormat::Contiguous);  // (contiguous() keeps an odd address)
         const int type = half_type(q);
         Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
         const kfa_tensor rq = record(q, type), rk = record(k, type), rv = record(v, type), ro = record(out, type),

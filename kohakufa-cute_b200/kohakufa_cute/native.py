@@ -278,6 +278,14 @@ def _for_tensor_cores(tensors):
     return [t if _rows_16_byte_addressable(t) else t.contiguous() for t in tensors], D
 
 
+def _for_window(tensors):
+    """The same for windowed calls, with copies also of operands that are dense but start off a 16-byte boundary."""
+    tensors, _ = _for_tensor_cores(tensors)
+    if not _all_rows_16_byte_addressable(*tensors):
+        tensors = [t if _rows_16_byte_addressable(t) else _addressable_copy(t) for t in tensors]
+    return tensors
+
+
 def _like(original, result):
     """``result`` (possibly with extra channels) copied into a tensor laid out like ``original``, as the
     reference allocates its outputs (native.cpp:295,348)."""
@@ -518,7 +526,7 @@ def window_forward(q, k, v, starts, start, window, sinks, scale, statistics=True
     lib = library()
     q, k, v = _plain(q), _plain(k), _plain(v)
     originals = (q, k, v)
-    (q, k, v), _ = _for_tensor_cores([q, k, v])
+    q, k, v = _for_window([q, k, v])
     if any(a is not b for a, b in zip((q, k, v), originals)):
         out, maximum, logsum = window_forward(q, k, v, starts, start, window, sinks, scale, statistics)
         return _like(originals[0], out), maximum, logsum
@@ -540,7 +548,7 @@ def window_backward(q, k, v, out, maximum, logsum, dout, start, window, sinks, s
     lib = library()
     q, k, v, out, dout = (_plain(t) for t in (q, k, v, out, dout))
     originals = (q, k, v)
-    (q, k, v, dout, out), _ = _for_tensor_cores([q, k, v, dout, out])
+    q, k, v, dout, out = _for_window([q, k, v, dout, out])
     if any(a is not b for a, b in zip((q, k, v), originals)):
         grads = window_backward(q, k, v, out, maximum, logsum, dout, start, window, sinks, scale)
         return tuple(_like(o, g) for o, g in zip(originals, grads))

@@ -494,3 +494,29 @@ def test_decoding_with_a_large_common_score(Sk, dtype):
     # the output's rounding and that of the probabilities; FP32 steps, on differences of scores, in the tenth
     assert bool(((got.cpu().double() - out).abs() <= u * out.abs() + u * (prob @ vd.abs())).all())
     assert native().device_status(reset=True) == 0
+
+
+def test_dense_rows_off_a_16_byte_boundary_run_on_the_same_kernels():
+    """A contiguous view that starts at an odd element: the same results, and no launch of the CUDA-core kernels."""
+    def shifted(x):
+        return torch.zeros(x.numel() + 1, dtype=x.dtype, device="cuda")[1:].view(x.shape).copy_(x)
+
+    def step(tensors):
+        leaves = [t.detach().requires_grad_(True) for t in tensors[:3]]
+        out = api().sliding_window_attention(*leaves, window=90, sinks=3)
+        return out.detach(), *torch.autograd.grad(out, leaves, tensors[3])
+
+    aligned = make_inputs(1, 4, 2, 300, 300, 64, torch.float16, seed=15)
+    want = step(aligned)
+    before = native().launch_stats()
+    for which in (0, 1, 2, 3):
+        got = step([shifted(t) if i == which else t for i, t in enumerate(aligned)])
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+    with torch.no_grad():
+        q, k, v = (t[:, :, -1:].contiguous() if i == 0 else t for i, t in enumerate(aligned[:3]))
+        call = dict(window=90, query_start=299)
+        one = api().sliding_window_attention(q, k, v, **call)
+        for operands in ((shifted(q), k, v), (q, shifted(k), v), (q, k, shifted(v))):
+            assert torch.equal(one, api().sliding_window_attention(*operands, **call))
+    after = native().launch_stats()
+    assert all(after[name] == before.get(name, 0) for name in after if name.startswith("general"))
