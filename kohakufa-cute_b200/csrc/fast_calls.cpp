@@ -55,7 +55,8 @@ struct Unserved {};  // the Python layer has to take this call
 
 // ------------------------------------------------------------------ arguments
 bool plain(const Tensor& t) {
-    return t.is_cuda() && t.layout() == at::kStrided && !t.is_conj() && !t.is_neg() && !at::isTensorSubclassLike(t);
+    return t.is_cuda() && t.layout() == at::kStrided && !t.is_conj() && !t.is_neg() && !at::isTensorSubclassLike(t) &&
+           !t._fw_grad(0).defined();  // (a forward-mode tangent, which Python refuses)
 }
 
 const Tensor& tensor(PyObject* o) {

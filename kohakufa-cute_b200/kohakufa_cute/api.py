@@ -20,6 +20,7 @@ from functools import lru_cache
 from math import isfinite, prod
 
 import torch
+from torch.autograd import forward_ad
 
 from . import native
 
@@ -154,6 +155,14 @@ def _window_arguments(name, batch, device, window, sinks, query_start):
     return None, query_start
 
 
+def _no_tangent(name, *tensors):
+    """Raises ``ValueError`` for operands with forward-mode tangents: the kernels would drop them."""
+    if torch.compiler.is_compiling():
+        return
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"{name}: forward-mode differentiation is not supported.")
+
+
 def _resolved_scale(name, scale, head_dim):
     scale = head_dim**-0.5 if scale is None else float(scale)
     if not isfinite(scale) or abs(scale) > torch.finfo(torch.float32).max:
@@ -169,13 +178,14 @@ def sliding_window_attention(q, k, v, *, window, sinks=0, query_start=0, scale=N
     ``c < sinks``); a row that sees no key is zero.  ``query_start`` is an int (0: queries and keys start together, as
     in training), or an int32 ``[B]`` CUDA tensor with one position per sequence, read by the kernels (a captured
     graph can be replayed with new positions; any value is allowed, keys behind a sequence's last position may hold
-    anything).  Differentiable (once) with respect to Q, K and V when ``query_start`` is an int.
+    anything).  Differentiable (once, in reverse mode) with respect to Q, K and V when ``query_start`` is an int.
     """
     if native.fast is not None and not torch.compiler.is_compiling():
         out = native.fast.window_attention(q, k, v, window, sinks, query_start, scale)
         if out is not None:
             return out
     _check_arguments(q, k, v, None, 0.0, False, True)
+    _no_tangent("sliding_window_attention", q, k, v)
     starts, start = _window_arguments("sliding_window_attention", q.shape[0], q.device, window, sinks, query_start)
     scale = _resolved_scale("sliding_window_attention", scale, q.shape[-1])
     from . import window_ops

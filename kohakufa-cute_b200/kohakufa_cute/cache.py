@@ -11,7 +11,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import native
-from .api import _HALF_TYPES, _device_supported, _resolved_scale, _window_arguments
+from .api import _HALF_TYPES, _device_supported, _no_tangent, _resolved_scale, _window_arguments
 
 GROUP = 64
 
@@ -71,6 +71,7 @@ def _positions(name, what, value, batch, device):
 def _no_gradient(name, *tensors):
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise ValueError(f"{name}: inference only; the operands must not require gradients.")
+    _no_tangent(name, *tensors)
 
 
 @torch.library.custom_op("kohakufa_cute::quantized_cache_write",

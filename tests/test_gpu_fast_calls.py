@@ -193,3 +193,31 @@ def test_a_report_of_a_wait_that_ran_out_reaches_both_directions(counted):
         native().device_status(reset=True)
     torch.autograd.grad(api().sliding_window_attention(q, q, q, window=20).sum(), q)
     assert native().device_status() == 0
+
+
+def test_forward_mode_is_refused_both_ways(counted, monkeypatch):
+    """A tangent would be dropped: an error instead, also where nothing requires a gradient."""
+    forward_ad = torch.autograd.forward_ad
+    q, k, v = (rows(1, 2, 100, 64, seed=s) for s in (1, 2, 3))
+    cache = api().quantized_cache(1, 2, 100, 64)
+    calls = (lambda q, k, v: api().sliding_window_attention(q, k, v, window=9),
+             lambda q, k, v: api().quantized_cache_write(cache, k, v),
+             lambda q, k, v: api().quantized_cache_attention(q[:, :, :2], cache, query_start=98))
+
+    def dual():
+        with forward_ad.dual_level():
+            for n, call in enumerate(calls):
+                for which in ((0, 1, 2), (1, 2), (0,))[n]:
+                    operands = [q, k, v]
+                    operands[which] = forward_ad.make_dual(operands[which], torch.ones_like(q))
+                    with pytest.raises(ValueError, match="forward-mode"):
+                        call(*operands)
+                    operands[which] = forward_ad.make_dual(operands[which].detach().requires_grad_(), torch.ones_like(q))
+                    with pytest.raises(ValueError, match="forward-mode|gradients"):
+                        call(*operands)
+                call(q, k, v)  # (without a tangent)
+        with pytest.raises(ValueError, match="forward-mode"):
+            torch.func.jvp(lambda q: calls[0](q, k, v), (q,), (torch.ones_like(q),))
+
+    dual()
+    without(monkeypatch, dual)
