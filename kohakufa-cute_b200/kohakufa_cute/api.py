@@ -27,6 +27,7 @@ from . import native
 _native_sdpa = torch.nn.functional.scaled_dot_product_attention
 _HALF_TYPES = (torch.float16, torch.bfloat16)
 _SUPPORTED_CAPABILITY = (10, 0)
+_LONGEST = 2**40  # positions end at 2^32
 
 
 def _device_supported(device):
@@ -163,6 +164,11 @@ def _no_tangent(name, *tensors):
         raise ValueError(f"{name}: forward-mode differentiation is not supported.")
 
 
+def _in_64_bits(window, sinks):
+    """The two as the library takes them: beyond every position, longer is the same (an integer may have any length)."""
+    return min(window, _LONGEST), min(sinks, _LONGEST)
+
+
 def _resolved_scale(name, scale, head_dim):
     scale = head_dim**-0.5 if scale is None else float(scale)
     if not isfinite(scale) or abs(scale) > torch.finfo(torch.float32).max:
@@ -190,7 +196,7 @@ def sliding_window_attention(q, k, v, *, window, sinks=0, query_start=0, scale=N
     scale = _resolved_scale("sliding_window_attention", scale, q.shape[-1])
     from . import window_ops
 
-    return window_ops.attention(q, k, v, starts, start, window, sinks, scale)
+    return window_ops.attention(q, k, v, starts, start, *_in_64_bits(window, sinks), scale)
 
 
 def neighborhood_attention(q, k, v, *, spatial_shape, window_size, scale=None):

@@ -11,7 +11,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import native
-from .api import _HALF_TYPES, _device_supported, _no_tangent, _resolved_scale, _window_arguments
+from .api import _HALF_TYPES, _device_supported, _in_64_bits, _no_tangent, _resolved_scale, _window_arguments
 
 GROUP = 64
 
@@ -203,7 +203,7 @@ def quantized_cache_attention(q, cache, *, query_start, window=None, sinks=0, sc
         raise ValueError(f"{name}: sinks need a window.")
     starts, at = _window_arguments(name, q.shape[0], q.device, 1 if window is None else window, sinks, query_start)
     scale = _resolved_scale(name, scale, q.shape[3])
-    arguments = (q, *cache, starts, at, 0 if window is None else window, sinks, scale)
+    arguments = (q, *cache, starts, at, *_in_64_bits(0 if window is None else window, sinks), scale)
     if torch.compiler.is_compiling():
         return _attention_op(*arguments)
     return native.cache_attention(*arguments)

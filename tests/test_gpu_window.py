@@ -520,3 +520,22 @@ def test_dense_rows_off_a_16_byte_boundary_run_on_the_same_kernels():
             assert torch.equal(one, api().sliding_window_attention(*operands, **call))
     after = native().launch_stats()
     assert all(after[name] == before.get(name, 0) for name in after if name.startswith("general"))
+
+
+def test_windows_and_sinks_of_any_size():
+    """Integers of any size: beyond 64 bits they are as long as the sequence, not what is left of them in 64 bits."""
+    q, k, v, dout = make_inputs(1, 4, 2, 130, 200, 64, torch.bfloat16, seed=14)
+    f = api().sliding_window_attention
+    for window, sinks, same in ((2**64 + 5, 0, dict(window=1000, sinks=0)), (5, 2**64, dict(window=5, sinks=200)),
+                                (2**63, 2**70 + 3, dict(window=1000, sinks=200)), (2**62, 2**62, dict(window=1000, sinks=200))):
+        call = dict(window=window, sinks=sinks)
+        want = run_attention(f, q, k, v, dout, query_start=60, **same)
+        assert all(torch.equal(a, b) for a, b in zip(want, run_attention(f, q, k, v, dout, query_start=60, **call)))
+        compiled = torch.compile(lambda q, k, v: f(q, k, v, query_start=60, **call), fullgraph=True, backend="aot_eager")
+        with torch.no_grad():
+            assert torch.equal(compiled(q, k, v), f(q, k, v, query_start=60, **same))
+        cache = api().quantized_cache(1, 2, 200, 64)
+        api().quantized_cache_write(cache, k, v)
+        few = q[:, :, :2]
+        assert torch.equal(api().quantized_cache_attention(few, cache, query_start=150, **call),
+                           api().quantized_cache_attention(few, cache, query_start=150, **same))
