@@ -268,7 +268,7 @@ KFA_API int kfa_window_backward(const kfa_tensor* q, const kfa_tensor* k, const 
  * group with a value that is not finite gets a NaN scale.  Rows that fall outside [0, capacity), and rows at or behind
  * a sequence's length, are not written.  start_b is `start` or, where `starts` is given, starts[b] (int32 [B], device).
  * kfa_cache_read writes the values of the rows start_b + r to k, v [B,H,n,D] (rounded once); rows outside the cache
- * read as zeros.
+ * read as zeros.  What is written must not overlap: the four tensors, and each tensor's rows, lie apart in memory.
  *
  * kfa_cache_attention is the attention of q [B,Hq,Sq,D] (unit channel stride, 16-byte addressable rows) to such a
  * cache, D = 64 or 128: query row r stands at position start_b + r and sees the keys c <= start_b + r, and, with

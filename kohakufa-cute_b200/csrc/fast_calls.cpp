@@ -94,6 +94,25 @@ bool addressable(const Tensor& t) {
     return true;
 }
 
+// Whether two elements may share memory: an axis whose stride does not clear what the axes of smaller strides reach.
+bool may_overlap(const Tensor& t) {
+    int64_t reach = 0, done = -1;
+    for (int n = 0; n < t.dim(); ++n) {  // in the order of their strides, equal ones of two axes are an overlap
+        int64_t next = INT64_MAX, size = 1;
+        for (int i = 0; i < t.dim(); ++i) {
+            if (t.size(i) == 1 || t.stride(i) > next || t.stride(i) <= done) continue;
+            if (t.stride(i) == next) return true;
+            next = t.stride(i);
+            size = t.size(i);
+        }
+        if (size == 1) break;
+        if (next <= reach) return true;
+        reach += next * (size - 1);
+        done = next;
+    }
+    return false;
+}
+
 bool differentiated(std::initializer_list<const Tensor*> tensors) {
     if (!at::GradMode::is_enabled()) return false;
     for (const Tensor* t : tensors)
@@ -324,9 +343,7 @@ PyObject* py_cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
             k.size(1) != kc.size(1) || k.size(3) != cache.channels)
             throw Unserved();
         for (const Tensor* t : {cache.k_codes, cache.k_params, cache.v_codes, cache.v_params})
-            if (!t->is_contiguous())
-                for (int64_t stride : t->strides())
-                    if (stride == 0) throw Unserved();
+            if (!t->is_contiguous() && may_overlap(*t)) throw Unserved();
         if (differentiated({&k, &v}) || !addressable(k) || !addressable(v)) throw Unserved();
         const Positions at = positions(args[3], kc);
         if (!at.each && at.all + k.size(2) > kc.size(2)) throw Unserved();

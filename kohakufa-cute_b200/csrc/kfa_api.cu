@@ -1375,6 +1375,8 @@ int kfa_cache_write(const kfa_tensor* k, const kfa_tensor* v, kfa_tensor* k_code
     kfa::CacheCall p;
     if (int e = fill_cache_call(p, k, v, k_codes, k_params, v_codes, v_params, starts, start)) return e;
     if (int e = check_positions(lengths, p.B, "lengths")) return e;
+    if (k_codes->data == v_codes->data || k_params->data == v_params->data)
+        return fail(KFA_INVALID_ARGUMENT, "quantized cache: keys and values overlap in memory");
     p.lengths = lengths ? static_cast<const int32_t*>(lengths->data) : nullptr;
     p.in[0] = k->data;
     p.in[1] = v->data;

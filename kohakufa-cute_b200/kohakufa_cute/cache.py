@@ -57,6 +57,18 @@ def _check_cache(name, cache):
         raise ValueError("This build of CuTe attention requires an sm_100 (B200) device.")
 
 
+def _may_overlap(t):
+    """Whether two elements of ``t`` may share memory: an axis whose stride does not clear what the axes of smaller
+    strides reach.  An axis of one element has no stride that matters."""
+    reach = 0
+    for stride, size in sorted(zip(t.stride(), t.shape)):
+        if size > 1:
+            if stride <= reach:
+                return True
+            reach += stride * (size - 1)
+    return False
+
+
 def _positions(name, what, value, batch, device):
     """``(tensor, int)`` of a position argument: one int for all sequences or an int32 ``[batch]`` tensor."""
     if isinstance(value, torch.Tensor):
@@ -133,7 +145,7 @@ def quantized_cache_write(cache, k, v, *, start=0, lengths=None):
         raise ValueError(f"{name}: K and V must have the cache's device and type.")
     if (k.shape[0], k.shape[1], k.shape[3]) != (kc.shape[0], kc.shape[1], 2 * kc.shape[3]):
         raise ValueError(f"{name}: K and V must match the cache's batch, heads and channels.")
-    if any(0 in t.stride() and not t.is_contiguous() for t in cache):
+    if any(not t.is_contiguous() and _may_overlap(t) for t in cache):
         raise ValueError(f"{name}: the cache's rows overlap in memory (an expanded view can only be read).")
     _no_gradient(name, k, v)
     starts, at = _positions(name, "start", start, kc.shape[0], kc.device)

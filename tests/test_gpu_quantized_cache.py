@@ -567,3 +567,29 @@ def test_dense_rows_off_a_16_byte_boundary_are_taken():
     few = q[:, :, :2].contiguous()
     want = api().quantized_cache_attention(few, cache, query_start=20)
     assert torch.equal(want, api().quantized_cache_attention(shifted(few), cache, query_start=20))
+
+
+def test_caches_whose_rows_share_memory_are_not_written():
+    """An overlap by any strides, and keys that are the values' own memory, are refused; a stride of an axis of one
+    element says nothing."""
+    k = rows(2, 2, 5, 64, dtype=torch.bfloat16, seed=64)
+    plain = api().quantized_cache(2, 2, 40, 64)
+    store = torch.zeros(2 * 2 * 40 * 32, dtype=torch.uint8, device="cuda")
+    sliding = store.as_strided((2, 2, 40, 32), (32 * 40, 32 * 20, 32, 1))  # the second head starts inside the first
+    pairs = torch.zeros(2 * 2 * 40 * 2, dtype=torch.bfloat16, device="cuda")
+    behind = pairs.as_strided((2, 2, 40, 1, 2), (160, 80, 0, 2, 1))        # every token the same pair
+    for bad in (plain._replace(k_codes=sliding), plain._replace(v_codes=sliding), plain._replace(k_params=behind),
+                plain._replace(v_codes=plain.k_codes), plain._replace(v_params=plain.k_params)):
+        with pytest.raises(ValueError, match="overlap"):
+            api().quantized_cache_write(bad, k, k)
+    assert not store.any() and not pairs.any() and not any(t.any() for t in plain)
+    one = api().quantized_cache(1, 2, 40, 64)
+    loose = api().QuantizedCache(*(t.as_strided(t.shape, (0, *t.stride()[1:])) for t in one))
+    api().quantized_cache_write(loose, k[:1], k[:1], start=3)
+    want = api().quantized_cache(1, 2, 40, 64)
+    api().quantized_cache_write(want, k[:1], k[:1], start=3)
+    assert all(torch.equal(a, b) for a, b in zip(one, want))
+    swapped = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in plain]  # [B, capacity, H, ...] in memory
+    api().quantized_cache_write(api().QuantizedCache(*swapped), k, k, start=3)
+    api().quantized_cache_write(plain, k, k, start=3)
+    assert all(torch.equal(a, b) for a, b in zip(swapped, plain))

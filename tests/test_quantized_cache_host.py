@@ -52,3 +52,23 @@ def test_gradients_are_refused():
         qc._no_gradient("f", torch.zeros(1, requires_grad=True))
     with torch.no_grad():
         qc._no_gradient("f", torch.zeros(1, requires_grad=True))
+
+
+def test_overlaps_are_found_by_their_strides():
+    """Against enumeration: what shares memory is found, and ordinary layouts are not suspected."""
+    import itertools
+
+    base = torch.zeros(4000)
+    for sizes in ((2, 3, 4), (1, 5, 2), (3, 1, 1), (2, 2, 2, 2, 2)):
+        for strides in itertools.product((0, 1, 2, 3, 5, 8, 24), repeat=min(len(sizes), 3)):
+            strides = strides + tuple(30 * 2**i for i in range(len(sizes) - 3))
+            t = base.as_strided(sizes, strides)
+            places = {sum(i * s for i, s in zip(at, strides)) for at in itertools.product(*map(range, sizes))}
+            if len(places) < t.numel():
+                assert qc._may_overlap(t), (sizes, strides)
+    whole = torch.zeros(3, 4, 5, 8)
+    for t in (whole, whole.transpose(1, 2), whole[1:, ::2, 1:3], whole.permute(3, 1, 0, 2), whole[..., :1], whole[:1].expand(1, 4, 5, 8),
+              torch.zeros(1, 4, 5, 8).as_strided((1, 4, 5, 8), (0, 40, 8, 1))):
+        assert not qc._may_overlap(t)
+    for t in (whole[:1].expand(2, 4, 5, 8), whole.as_strided((2, 4, 5, 8), (20, 40, 8, 1)), whole.as_strided((3, 4), (4, 2))):
+        assert qc._may_overlap(t)
