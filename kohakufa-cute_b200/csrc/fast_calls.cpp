@@ -344,7 +344,7 @@ PyObject* py_cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
             throw Unserved();
         for (const Tensor* t : {cache.k_codes, cache.k_params, cache.v_codes, cache.v_params})
             if (!t->is_contiguous() && may_overlap(*t)) throw Unserved();
-        if (differentiated({&k, &v}) || !addressable(k) || !addressable(v)) throw Unserved();
+        if (differentiated({&k, &v, cache.k_params, cache.v_params}) || !addressable(k) || !addressable(v)) throw Unserved();
         const Positions at = positions(args[3], kc);
         if (!at.each && at.all + k.size(2) > kc.size(2)) throw Unserved();
         std::optional<Tensor> lengths;
@@ -367,6 +367,7 @@ PyObject* py_cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (n != 3) throw Unserved();
         const Cache cache(args[0]);
         const Tensor& kc = *cache.k_codes;
+        if (differentiated({cache.k_params, cache.v_params})) throw Unserved();
         const Positions at = positions(args[1], kc);
         if (args[2] == Py_None && at.each) throw Unserved();
         const int64_t length = args[2] == Py_None ? kc.size(2) - at.all : integer(args[2]);
@@ -399,7 +400,7 @@ PyObject* py_cache_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
             throw Unserved();
         const int64_t window = args[3] == Py_None ? 0 : integer(args[3]), sinks = integer(args[4]);
         if (args[3] == Py_None ? sinks != 0 : window < 1 || sinks < 0) throw Unserved();
-        if (differentiated({&q}) || !addressable(q)) throw Unserved();
+        if (differentiated({&q, cache.k_params, cache.v_params}) || !addressable(q)) throw Unserved();
         const Positions at = positions(args[2], q);
         const double scale = scale_of(args[5], cache.channels);
         const c10::cuda::CUDAGuard guard(q.device());

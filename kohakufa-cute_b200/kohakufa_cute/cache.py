@@ -147,7 +147,7 @@ def quantized_cache_write(cache, k, v, *, start=0, lengths=None):
         raise ValueError(f"{name}: K and V must match the cache's batch, heads and channels.")
     if any(not t.is_contiguous() and _may_overlap(t) for t in cache):
         raise ValueError(f"{name}: the cache's rows overlap in memory (an expanded view can only be read).")
-    _no_gradient(name, k, v)
+    _no_gradient(name, k, v, kp, cache[3])
     starts, at = _positions(name, "start", start, kc.shape[0], kc.device)
     if starts is None and at + k.shape[2] > kc.shape[2]:
         raise ValueError(f"{name}: rows {at}..{at + k.shape[2]} do not fit a cache of {kc.shape[2]} tokens.")
@@ -172,6 +172,7 @@ def quantized_cache_read(cache, *, start=0, length=None):
     name = "quantized_cache_read"
     _check_cache(name, cache)
     kc = cache[0]
+    _no_gradient(name, cache[1], cache[3])
     starts, at = _positions(name, "start", start, kc.shape[0], kc.device)
     if length is None:
         if starts is not None:
@@ -210,7 +211,7 @@ def quantized_cache_attention(q, cache, *, query_start, window=None, sinks=0, sc
         raise ValueError(f"{name}: Q must match the cache's batch and channels, its heads a multiple of the cache's.")
     if q.shape[3] not in (64, 128):
         raise ValueError(f"{name}: head dimensions 64 and 128 are supported.")
-    _no_gradient(name, q)
+    _no_gradient(name, q, kp, cache[3])
     if window is None and sinks != 0:
         raise ValueError(f"{name}: sinks need a window.")
     starts, at = _window_arguments(name, q.shape[0], q.device, 1 if window is None else window, sinks, query_start)

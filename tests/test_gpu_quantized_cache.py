@@ -593,3 +593,20 @@ def test_caches_whose_rows_share_memory_are_not_written():
     api().quantized_cache_write(api().QuantizedCache(*swapped), k, k, start=3)
     api().quantized_cache_write(plain, k, k, start=3)
     assert all(torch.equal(a, b) for a, b in zip(swapped, plain))
+
+
+def test_params_that_require_gradients_are_refused():
+    """The calls record nothing, so that a gradient with respect to scales and zeros would be missing without a word."""
+    plain = filled(1, 2, 30, 64, torch.bfloat16, seed=65)
+    q = rows(1, 2, 1, 64, dtype=torch.bfloat16, seed=66)
+    for name in ("k_params", "v_params"):
+        cache = plain._replace(**{name: getattr(plain, name).clone().requires_grad_()})
+        calls = (lambda: api().quantized_cache_read(cache), lambda: api().quantized_cache_write(cache, q, q),
+                 lambda: api().quantized_cache_attention(q, cache, query_start=29))
+        for call in calls:
+            with pytest.raises(ValueError, match="inference only"):
+                call()
+        with torch.no_grad():
+            assert all(torch.equal(a, b) for a, b in zip(calls[0](), api().quantized_cache_read(plain)))
+            calls[1]()
+            assert torch.equal(calls[2](), calls[2]())
