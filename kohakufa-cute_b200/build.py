@@ -87,26 +87,40 @@ def build(force=False, verbose=True, phases=False):
     return lib
 
 
+def _compile_module(target, cmd, stamp, digest, force, verbose):
+    """Compiles an optional module unless it is there as `digest` describes it; ``None``, and no module of other sources or
+    another torch left behind, where that fails."""
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    if force or not os.path.exists(target) or not os.path.exists(stamp) or open(stamp).read() != digest:
+        if verbose:
+            print(" ".join(cmd + ["-o", target]), flush=True)
+        try:
+            subprocess.check_call(cmd + ["-o", target])
+        except (OSError, subprocess.CalledProcessError) as error:
+            return _left_out(target, error)
+        with open(stamp, "w") as f:
+            f.write(digest)
+    return target
+
+
+def _left_out(target, reason):
+    print(f"left out: {target} ({reason})", flush=True)
+    if os.path.exists(target):
+        os.remove(target)
+    return None
+
+
 def build_records(force=False, verbose=True):
     """The optional CPython module that packs tensor records (``csrc/fast_records.c``), or ``None`` without Python's
-    headers: the binding then packs them itself, with the same results."""
+    headers or a compiler for them: the binding then packs them itself, with the same results."""
     include = sysconfig.get_paths()["include"]
     source = os.path.join(CSRC, "fast_records.c")
     header = os.path.join(os.path.dirname(HERE), "include", "kfa.h")
     target = os.path.join(OUT_DIR, "_fast_records" + sysconfig.get_config_var("EXT_SUFFIX"))
     if not os.path.exists(os.path.join(include, "Python.h")):
-        return None
+        return _left_out(target, "no Python.h")
     cmd = [os.environ.get("CC", "gcc"), "-O2", "-std=c11", "-Wall", "-Wextra", "-shared", "-fPIC", "-I", include, source]
-    os.makedirs(OBJ_DIR, exist_ok=True)
-    stamp = os.path.join(OBJ_DIR, "fast_records.sha")
-    digest = _digest([source, header], cmd)
-    if force or not os.path.exists(target) or not os.path.exists(stamp) or open(stamp).read() != digest:
-        if verbose:
-            print(" ".join(cmd + ["-o", target]), flush=True)
-        subprocess.check_call(cmd + ["-o", target])
-        with open(stamp, "w") as f:
-            f.write(digest)
-    return target
+    return _compile_module(target, cmd, os.path.join(OBJ_DIR, "fast_records.sha"), _digest([source, header], cmd), force, verbose)
 
 
 def build_calls(force=False, verbose=True):
@@ -117,34 +131,22 @@ def build_calls(force=False, verbose=True):
     spec = importlib.util.find_spec("torch")
     home = os.path.dirname(spec.origin) if spec and spec.origin else ""
     cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(shutil.which(_nvcc()) or _nvcc()))), "include")
+    target = os.path.join(OUT_DIR, "_fast_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
+    version = os.path.join(home, "version.py")
     needed = (os.path.join(include, "Python.h"), os.path.join(home, "include", "c10", "cuda", "CUDAStream.h"),
-              os.path.join(cuda, "cuda_runtime_api.h"))
-    if not all(os.path.exists(path) for path in needed):
-        return None
+              os.path.join(cuda, "cuda_runtime_api.h"), version)
+    missing = [path for path in needed if not os.path.exists(path)]
+    if missing:
+        return _left_out(target, f"no {missing[0]}")
     source = os.path.join(CSRC, "fast_calls.cpp")
     header = os.path.join(os.path.dirname(HERE), "include", "kfa.h")
-    target = os.path.join(OUT_DIR, "_fast_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
+    # (the module belongs to one torch: its version is part of the stamp)
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-Wall", "-shared", "-fPIC", "-fvisibility=hidden", "-I", include]
     for path in (os.path.join(home, "include"), os.path.join(home, "include", "torch", "csrc", "api", "include"), cuda):
         cmd += ["-isystem", path]
     cmd += [source, "-L", os.path.join(home, "lib"), "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda"]
-    os.makedirs(OBJ_DIR, exist_ok=True)
-    stamp = os.path.join(OBJ_DIR, "fast_calls.sha")
-    # (the module belongs to one torch: its version is part of the stamp)
-    digest = _digest([source, header, os.path.join(home, "version.py")], cmd)
-    if force or not os.path.exists(target) or not os.path.exists(stamp) or open(stamp).read() != digest:
-        if verbose:
-            print(" ".join(cmd + ["-o", target]), flush=True)
-        try:
-            subprocess.check_call(cmd + ["-o", target])
-        except (OSError, subprocess.CalledProcessError) as error:
-            print(f"left out: {target} ({error})", flush=True)
-            if os.path.exists(target):  # (of other sources or another torch)
-                os.remove(target)
-            return None
-        with open(stamp, "w") as f:
-            f.write(digest)
-    return target
+    return _compile_module(target, cmd, os.path.join(OBJ_DIR, "fast_calls.sha"), _digest([source, header, version], cmd), force,
+                           verbose)
 
 
 if __name__ == "__main__":
