@@ -11,6 +11,7 @@ how many cycles each role of one CTA spends in each phase of its loop (see ``csr
 import hashlib
 import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -140,8 +141,13 @@ def build_calls(force=False, verbose=True):
         return _left_out(target, f"no {missing[0]}")
     source = os.path.join(CSRC, "fast_calls.cpp")
     header = os.path.join(os.path.dirname(HERE), "include", "kfa.h")
-    # (the module belongs to one torch: its version is part of the stamp)
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-Wall", "-shared", "-fPIC", "-fvisibility=hidden", "-I", include]
+    # the module belongs to one torch, whose version it carries: the binding uses it with no other
+    with open(version) as f:
+        torch_version = re.search(r"""^__version__ = ['"]([^'"]+)""", f.read(), re.MULTILINE)
+    if torch_version is None:
+        return _left_out(target, "torch has no version")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-Wall", "-shared", "-fPIC", "-fvisibility=hidden", "-I", include,
+           f'-DKFA_TORCH_VERSION="{torch_version.group(1)}"']
     for path in (os.path.join(home, "include"), os.path.join(home, "include", "torch", "csrc", "api", "include"), cuda):
         cmd += ["-isystem", path]
     cmd += [source, "-L", os.path.join(home, "lib"), "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda"]

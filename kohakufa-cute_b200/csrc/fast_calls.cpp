@@ -12,6 +12,7 @@
 //   cache_write(cache, k, v, start, lengths)                          -> True or None
 //   cache_read(cache, start, length)                                  -> (K, V) or None
 //   cache_attention(q, cache, query_start, window, sinks, scale)      -> O or None
+//   torch_version                  of the torch whose headers it was built with, the only one it may be used with
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -471,4 +472,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast_calls", nullptr, -1, methods
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__fast_calls() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__fast_calls() {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "torch_version", KFA_TORCH_VERSION) < 0) Py_CLEAR(m);
+    return m;
+}

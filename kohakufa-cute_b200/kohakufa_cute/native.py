@@ -21,10 +21,17 @@ try:  # optional: packs tensor records in C (build.py leaves it out where Python
     from . import _fast_records
 except ImportError:
     _fast_records = None
+def _of_this_torch(module):
+    """``module`` if it was built with the running torch's headers, else ``None``: another's objects may be laid out
+    differently, also where all symbols resolve."""
+    return module if module is not None and getattr(module, "torch_version", None) == str(torch.__version__) else None
+
+
 try:  # optional: plain window and cache calls in one step (build.py leaves it out where torch's headers are missing)
-    from . import _fast_calls as fast
+    from . import _fast_calls
 except ImportError:
-    fast = None
+    _fast_calls = None
+fast = _of_this_torch(_fast_calls)
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIBRARY_PATH = os.path.join(_HERE, "libkfa.so")

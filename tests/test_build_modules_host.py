@@ -1,10 +1,14 @@
-"""The optional host modules: left out where they cannot be built, never in the way."""
+"""The optional host modules: left out where they cannot be built or belong to another torch, never in the way."""
 
 import importlib.util
 import os
 import subprocess
+import types
 
 import pytest
+import torch
+
+from kohakufa_cute import native
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -49,3 +53,12 @@ def test_missing_headers_leave_a_module_out(build, monkeypatch, step, name):
     monkeypatch.setattr(build.os.path, "exists", lambda p: not str(p).endswith("Python.h") and exists(p))
     monkeypatch.setattr(build.subprocess, "check_call", lambda *a, **k: pytest.fail("compiled without headers"))
     assert getattr(build, step)(verbose=False) is None and not exists(path)
+
+
+def test_a_module_of_another_torch_is_not_used():
+    mine = types.SimpleNamespace(torch_version=str(torch.__version__))
+    assert native._of_this_torch(mine) is mine
+    for other in (None, types.SimpleNamespace(), types.SimpleNamespace(torch_version="1.0.0")):
+        assert native._of_this_torch(other) is None
+    if native._fast_calls is not None:
+        assert native.fast is native._fast_calls and native.fast.torch_version == str(torch.__version__)
