@@ -3,19 +3,20 @@
 // beyond the head with zeros, which add nothing to either product, and the tiled store drops them again),
 // FP16/BF16, causal and/or boolean masks, grouped-query heads.
 //
-// One CTA owns 256 query rows of one (batch, query head) as two 128-row tiles (windowed calls: 128 as one) and walks
-// the 128-key tiles they can see.  Warp roles (384 threads):
+// One CTA owns 256 query rows of one (batch, query head) as two 128-row tiles and walks the 128-key tiles they can see.
+// Warp roles (384 threads):
 //   warps 0-3  softmax of query tile 0   (thread i <-> TMEM lane i <-> query row i)
 //   warps 4-7  softmax of query tile 1
 //   warp  8    issues every tcgen05.mma (one elected lane), owns the TMEM allocation
 //   warp  9    TMA loader (one elected lane); warps 10-11 idle (they complete the warpgroup so
 //              that registers can be moved from it to the softmax warpgroups)
-// Tensor memory (512 columns): S0 | S1 | O0 | O1, 128 columns each.  The 16-bit
-// probabilities overwrite the first 64 columns of their score tile and feed the second
+// Tensor memory (512 columns): S0 | S1 | O0 | O1, 128 columns each.  Windowed calls: one tile of 128 rows, 256 threads
+// (warps 0-3 softmax, 4 products, 5 loader, 6-7 idle), S | O in 256 columns, and two such CTAs per SM.
+// The 16-bit probabilities overwrite the first 64 columns of their score tile and feed the second
 // product straight from tensor memory; they are handed over in two halves of 64 keys, so
 // the first half of P*V runs while the second half of the exponentials is formed.  While
-// one tile's softmax runs, the tensor core works on the other tile, and K/V tiles are
-// shared by both.  Block-wise callers (one block of a longer key sequence per call) get
+// one tile's softmax runs, the tensor core works on the other tile (of the other CTA in windowed calls), and K/V tiles
+// are shared by both tiles of a CTA.  Block-wise callers (one block of a longer key sequence per call) get
 // the tile folded into a running FP32 state instead of a normalised output.
 //
 // Arithmetic (reference behaviour: src/kohakufa_cute/blackwell_pipeline.py:141-209,
@@ -101,9 +102,9 @@ __device__ __forceinline__ int key_tile_state(const AttnParams& p, int b, int h,
 }
 
 // MASKED = false is the instantiation for calls without a mask (the flag is cleared at compile time).
-// WINDOW is the instantiation for sliding-window calls (window.cuh; neither a mask nor `causal` then): a query tile
-// walks the key tiles of the sinks and of its window, two tiles of a CTA need not see the same ones, and positions
-// come from device memory where the call gives one per sequence.  With `key_splits` a cluster of CTAs shares a tile's keys.
+// WINDOW is the instantiation for sliding-window calls (window.cuh; neither a mask nor `causal` then): the query tile
+// walks the key tiles of the sinks and of its window, and positions come from device memory where the call gives one per
+// sequence.  With `key_splits` a cluster of CTAs shares a tile's keys.
 template <int D, bool BF16, bool MASKED, bool WINDOW>
 __global__ void __launch_bounds__(threads_of(WINDOW ? 1 : 2), WINDOW ? 2 : 1)
     pipeline_forward(const __grid_constant__ FwdMaps maps, AttnParams p) {
@@ -113,8 +114,8 @@ __global__ void __launch_bounds__(threads_of(WINDOW ? 1 : 2), WINDOW ? 2 : 1)
     using Cfg = FwdCfg<D, kTiles>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* sQ = smem;                          // two query tiles
-    uint8_t* sKV = smem + kTiles * Cfg::kTileBytes;   // ring of K/V tiles
+    uint8_t* sQ = smem;                              // the query tiles
+    uint8_t* sKV = smem + kTiles * Cfg::kTileBytes;  // ring of K/V tiles
     Shared& sh = *reinterpret_cast<Shared*>(sKV + Cfg::kStages * Cfg::kTileBytes);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -136,12 +137,12 @@ __global__ void __launch_bounds__(threads_of(WINDOW ? 1 : 2), WINDOW ? 2 : 1)
     const int kvh = h / p.group;
     const int q0 = qblk * kTiles * kTileQ;
 
-    // key tiles each query tile may see: those below n_t[t]; in a windowed call the ones its `wt` names (n_t[t] is
-    // the end of them) and, for the CTA, their union `both`
+    // key tiles each query tile may see: those below n_t[t]; in a windowed call the ones that `seen` names (n_t[0] is
+    // the end of them)
     int n_t[2];
     const int64_t start = WINDOW ? window_start(p, b) : 0;
-    WindowTiles wt[2] = {{0, 0, 0}, {0, 0, 0}}, both = {0, 0, 0};
-    int lo_t[2] = {0, 0}, hi_t[2] = {0, 0};  // keys some row of the tile sees, apart from sinks below lo_t
+    WindowTiles seen = {0, 0, 0};
+    int seen_lo = 0, seen_hi = 0;  // keys some row of the tile sees, apart from sinks below seen_lo
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         const int row_lo = q0 + t * kTileQ;
@@ -149,11 +150,11 @@ __global__ void __launch_bounds__(threads_of(WINDOW ? 1 : 2), WINDOW ? 2 : 1)
             n_t[t] = 0;
         } else if (WINDOW) {
             const int row_hi = min(p.Sq, row_lo + kTileQ);
-            wt[t] = window_key_tiles(start, row_lo, row_hi, p.window, p.sinks, p.Sk);
-            if (splits > 1) wt[t] = window_piece(wt[t], piece, splits);
-            lo_t[t] = window_span(start, row_lo, p.window, p.Sk).lo;
-            hi_t[t] = window_span(start, row_hi - 1, p.window, p.Sk).hi;
-            n_t[t] = wt[t].end;
+            seen = window_key_tiles(start, row_lo, row_hi, p.window, p.sinks, p.Sk);
+            if (splits > 1) seen = window_piece(seen, piece, splits);
+            seen_lo = window_span(start, row_lo, p.window, p.Sk).lo;
+            seen_hi = window_span(start, row_hi - 1, p.window, p.Sk).hi;
+            n_t[t] = seen.end;
         } else {
             const int row_hi = min(p.Sq, row_lo + kTileQ);
             const int k_hi = p.causal ? min(p.Sk, row_hi) : p.Sk;
@@ -161,14 +162,6 @@ __global__ void __launch_bounds__(threads_of(WINDOW ? 1 : 2), WINDOW ? 2 : 1)
         }
     }
     const int n_max = max(n_t[0], n_t[1]);
-    if (WINDOW) {
-        const bool some0 = wt[0].first < wt[0].end, some1 = wt[1].first < wt[1].end;
-        both.sink_end = max(wt[0].sink_end, wt[1].sink_end);
-        both.end = n_max;
-        both.first = some0 ? (some1 ? min(wt[0].first, wt[1].first) : wt[0].first) : (some1 ? wt[1].first : n_max);
-        both.first = max(both.first, both.sink_end);
-    }
-    const int cta_hi = max(hi_t[0], hi_t[1]);
 
     if (threadIdx.x == 0) {
         sh.abort_word = *reinterpret_cast<volatile int*>(p.abort_flag) != 0 ? 90 : 0;  // 90: an earlier CTA gave up
@@ -198,20 +191,19 @@ __global__ void __launch_bounds__(threads_of(WINDOW ? 1 : 2), WINDOW ? 2 : 1)
     const uint8_t* states = sh.tile_state;
     const bool masked_call = p.has_mask != 0;
     auto state_of = [&](int j) -> int { return masked_call ? states[j] : 2; };
-    // the CTA's walk over its key tiles, and which of them query tile t sees
+    // the CTA's walk over its key tiles; query tile t sees those below n_t[t]
     auto first_tile = [&]() -> int {
-        if (WINDOW) return both.begin();
+        if (WINDOW) return seen.begin();
         int j = 0;
         while (j < n_max && state_of(j) == 0) ++j;
         return j;
     };
     auto next_tile = [&](int j) -> int {
-        if (WINDOW) return both.next(j);
+        if (WINDOW) return seen.next(j);
         ++j;
         while (j < n_max && state_of(j) == 0) ++j;
         return j;
     };
-    auto sees = [&](int t, int j) -> bool { return WINDOW ? wt[t].has(j) : j < n_t[t]; };
     volatile int* abort_word = &sh.abort_word;
 
     const bool dead = sh.abort_word != 0;  // set before the barrier above: skip straight to the tear-down
@@ -282,25 +274,24 @@ __global__ void __launch_bounds__(threads_of(WINDOW ? 1 : 2), WINDOW ? 2 : 1)
                     umma_ts(tmem + kColO + t * 128, tmem + t * 128 + kk * 8, umma_desc_advance(v_desc, b0 + kk * 2048),
                             idesc_o, accumulate || kk > 0);
             };
-            // The same in a windowed call: steps of 16 keys that no row of the tile sees are left out.
-            bool begun[2] = {false, false};  // the tile's accumulator holds something
-            auto issue_o_window = [&](int t, int slot, int half, int j) {
+            // The same in a windowed call (of its one tile): steps of 16 keys that no row sees are left out.
+            bool begun = false;  // the accumulator holds something
+            auto issue_o_window = [&](int slot, int half, int j) {
                 const uint32_t b0 = slot * Cfg::kTileBytes;
 #pragma unroll
                 for (int kk = half * (kTileK / 32); kk < (half + 1) * (kTileK / 32); ++kk) {
                     const int key = j * kTileK + kk * 16;
-                    if (key >= hi_t[t] || (key + 16 <= lo_t[t] && key >= p.sinks)) continue;
-                    umma_ts(tmem + kColO + t * 128, tmem + t * 128 + kk * 8, umma_desc_advance(v_desc, b0 + kk * 2048),
-                            idesc_o, begun[t]);
-                    begun[t] = true;
+                    if (key >= seen_hi || (key + 16 <= seen_lo && key >= p.sinks)) continue;
+                    umma_ts(tmem + kColO, tmem + kk * 8, umma_desc_advance(v_desc, b0 + kk * 2048), idesc_o, begun);
+                    begun = true;
                 }
             };
             // Values behind the last key that the CTA's rows see may never have been written (the free end of a
             // cache): their probabilities are zero, but zero times a NaN is not.  The rest of the 16-key step the
             // last key falls into is overwritten with zeros (at most 15 rows; rows beyond Sk arrive as zeros).
             auto clear_unseen = [&](int slot, int j) {
-                const int r0 = cta_hi - j * kTileK;
-                if (r0 <= 0 || r0 >= kTileK || cta_hi >= p.Sk || r0 % 16 == 0) return;
+                const int r0 = seen_hi - j * kTileK;
+                if (r0 <= 0 || r0 >= kTileK || seen_hi >= p.Sk || r0 % 16 == 0) return;
                 uint8_t* tile = sKV + slot * Cfg::kTileBytes;
                 for (int r = r0; r % 16 != 0; ++r)
                     for (int c = 0; c < Cfg::kChunks; ++c)
@@ -320,7 +311,7 @@ __global__ void __launch_bounds__(threads_of(WINDOW ? 1 : 2), WINDOW ? 2 : 1)
                 if (ok) {
                     tc_fence_after();
                     for (int t = 0; t < kTiles; ++t)
-                        if (sees(t, j)) {
+                        if (j < n_t[t]) {
                             issue_s(t, slot);
                             umma_commit(&sh.s_ready[t]);
                         }
@@ -344,26 +335,23 @@ __global__ void __launch_bounds__(threads_of(WINDOW ? 1 : 2), WINDOW ? 2 : 1)
                 bool k_waited = false;
                 if (WINDOW && ok) clear_unseen(v_slot, j);
                 for (int t = 0; t < kTiles && ok; ++t) {
-                    const bool now = sees(t, j), then = sees(t, jn);
-                    if (!now && !(WINDOW && then)) continue;
-                    if (now) {
-                        ok = mbar_wait(&sh.p_half[t][0], iter[t] & 1, abort_word, 23 + t);
-                        if (!ok) break;
-                        PH(1);
-                        tc_fence_after();
-                        if (WINDOW) issue_o_window(t, v_slot, 0, j);
-                        else issue_o(t, v_slot, 0, iter[t] > 0);
-                        PH(2);
-                        ok = mbar_wait(&sh.p_half[t][1], iter[t] & 1, abort_word, 26 + t);
-                        if (!ok) break;
-                        PH(1);
-                        tc_fence_after();
-                        if (WINDOW) issue_o_window(t, v_slot, 1, j);
-                        else issue_o(t, v_slot, 1, true);
-                        PH(2);
-                        ++iter[t];
-                    }
-                    if (then) {
+                    if (j >= n_t[t]) continue;
+                    ok = mbar_wait(&sh.p_half[t][0], iter[t] & 1, abort_word, 23 + t);
+                    if (!ok) break;
+                    PH(1);
+                    tc_fence_after();
+                    if (WINDOW) issue_o_window(v_slot, 0, j);
+                    else issue_o(t, v_slot, 0, iter[t] > 0);
+                    PH(2);
+                    ok = mbar_wait(&sh.p_half[t][1], iter[t] & 1, abort_word, 26 + t);
+                    if (!ok) break;
+                    PH(1);
+                    tc_fence_after();
+                    if (WINDOW) issue_o_window(v_slot, 1, j);
+                    else issue_o(t, v_slot, 1, true);
+                    PH(2);
+                    ++iter[t];
+                    if (jn < n_t[t]) {
                         if (!k_waited) {
                             ok = mbar_wait(&sh.kv_full[k_slot], k_par, abort_word, 25);
                             if (!ok) break;
@@ -373,12 +361,9 @@ __global__ void __launch_bounds__(threads_of(WINDOW ? 1 : 2), WINDOW ? 2 : 1)
                         PH(3);
                         issue_s(t, k_slot);
                     }
-                    // one commit per score tile and one behind the last product; a tile that pauses between the
-                    // sinks and its window gets the next score tile's commit
-                    if (!WINDOW || then || jn >= n_t[t]) umma_commit(&sh.s_ready[t]);
+                    umma_commit(&sh.s_ready[t]);  // one per score tile, and one behind the last product
                     PH(4);
                 }
-                if (WINDOW && ok && k_slot >= 0 && !k_waited) ok = mbar_wait(&sh.kv_full[k_slot], k_par, abort_word, 25);
                 if (!ok) break;
                 umma_commit(&sh.kv_empty[v_slot]);
                 if (k_slot >= 0) umma_commit(&sh.kv_empty[k_slot]);
@@ -411,11 +396,10 @@ __global__ void __launch_bounds__(threads_of(WINDOW ? 1 : 2), WINDOW ? 2 : 1)
         int iter = 0;
         bool ok = true;
         PH_DECL;
-        // a windowed call: this row's window, and the tile's own walk
+        // a windowed call: this row's window
         const WindowSpan span = WINDOW ? window_span(start, min(row, p.Sq - 1), p.window, p.Sk) : WindowSpan{0, 0};
-        const WindowTiles mine = t == 0 ? wt[0] : wt[1];
         const int n_mine = t == 0 ? n_t[0] : n_t[1];
-        for (int j = WINDOW ? mine.begin() : 0; j < n_mine && ok; j = WINDOW ? mine.next(j) : j + 1) {
+        for (int j = WINDOW ? seen.begin() : 0; j < n_mine && ok; j = WINDOW ? seen.next(j) : j + 1) {
             const int state = state_of(j);
             if (state == 0) continue;
             PH(5);
