@@ -160,7 +160,7 @@ def _no_tangent(name, *tensors):
     """Raises ``ValueError`` for operands with forward-mode tangents: the kernels would drop them."""
     if torch.compiler.is_compiling():
         return
-    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):  # (none outside a dual level)
         raise ValueError(f"{name}: forward-mode differentiation is not supported.")
 
 
