@@ -265,9 +265,10 @@ KFA_API int kfa_window_backward(const kfa_tensor* q, const kfa_tensor* k, const 
  *
  * kfa_cache_write quantises k, v [B,H,n,D] (16-byte addressable rows) into the rows start_b + r, r < lengths[b]
  * (lengths NULL: all n): scale = round16((max - min) / 15), zero = min, code = round_half_even((x - zero) / scale).  A
- * group with a value that is not finite gets a NaN scale.  Rows that fall outside [0, capacity), and rows at or behind
+ * group with a value that is not finite, or whose max - min is beyond FP32, gets a NaN scale.  Rows that fall outside [0, capacity), and rows at or behind
  * a sequence's length, are not written.  start_b is `start` or, where `starts` is given, starts[b] (int32 [B], device).
- * kfa_cache_read writes the values of the rows start_b + r to k, v [B,H,n,D] (rounded once); rows outside the cache
+ * kfa_cache_read writes the values of the rows start_b + r to k, v [B,H,n,D] (rounded once, at most the type's largest
+ * value; attention does not cut them off there); rows outside the cache
  * read as zeros.  What is written must not overlap: the four tensors, and each tensor's rows, lie apart in memory.
  *
  * kfa_cache_attention is the attention of q [B,Hq,Sq,D] (unit channel stride, 16-byte addressable rows) to such a

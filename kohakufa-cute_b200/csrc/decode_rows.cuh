@@ -6,6 +6,8 @@
 // nothing extra and the cache goes from shared memory to registers once:
 //   S^T = K q^T     A = 16 tokens x 16 channels, B = 16 channels x 8 query rows
 //   O^T = V^T P^T   A = 16 channels x 16 tokens, B = 16 tokens x 8 query rows (P^T by two 8x8 register transposes)
+// The probabilities enter the second product in 16 bits, as they do in the other forward kernels (one rounding each, relative
+// to the row's reference; their sum is of the unrounded ones); everything between is FP32.
 // (tcgen05 wants 128 rows of operand A in shared memory: the 4-bit cache would have to be widened into it, 4 x the
 // bytes, and its rows are tokens only in one of the two products.)
 //

@@ -38,7 +38,8 @@ bool decode_forward_supported(const AttnParams& p);
 size_t decode_forward_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D);
 cudaError_t launch_decode_forward(const AttnParams& p, bool bf16, void* workspace, int* launches, cudaStream_t st);
 
-// Windowed forward for at most 16 query rows per K/V head (64 or 128 channels, 16-byte addressable rows): no statistics.
+// Windowed forward for few query rows per K/V head, without statistics (64 or 128 channels, 16-byte addressable rows): up to
+// 16 always, more where window_decode_shape takes it for faster than the tensor-memory forward.
 bool window_decode_shape(const AttnParams& p);
 size_t window_decode_workspace_bytes(const AttnParams& p);
 cudaError_t launch_window_decode(const AttnParams& p, bool bf16, void* workspace, int* launches, cudaStream_t st);

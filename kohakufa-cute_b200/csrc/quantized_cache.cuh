@@ -3,9 +3,11 @@
 // Each token's row of D channels is held in groups of 64 channels.  A group has a scale and a zero in the model's
 // 16-bit type and 64 codes of 4 bits; byte i of a row holds channels 2i (low half) and 2i + 1 (high half):
 //     low = min x, scale = round16((max x - low) / 15), zero = low, code = round_half_even((x - low) / scale), 0..15
-//     value = zero + scale * code          (read back in 16 bits it saturates at the type's largest value)
+//     value = zero + scale * code          (read back in 16 bits it saturates at the type's largest value; attention
+//                                           takes it as it is, in FP32)
 // 36 bytes per group instead of 128.  A group whose values are all equal (or whose scale underflows to zero) has
-// codes 0 and is read back as `low`; a group with a value that is not finite has a NaN scale and reads back as NaN.
+// codes 0 and is read back as `low`; a group with a value that is not finite, or whose max - low is beyond FP32 (BF16 only),
+// has a NaN scale and reads back as NaN.
 #pragma once
 #include "kfa_common.cuh"
 

@@ -183,8 +183,8 @@ def sliding_window_attention(q, k, v, *, window, sinks=0, query_start=0, scale=N
     ``p = query_start + r`` of its key sequence and sees key ``c`` iff ``c <= p`` and (``c > p - window`` or
     ``c < sinks``); a row that sees no key is zero.  ``query_start`` is an int (0: queries and keys start together, as
     in training), or an int32 ``[B]`` CUDA tensor with one position per sequence, read by the kernels (a captured
-    graph can be replayed with new positions; any value is allowed, keys behind a sequence's last position may hold
-    anything).  Differentiable (once, in reverse mode) with respect to Q, K and V when ``query_start`` is an int.
+    graph can be replayed with new positions; any value is allowed).  Keys and values behind a sequence's last position
+    may hold anything; up to there they have to be finite, also where no row sees them.  Differentiable (once, in reverse mode) with respect to Q, K and V when ``query_start`` is an int.
     """
     if native.fast is not None and not torch.compiler.is_compiling():
         out = native.fast.window_attention(q, k, v, window, sinks, query_start, scale)

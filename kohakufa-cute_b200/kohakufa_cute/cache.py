@@ -130,8 +130,9 @@ def quantized_cache_write(cache, k, v, *, start=0, lengths=None):
     Row ``r`` of sequence ``b`` goes to position ``start_b + r``; ``start`` is an int or an int32 ``[B]`` tensor.
     ``lengths`` (int32 ``[B]``) limits each sequence to its first rows (a padded batch of prompts).  Everything else in
     the cache stays as it was: rows at or behind a sequence's length, and rows whose position lies outside the cache
-    (an int ``start`` that would write past the end is refused).  A group of channels with a value that is not finite
-    reads back as NaN.
+    (an int ``start`` that would write past the end is refused).  A group of channels with a value that is not finite, or
+    with values further apart than FP32 holds (near the ends of BF16's range), reads back as NaN.  The cache's tensors,
+    and the rows of each, must not overlap in memory.
     """
     if native.fast is not None and not torch.compiler.is_compiling():
         if native.fast.cache_write(cache, k, v, start, lengths):
@@ -163,8 +164,9 @@ def quantized_cache_write(cache, k, v, *, start=0, lengths=None):
 
 def quantized_cache_read(cache, *, start=0, length=None):
     """``(k, v)``: the values of ``length`` rows of every sequence from position ``start`` (an int or an int32 ``[B]``
-    tensor) on, ``[B, H, length, D]`` in the cache's type, rounded once.  ``length`` defaults to the rest of the cache
-    behind an int ``start``; rows outside the cache (possible with a tensor) read as zeros."""
+    tensor) on, ``[B, H, length, D]`` in the cache's type, rounded once (at most the type's largest value).  ``length``
+    defaults to the rest of the cache behind an int ``start``; rows outside the cache (possible with a tensor) read as
+    zeros.  Inference only."""
     if native.fast is not None and not torch.compiler.is_compiling():
         rows = native.fast.cache_read(cache, start, length)
         if rows is not None:
