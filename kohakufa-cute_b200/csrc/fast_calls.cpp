@@ -359,6 +359,8 @@ PyObject* py_cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
             return cache_write(&rk, &rv, &cache.r[0], &cache.r[1], &cache.r[2], &cache.r[3], at.each ? &rs : nullptr,
                                lengths ? &rl : nullptr, at.all, stream_of(kc));
         });
+        for (const Tensor* t : {cache.k_codes, cache.k_params, cache.v_codes, cache.v_params})
+            if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
         Py_RETURN_TRUE;
     });
 }

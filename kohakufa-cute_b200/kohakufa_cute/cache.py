@@ -160,6 +160,9 @@ def quantized_cache_write(cache, k, v, *, start=0, lengths=None):
         _write_op(k, v, *cache, starts, lengths, at)
     else:
         native.cache_write(k, v, *cache, starts, lengths, at)
+        for t in cache:  # a change in place, for what autograd may have saved (inference tensors keep no count)
+            if not t.is_inference():
+                torch.autograd.graph.increment_version(t)
 
 
 def quantized_cache_read(cache, *, start=0, length=None):

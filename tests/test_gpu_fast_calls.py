@@ -221,3 +221,31 @@ def test_forward_mode_is_refused_both_ways(counted, monkeypatch):
 
     dual()
     without(monkeypatch, dual)
+
+
+def test_writes_count_as_changes_in_place(counted, monkeypatch):
+    """A cache tensor that autograd has saved is known to have changed, as after any in-place operation of torch."""
+    k = rows(1, 2, 3, 64)
+
+    def write():
+        cache = api().quantized_cache(1, 2, 8, 64)
+        before = [t._version for t in cache]
+        x = torch.ones_like(cache.v_params, requires_grad=True)
+        product = (x * cache.v_params).sum()  # saves the values
+        api().quantized_cache_write(cache, k, k)
+        assert all(t._version > n for t, n in zip(cache, before))
+        with pytest.raises(RuntimeError, match="inplace"):
+            product.backward()
+        view = api().QuantizedCache(*(t[:, :, 4:] for t in cache))
+        before = [t._version for t in cache]
+        api().quantized_cache_write(view, k, k)
+        assert all(t._version > n for t, n in zip(cache, before))
+        with torch.inference_mode():  # (tensors that keep no count)
+            held = api().quantized_cache(1, 2, 8, 64)
+            api().quantized_cache_write(held, k, k)
+        assert torch.equal(held.k_codes[:, :, :3], cache.k_codes[:, :, :3])
+
+    served = counted.served
+    write()
+    assert counted.served == served + 3
+    without(monkeypatch, write)
